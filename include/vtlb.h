@@ -402,6 +402,51 @@ int vtlb_batchnorm1d_bwd_f32(vtlb_ctx* ctx, const void* d_g, const void* d_x, in
                              const void* d_batch_mean, const void* d_batch_var, double eps, void* d_dx_or_null,
                              void* d_dgamma_or_null, void* d_dbeta_or_null);
 
+/* ---- token models: embedding, dropout, group norm --------------------------------
+ * No counterpart in the reference's device code; its layers of these kinds are host loops.  All of them run on the
+ * context's compute stream without blocking (but for `check`), allocate nothing outside the context's scratch, and may
+ * be captured: a call under capture takes its workspace from the graph, so graphs and calls may overlap as far as their
+ * own buffers allow.  Sums are taken in a fixed order: the same call gives the same bits.
+ *
+ * Dropout: y_i = x_i / (1 - p) (one f32 product with the rounded 1 / (1 - p)) where r_i >= floor(p * 2^32), else 0
+ * whatever x_i holds; r_i is word i % 4 of the Philox4x32-10 block with key `seed` and counter (i / 4, step), each 64
+ * bits, low words first.  The mask is a function of (seed, step, i) alone and is not stored: the backward pass is given
+ * the seed and step of the forward pass and draws it again.  Every pass wants a step of its own, a captured call
+ * included: a replay repeats the mask it was captured with.  0 <= p <= 1; d_y may be d_x (not overlap it in part). */
+int vtlb_dropout_fwd_f32(vtlb_ctx* ctx, const void* d_x, void* d_y, size_t n, double p, uint64_t seed, uint64_t step);
+int vtlb_dropout_bwd_f32(vtlb_ctx* ctx, const void* d_g, void* d_dx, size_t n, double p, uint64_t seed, uint64_t step);
+/* Embedding: Y[j, :] = scale * W[ids[j], :] for j < n, W[V, D].  An id outside [0, V) (padding, by convention -1) is
+ * never dereferenced: its row of Y is zero, and it takes part in no gradient; with check != 0 the call blocks and
+ * reports it as VTLB_EINVAL (Y is written all the same; not available under capture: VTLB_ESTATE).  With p > 0 dropout
+ * is applied to the scaled rows in the same pass: bit for bit vtlb_dropout_fwd_f32 on Y[n * D].
+ * Gradient: dW[v, :] = scale * (sum of G[j, :] over the positions j with ids[j] = v), with the mask of the forward pass
+ * applied to G first where p > 0.  accumulate == 0 writes all of dW, rows of tokens that do not occur as zeros;
+ * accumulate != 0 adds to the rows of the tokens that occur and leaves the others untouched (a table shared with
+ * another layer, several batches per update).  n <= 2^31 - 1; the results may not overlap the inputs. */
+int vtlb_embedding_fwd_f32(vtlb_ctx* ctx, const void* d_W, int V, int D, const void* d_ids_i32, size_t n, float scale,
+                           double p, uint64_t seed, uint64_t step, void* d_Y, int check);
+int vtlb_embedding_bwd_f32(vtlb_ctx* ctx, const void* d_G, const void* d_ids_i32, size_t n, int V, int D, float scale,
+                           double p, uint64_t seed, uint64_t step, void* d_dW, int accumulate);
+/* ids[i] = src[i] where that is a whole number in [0, 2^31), else -1: tokens that arrive in an f32 tensor. */
+int vtlb_ids_from_f32(vtlb_ctx* ctx, const void* d_src, size_t n, void* d_ids_i32);
+/* Group norm with an activation, channels last: x[B, S, C] (S = positions of a feature map or a sequence, 1 for plain
+ * features), the C channels in `groups` equal groups.  Per sample and group: h = (x - mean) * rstd with
+ * rstd = 1 / sqrt(variance + eps) (biased), z = gamma[c] * h + beta[c] (NULL: 1 and 0), y = act(z): nothing, ReLU as
+ * above, or SiLU z / (1 + exp(-z)).  groups = 1 and S = 1 is a layer norm over C.  d_mean and d_rstd [B, groups] receive
+ * the statistics; the backward pass reads them, and x, and recomputes z.  d_y may be d_x where x is not needed again.
+ * Backward, dz = g * act'(z): dgamma[c] = sum dz * h, dbeta[c] = sum dz over samples and positions,
+ * dx = rstd * (gamma dz - mean(gamma dz) - h * mean(gamma dz h)), the means over the group; any output may be NULL,
+ * d_dx may be d_g or d_x. */
+#define VTLB_ACT_NONE 0
+#define VTLB_ACT_RELU 1
+#define VTLB_ACT_SILU 2
+int vtlb_groupnorm_fwd_f32(vtlb_ctx* ctx, const void* d_x, int B, int S, int C, int groups, const void* d_gamma_or_null,
+                           const void* d_beta_or_null, double eps, int act, void* d_y, void* d_mean, void* d_rstd);
+int vtlb_groupnorm_bwd_f32(vtlb_ctx* ctx, const void* d_g, const void* d_x, int B, int S, int C, int groups,
+                           const void* d_gamma_or_null, const void* d_beta_or_null, const void* d_mean,
+                           const void* d_rstd, int act, void* d_dx_or_null, void* d_dgamma_or_null,
+                           void* d_dbeta_or_null);
+
 /* ---- input pipeline: copies that overlap the compute stream -------------------
  * The reference stages every batch through the host synchronously (cuda_memcpy_host_to_device
  * in storage/cuda_d_cuda.v:32-60 and GpuBufF64.upload, then a blocking download); its loader

@@ -82,6 +82,13 @@ _PROTOS = {
     "vtlb_batchnorm1d_train_f32": [_vp, _vp, _i, _i, _vp, _vp, _d, _vp, _vp, _vp, _vp, _vp, _d],
     "vtlb_batchnorm1d_infer_f32": [_vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _d, _vp],
     "vtlb_batchnorm1d_bwd_f32": [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _d, _vp, _vp, _vp],
+    "vtlb_dropout_fwd_f32": [_vp, _vp, _vp, _sz, _d, C.c_uint64, C.c_uint64],
+    "vtlb_dropout_bwd_f32": [_vp, _vp, _vp, _sz, _d, C.c_uint64, C.c_uint64],
+    "vtlb_embedding_fwd_f32": [_vp, _vp, _i, _i, _vp, _sz, C.c_float, _d, C.c_uint64, C.c_uint64, _vp, _i],
+    "vtlb_embedding_bwd_f32": [_vp, _vp, _vp, _sz, _i, _i, C.c_float, _d, C.c_uint64, C.c_uint64, _vp, _i],
+    "vtlb_ids_from_f32": [_vp, _vp, _sz, _vp],
+    "vtlb_groupnorm_fwd_f32": [_vp, _vp, _i, _i, _i, _i, _vp, _vp, _d, _i, _vp, _vp, _vp],
+    "vtlb_groupnorm_bwd_f32": [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp],
     "vtlb_copy_d2h_async": [_vp, _vp, _vp, _sz],
     "vtlb_copy_wait": [_vp, _i],
     "vtlb_gather_rows_f32": [_vp, _vp, _i, _sz, _vp, _i, _vp, _i],
@@ -507,6 +514,34 @@ class Device:
     def batchnorm1d_bwd_f32(self, g, x, B, F, gamma, mean, var, eps, dx=None, dgamma=None, dbeta=None):
         self._ck(self.lib.vtlb_batchnorm1d_bwd_f32(self.h, _ptr(g), _ptr(x), B, F, _ptr(gamma), _ptr(mean), _ptr(var),
                                                    eps, _ptr(dx), _ptr(dgamma), _ptr(dbeta)))
+
+    # -- token models
+    ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2
+
+    def dropout_fwd_f32(self, x, y, n, p, seed, step):
+        self._ck(self.lib.vtlb_dropout_fwd_f32(self.h, _ptr(x), _ptr(y), n, p, seed, step))
+
+    def dropout_bwd_f32(self, g, dx, n, p, seed, step):
+        self._ck(self.lib.vtlb_dropout_bwd_f32(self.h, _ptr(g), _ptr(dx), n, p, seed, step))
+
+    def embedding_fwd_f32(self, W, V, D, ids, n, Y, scale=1.0, p=0.0, seed=0, step=0, check=True):
+        self._ck(self.lib.vtlb_embedding_fwd_f32(self.h, _ptr(W), V, D, _ptr(ids), n, scale, p, seed, step, _ptr(Y),
+                                                 int(check)))
+
+    def embedding_bwd_f32(self, G, ids, n, V, D, dW, scale=1.0, p=0.0, seed=0, step=0, accumulate=False):
+        self._ck(self.lib.vtlb_embedding_bwd_f32(self.h, _ptr(G), _ptr(ids), n, V, D, scale, p, seed, step, _ptr(dW),
+                                                 int(accumulate)))
+
+    def ids_from_f32(self, src, n, ids):
+        self._ck(self.lib.vtlb_ids_from_f32(self.h, _ptr(src), n, _ptr(ids)))
+
+    def groupnorm_fwd_f32(self, x, B, S, Cc, groups, gamma, beta, eps, act, y, mean, rstd):
+        self._ck(self.lib.vtlb_groupnorm_fwd_f32(self.h, _ptr(x), B, S, Cc, groups, _ptr(gamma), _ptr(beta), eps, act,
+                                                 _ptr(y), _ptr(mean), _ptr(rstd)))
+
+    def groupnorm_bwd_f32(self, g, x, B, S, Cc, groups, gamma, beta, mean, rstd, act, dx=None, dgamma=None, dbeta=None):
+        self._ck(self.lib.vtlb_groupnorm_bwd_f32(self.h, _ptr(g), _ptr(x), B, S, Cc, groups, _ptr(gamma), _ptr(beta),
+                                                 _ptr(mean), _ptr(rstd), act, _ptr(dx), _ptr(dgamma), _ptr(dbeta)))
 
     # -- int8
     def i8_ld(self, K: int) -> int:

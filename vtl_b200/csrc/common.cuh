@@ -158,6 +158,39 @@ inline void vtlb_comm_track(vtlb_ctx* ctx, const void* p, size_t bytes) {
 // Returns a scratch region of at least `bytes` (grown on demand; growth
 // synchronises the stream first because earlier kernels may still use the old one).
 int vtlb_scratch(vtlb_ctx* ctx, size_t bytes, void** out);
+// Whether the compute stream is being captured into a graph.
+inline int vtlb_capturing(vtlb_ctx* ctx, bool* out) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  VTLB_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &st));
+  *out = st != cudaStreamCaptureStatusNone;
+  return VTLB_OK;
+}
+
+// Workspace of one call.  Outside a capture it is the context's scratch, which the compute stream orders between
+// calls.  While the compute stream is being captured it is an allocation of the graph's own, made and freed by
+// nodes of that graph: the scratch may be replaced by a larger one before the graph is replayed, and two graphs
+// (or a graph and a call) that run side by side must not share it.
+class vtlb_workspace {
+ public:
+  explicit vtlb_workspace(vtlb_ctx* c) : ctx_(c) {}
+  ~vtlb_workspace() {
+    if (own_) cudaFreeAsync(own_, ctx_->stream);
+  }
+  vtlb_workspace(const vtlb_workspace&) = delete;
+  vtlb_workspace& operator=(const vtlb_workspace&) = delete;
+  int get(size_t bytes, void** out) {
+    bool capturing = false;
+    if (int rc = vtlb_capturing(ctx_, &capturing)) return rc;
+    if (!capturing) return vtlb_scratch(ctx_, bytes, out);
+    VTLB_CUDA(ctx_, cudaMallocAsync(&own_, bytes, ctx_->stream));
+    *out = own_;
+    return VTLB_OK;
+  }
+
+ private:
+  vtlb_ctx* ctx_;
+  void* own_ = nullptr;
+};
 
 // Launch with programmatic stream serialisation: the kernel's CTAs may become resident while
 // the kernel in front of it in the stream is still finishing, which hides the launch latency
