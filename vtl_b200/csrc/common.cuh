@@ -182,7 +182,14 @@ class vtlb_workspace {
     bool capturing = false;
     if (int rc = vtlb_capturing(ctx_, &capturing)) return rc;
     if (!capturing) return vtlb_scratch(ctx_, bytes, out);
-    VTLB_CUDA(ctx_, cudaMallocAsync(&own_, bytes, ctx_->stream));
+    if (own_ && bytes > own_bytes_) {
+      VTLB_CUDA(ctx_, cudaFreeAsync(own_, ctx_->stream));
+      own_ = nullptr;
+    }
+    if (!own_) {
+      VTLB_CUDA(ctx_, cudaMallocAsync(&own_, bytes, ctx_->stream));
+      own_bytes_ = bytes;
+    }
     *out = own_;
     return VTLB_OK;
   }
@@ -190,6 +197,7 @@ class vtlb_workspace {
  private:
   vtlb_ctx* ctx_;
   void* own_ = nullptr;
+  size_t own_bytes_ = 0;
 };
 
 // Launch with programmatic stream serialisation: the kernel's CTAs may become resident while
