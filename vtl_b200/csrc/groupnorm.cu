@@ -4,7 +4,10 @@
 // Backward, with dz = g * act'(z) and n = S * C/groups:
 //   dgamma_c = sum over samples and positions of dz * h,   dbeta_c = sum of dz,
 //   dx = rstd * (gamma_c * dz - (sum gamma dz) / n - h * (sum gamma dz h) / n), the sums over the group.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
+#include "groupnorm_plan.h"
 
 namespace {
 
@@ -133,6 +136,312 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const float* x, const flo
   }
 }
 
+// ---------------------------------------------------------------- groups that fit the registers of a cluster
+// x is read once: it stays in registers between the sums and the result (groupnorm_plan.h).  Bound by HBM, 8 bytes per
+// element forward, 12 backward.
+struct GnTile {
+  GnDims d;
+  int groups, slabs, csplit, channels, rows;
+};
+
+template <int VEC>
+struct GnVec {
+  float e[VEC];
+};
+template <int VEC>
+__device__ __forceinline__ GnVec<VEC> gn_load(const float* p) {
+  GnVec<VEC> v;
+  if constexpr (VEC == 4) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v.e[0] = f.x, v.e[1] = f.y, v.e[2] = f.z, v.e[3] = f.w;
+  } else {
+    v.e[0] = *p;
+  }
+  return v;
+}
+template <int VEC>
+__device__ __forceinline__ void gn_store(float* p, const GnVec<VEC>& v) {
+  if constexpr (VEC == 4)
+    *reinterpret_cast<float4*>(p) = make_float4(v.e[0], v.e[1], v.e[2], v.e[3]);
+  else
+    *p = v.e[0];
+}
+
+// Where this CTA and thread stand.
+struct GnPlace {
+  int b, grp0, groups;  // sample, first group of the slab, groups in it
+  int c0, channels;     // first channel and channels of this CTA
+  int in_slab;          // c0 minus the slab's first channel
+  int cols, lanes;      // pieces of VEC channels, rows per step
+  int col, lane;        // this thread's
+  int r0, r1;           // rows of this CTA
+  bool on;
+};
+template <int VEC>
+__device__ __forceinline__ GnPlace gn_place(const GnTile& t, int rank, int cluster) {
+  GnPlace p;
+  const unsigned unit = blockIdx.x / cluster;
+  p.b = (int)(unit / t.slabs);
+  const int slab = (int)(unit % t.slabs);
+  p.grp0 = slab * t.groups;
+  p.groups = min(t.groups, t.d.G - p.grp0);
+  p.in_slab = (rank % t.csplit) * t.channels;
+  p.c0 = p.grp0 * t.d.width + p.in_slab;
+  p.channels = min(t.channels, p.groups * t.d.width - p.in_slab);
+  p.cols = p.channels / VEC;
+  p.lanes = kGnThreads / p.cols;
+  p.col = threadIdx.x % p.cols;
+  p.lane = threadIdx.x / p.cols;
+  p.r0 = min(t.d.S, (rank / t.csplit) * t.rows);
+  p.r1 = min(t.d.S, p.r0 + t.rows);
+  p.on = p.lane < p.lanes;
+  return p;
+}
+
+template <int ACT, int VEC, int VPT, bool GROUPED>
+__global__ void __launch_bounds__(kGnThreads) gn_fwd_tile_kernel(const float* x, const float* gamma, const float* beta,
+                                                                 GnTile t, double eps, float* y, float* mean_out,
+                                                                 float* rstd_out) {
+  namespace cg = cooperative_groups;
+  constexpr int PAIRS = GROUPED ? 1 : VEC;  // GROUPED: the channels of a thread's piece are all of one group
+  __shared__ double2 sm_pair[kGnThreads * PAIRS];
+  __shared__ double2 sm_sum[kGnMaxGroups];
+  __shared__ float2 sm_stat[kGnMaxGroups];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
+  const GnPlace p = gn_place<VEC>(t, rank, ctas);
+  const int tid = threadIdx.x, warp = tid >> 5, width = t.d.width;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the kernel in front is done from here on
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const size_t base = ((size_t)p.b * t.d.S + p.r0 + p.lane) * t.d.C + p.c0 + (size_t)p.col * VEC;
+  const size_t step = (size_t)p.lanes * t.d.C;
+  GnVec<VEC> v[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    if (p.on && p.r0 + p.lane + i * p.lanes < p.r1) {
+      v[i] = gn_load<VEC>(x + base + i * step);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) v[i].e[k] = 0.0f;
+    }
+  }
+  // Sums of x and x^2 in f64, so that one pass over the registers does: the variance loses 2^-53 of the mean square.
+  double2 acc[PAIRS] = {};
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const double e = (double)v[i].e[k];
+      acc[k % PAIRS].x += e;
+      acc[k % PAIRS].y = fma(e, e, acc[k % PAIRS].y);
+    }
+#pragma unroll
+  for (int k = 0; k < PAIRS; ++k) sm_pair[tid * PAIRS + k] = acc[k];
+  __syncthreads();
+  // one warp per group of the slab: the entries of its channels in this CTA, all rows
+  constexpr int PER = VEC / PAIRS;  // channels per entry
+  for (int g = warp; g < p.groups; g += kGnThreads / 32) {
+    const int lo = max(g * width - p.in_slab, 0) / PER, hi = min((g + 1) * width - p.in_slab, p.channels) / PER;
+    double2 s = make_double2(0.0, 0.0);
+    const int n = hi > lo ? hi - lo : 0, entries = p.channels / PER;
+    for (int i = tid & 31; i < n * p.lanes; i += 32) {
+      const double2 e = sm_pair[(i / n) * entries + lo + i % n];
+      s.x += e.x, s.y += e.y;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
+    if ((tid & 31) == 0) sm_sum[g] = s;
+  }
+  if (ctas > 1) cluster.sync(); else __syncthreads();
+  if (tid < p.groups) {
+    double2 s = make_double2(0.0, 0.0);
+    for (int r = 0; r < ctas; ++r) {
+      const double2 e = *cluster.map_shared_rank(&sm_sum[tid], r);
+      s.x += e.x, s.y += e.y;
+    }
+    const double n = (double)t.d.S * width, mu = s.x / n, var = s.y / n - mu * mu;
+    const float2 st = make_float2((float)mu, (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + eps)));
+    sm_stat[tid] = st;
+    if (rank == 0) {
+      const size_t k = (size_t)p.b * t.d.G + p.grp0 + tid;
+      mean_out[k] = st.x;
+      rstd_out[k] = st.y;
+    }
+  }
+  if (ctas > 1) cluster.sync(); else __syncthreads();  // (and no CTA leaves while another reads its sums)
+  if (!p.on) return;
+  float mu[VEC], rs[VEC], ga[VEC], be[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    const int c = p.col * VEC + k;
+    const float2 st = sm_stat[(p.in_slab + c) / width];
+    mu[k] = st.x, rs[k] = st.y;
+    ga[k] = gamma ? __ldg(gamma + p.c0 + c) : 1.0f;
+    be[k] = beta ? __ldg(beta + p.c0 + c) : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    if (p.r0 + p.lane + i * p.lanes >= p.r1) break;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[i].e[k] = act<ACT>(ga[k] * __fmul_rn(__fsub_rn(v[i].e[k], mu[k]), rs[k]) + be[k]);
+    gn_store<VEC>(y + base + i * step, v[i]);
+  }
+}
+
+// Backward.  The channel sums of each CTA go to `sums` [B * rsplit][C] (dz * h, dz) for gn_params_kernel.
+template <int ACT, int VEC, int VPT>
+__global__ void __launch_bounds__(kGnThreads) gn_bwd_tile_kernel(const float* g, const float* x, const float* gamma,
+                                                                 const float* beta, const float* mean, const float* rstd,
+                                                                 GnTile t, float* dx, float2* sums) {
+  namespace cg = cooperative_groups;
+  __shared__ float2 sm_part[kGnThreads * VEC];  // [lane][channel]
+  __shared__ float2 sm_chan[kGnThreads * VEC];
+  __shared__ float2 sm_sum[kGnMaxGroups];
+  __shared__ float2 sm_coef[kGnMaxGroups];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
+  const GnPlace p = gn_place<VEC>(t, rank, ctas);
+  const int tid = threadIdx.x, warp = tid >> 5, width = t.d.width;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const size_t base = ((size_t)p.b * t.d.S + p.r0 + p.lane) * t.d.C + p.c0 + (size_t)p.col * VEC;
+  const size_t step = (size_t)p.lanes * t.d.C;
+  GnVec<VEC> vx[VPT], vg[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    if (p.on && p.r0 + p.lane + i * p.lanes < p.r1) {
+      vx[i] = gn_load<VEC>(x + base + i * step);
+      vg[i] = gn_load<VEC>(g + base + i * step);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) vx[i].e[k] = vg[i].e[k] = 0.0f;
+    }
+  }
+  float mu[VEC], rs[VEC], ga[VEC], be[VEC];
+  if (p.on) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const int c = p.col * VEC + k;
+      const size_t st = (size_t)p.b * t.d.G + p.grp0 + (p.in_slab + c) / width;
+      mu[k] = __ldg(mean + st), rs[k] = __ldg(rstd + st);
+      ga[k] = gamma ? __ldg(gamma + p.c0 + c) : 1.0f;
+      be[k] = beta ? __ldg(beta + p.c0 + c) : 0.0f;
+    }
+  }
+  float2 acc[VEC] = {};
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    if (!(p.on && p.r0 + p.lane + i * p.lanes < p.r1)) break;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const float h = __fmul_rn(__fsub_rn(vx[i].e[k], mu[k]), rs[k]);
+      const float dz = act_bwd<ACT>(vg[i].e[k], vx[i].e[k], mu[k], rs[k], ga[k], be[k], h);
+      acc[k].x = fmaf(dz, h, acc[k].x);
+      acc[k].y += dz;
+      vx[i].e[k] = h, vg[i].e[k] = dz;  // what dx is made of
+    }
+  }
+  if (p.on) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sm_part[p.lane * p.channels + p.col * VEC + k] = acc[k];
+  }
+  __syncthreads();
+  // per channel: `parts` threads take every parts-th row lane, then one adds theirs
+  const int parts = max(1, min(kGnThreads / p.channels, p.lanes));
+  for (int i = tid; i < parts * p.channels; i += kGnThreads) {
+    const int part = i / p.channels, c = i % p.channels;
+    float2 s = make_float2(0.f, 0.f);
+    for (int l = part; l < p.lanes; l += parts) {
+      const float2 e = sm_part[l * p.channels + c];
+      s.x += e.x, s.y += e.y;
+    }
+    sm_chan[i] = s;
+  }
+  __syncthreads();
+  for (int c = tid; c < p.channels; c += kGnThreads) {
+    float2 s = sm_chan[c];
+    for (int q = 1; q < parts; ++q) {
+      const float2 e = sm_chan[q * p.channels + c];
+      s.x += e.x, s.y += e.y;
+    }
+    if (sums) sums[((size_t)p.b * (ctas / t.csplit) + rank / t.csplit) * t.d.C + p.c0 + c] = s;
+    const float w = gamma ? __ldg(gamma + p.c0 + c) : 1.0f;
+    sm_part[c] = make_float2(w * s.x, w * s.y);
+  }
+  if (!dx) return;  // (all CTAs of the cluster alike: nobody reads another's shared memory)
+  __syncthreads();
+  for (int gr = warp; gr < p.groups; gr += kGnThreads / 32) {
+    const int lo = max(gr * width - p.in_slab, 0), hi = min((gr + 1) * width - p.in_slab, p.channels);
+    float2 s = make_float2(0.f, 0.f);
+    for (int c = lo + (tid & 31); c < hi; c += 32) s.x += sm_part[c].x, s.y += sm_part[c].y;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
+    if ((tid & 31) == 0) sm_sum[gr] = s;
+  }
+  if (ctas > 1) cluster.sync(); else __syncthreads();
+  if (tid < p.groups) {
+    float2 s = make_float2(0.f, 0.f);
+    for (int r = 0; r < ctas; ++r) {
+      const float2 e = *cluster.map_shared_rank(&sm_sum[tid], r);
+      s.x += e.x, s.y += e.y;
+    }
+    const float n = (float)t.d.S * (float)width;
+    sm_coef[tid] = make_float2(s.x / n, s.y / n);
+  }
+  if (ctas > 1) cluster.sync(); else __syncthreads();
+  if (!p.on) return;
+  float2 cf[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) cf[k] = sm_coef[(p.in_slab + p.col * VEC + k) / width];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    if (p.r0 + p.lane + i * p.lanes >= p.r1) break;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) vx[i].e[k] = rs[k] * (ga[k] * vg[i].e[k] - cf[k].y - vx[i].e[k] * cf[k].x);
+    gn_store<VEC>(dx + base + i * step, vx[i]);
+  }
+}
+
+// dgamma and dbeta from the channel sums: 32 channels and eight stretches of rows per CTA.
+__global__ void __launch_bounds__(256) gn_params_tile_kernel(const float2* sums, int rows, int C, float* dgamma, float* dbeta) {
+  __shared__ double2 sm[8][32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  double2 s = make_double2(0.0, 0.0);
+  if (c < C) {
+#pragma unroll 8
+    for (int r = part; r < rows; r += 8) {
+      const float2 e = sums[(size_t)r * C + c];
+      s.x += (double)e.x, s.y += (double)e.y;
+    }
+  }
+  sm[part][lane] = s;
+  __syncthreads();
+  if (part || c >= C) return;
+  for (int q = 1; q < 8; ++q) s.x += sm[q][lane].x, s.y += sm[q][lane].y;
+  if (dgamma) dgamma[c] = (float)s.x;
+  if (dbeta) dbeta[c] = (float)s.y;
+}
+
+template <typename... KArgs, typename... Args>
+cudaError_t cluster_launch(vtlb_ctx* ctx, void (*kern)(KArgs...), unsigned grid, int cluster, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kGnThreads);
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<Args&&>(args)...);
+}
+
+GnTile tile_of(const GnDims& d, const GnPlan& p) { return GnTile{d, p.groups, p.slabs, p.csplit, p.channels, p.rows}; }
+
 int check_dims(vtlb_ctx* ctx, const char* fn, int B, int S, int C, int groups, int act_kind, GnDims* d) {
   if (B <= 0 || S <= 0 || C <= 0 || groups <= 0 || C % groups)
     return vtlb_fail(ctx, VTLB_EINVAL, "%s: bad shape B=%d S=%d C=%d groups=%d", fn, B, S, C, groups);
@@ -147,6 +456,30 @@ int check_dims(vtlb_ctx* ctx, const char* fn, int B, int S, int C, int groups, i
 template <int ACT>
 int gn_forward(vtlb_ctx* ctx, const float* x, GnDims d, const float* gamma, const float* beta, double eps, float* y,
                float* mean, float* rstd) {
+  const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, vtlb_aligned16(x) && vtlb_aligned16(y), 8, 16, ctx->sm_count);
+  if (plan.on_chip) {
+    const GnTile t = tile_of(d, plan);
+    const int cluster = plan.csplit * plan.rsplit;
+    const unsigned grid = (unsigned)((size_t)d.B * plan.slabs * cluster);
+    const bool grouped = plan.vec == 1 || d.width % 4 == 0;
+#define VTLB_GN_FWD(VEC, VPT, GROUPED) \
+  cluster_launch(ctx, gn_fwd_tile_kernel<ACT, VEC, VPT, GROUPED>, grid, cluster, x, gamma, beta, t, eps, y, mean, rstd)
+#define VTLB_GN_FWD_VPT(VPT) \
+  case VPT:                  \
+    VTLB_CUDA(ctx, plan.vec == 1 ? VTLB_GN_FWD(1, VPT, true) : grouped ? VTLB_GN_FWD(4, VPT, true) : VTLB_GN_FWD(4, VPT, false)); \
+    break
+    switch (plan.vpt) {
+      VTLB_GN_FWD_VPT(1);
+      VTLB_GN_FWD_VPT(2);
+      VTLB_GN_FWD_VPT(4);
+      VTLB_GN_FWD_VPT(8);
+      VTLB_GN_FWD_VPT(16);
+    }
+#undef VTLB_GN_FWD_VPT
+#undef VTLB_GN_FWD
+    VTLB_LAUNCHED(ctx);
+    return VTLB_OK;
+  }
   const int chunks = (d.S + kRows - 1) / kRows;
   vtlb_workspace ws(ctx);
   void* partial = nullptr;
@@ -165,9 +498,41 @@ int gn_forward(vtlb_ctx* ctx, const float* x, GnDims d, const float* gamma, cons
 template <int ACT>
 int gn_backward(vtlb_ctx* ctx, const float* g, const float* x, GnDims d, const float* gamma, const float* beta,
                 const float* mean, const float* rstd, float* dx, float* dgamma, float* dbeta) {
-  const int chunks = (d.S + kRows - 1) / kRows;
+  const bool aligned = vtlb_aligned16(x) && vtlb_aligned16(g) && vtlb_aligned16(dx);
+  const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, aligned, 4, 8, ctx->sm_count);
   vtlb_workspace ws(ctx);
   void* scratch = nullptr;
+  if (plan.on_chip) {
+    const GnTile t = tile_of(d, plan);
+    const int cluster = plan.csplit * plan.rsplit;
+    const unsigned grid = (unsigned)((size_t)d.B * plan.slabs * cluster);
+    const int rows = d.B * plan.rsplit;
+    if (dgamma || dbeta)
+      if (int rc = ws.get((size_t)rows * d.C * sizeof(float2), &scratch)) return rc;
+    float2* sums = (float2*)scratch;
+#define VTLB_GN_BWD(VEC, VPT) \
+  cluster_launch(ctx, gn_bwd_tile_kernel<ACT, VEC, VPT>, grid, cluster, g, x, gamma, beta, mean, rstd, t, dx, sums)
+#define VTLB_GN_BWD_VPT(VPT) \
+  case VPT:                  \
+    VTLB_CUDA(ctx, plan.vec == 1 ? VTLB_GN_BWD(1, VPT) : VTLB_GN_BWD(4, VPT)); \
+    break
+    switch (plan.vpt) {
+      VTLB_GN_BWD_VPT(1);
+      VTLB_GN_BWD_VPT(2);
+      VTLB_GN_BWD_VPT(4);
+      VTLB_GN_BWD_VPT(8);
+    }
+#undef VTLB_GN_BWD_VPT
+#undef VTLB_GN_BWD
+    VTLB_LAUNCHED(ctx);
+    if (sums) {
+      VTLB_CUDA(ctx, vtlb_launch_early(gn_params_tile_kernel, dim3((d.C + 31) / 32), dim3(256), 0, ctx->stream,
+                                       (const float2*)sums, rows, d.C, dgamma, dbeta));
+      VTLB_LAUNCHED(ctx);
+    }
+    return VTLB_OK;
+  }
+  const int chunks = (d.S + kRows - 1) / kRows;
   const size_t sums = (size_t)d.B * chunks * d.C * sizeof(double2);
   if (int rc = ws.get(sums + (size_t)d.B * d.G * sizeof(float2), &scratch)) return rc;
   double2* partial = (double2*)scratch;

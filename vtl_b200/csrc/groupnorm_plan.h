@@ -1,0 +1,51 @@
+// How group norm cuts its work (groupnorm.cu); plain C++, so that it can be checked for every size without a GPU.
+#pragma once
+
+// Channels are taken in slabs of whole groups.  A thread-block cluster owns one slab of one sample; its CTAs cut the
+// positions into `rsplit` equal stretches (and a slab too wide for the threads of one CTA into `csplit` pieces), and
+// each CTA keeps its piece in registers: `vpt` pieces of `vec` channels a thread.
+struct GnPlan {
+  bool on_chip;     // false: the group does not fit a cluster's registers; x is read twice
+  int vec;          // channels per load: 4 (16-byte aligned rows) or 1
+  int vpt;          // rows per thread: 1, 2, 4, 8, 16
+  int groups;       // per slab; the last slab may have fewer
+  int slabs;
+  int csplit, rsplit;
+  int channels;     // per CTA (a multiple of vec), the last piece of a slab may have fewer
+  int rows;         // per CTA, the last stretch may have fewer
+};
+
+constexpr int kGnThreads = 512, kGnMaxGroups = 32, kGnMaxCluster = 8;
+
+// `most`: the largest vpt of the kernel at hand (registers), `usual`: the one it runs best with.
+inline GnPlan gn_plan(int B, int S, int C, int G, bool aligned, int usual, int most, int sm_count) {
+  GnPlan p = {};
+  const int width = C / G;
+  p.vec = aligned && C % 4 == 0 ? 4 : 1;
+  // Slabs of 32 channels and more: 128-byte pieces of a row.
+  int unit = 1;  // groups whose channels are a multiple of vec
+  while (((long long)unit * width) % p.vec) ++unit;
+  const long long per_unit = (long long)unit * width;
+  p.groups = unit * (int)((32 + per_unit - 1) / per_unit);
+  if (p.groups > G) p.groups = G;
+  p.slabs = (G + p.groups - 1) / p.groups;
+  const int slab = p.groups * width, cols = slab / p.vec;
+  p.csplit = 1;
+  while ((cols + p.csplit - 1) / p.csplit > kGnThreads && p.csplit < kGnMaxCluster) p.csplit *= 2;
+  const int cols_cta = (cols + p.csplit - 1) / p.csplit;
+  p.channels = cols_cta * p.vec;
+  if (cols_cta > kGnThreads || p.groups > kGnMaxGroups) return p;
+  const int lanes = kGnThreads / cols_cta;  // rows that a CTA takes in one step
+  const auto fits = [&](int vpt, int rsplit) { return (long long)lanes * vpt * rsplit >= S; };
+  const int max_r = kGnMaxCluster / p.csplit;
+  p.rsplit = 1;
+  while (p.rsplit < max_r && !fits(usual, p.rsplit)) p.rsplit *= 2;
+  if (!fits(most, p.rsplit)) return p;
+  // Too few CTAs for the SMs: shorter stretches.
+  while (p.rsplit < max_r && !fits(1, p.rsplit) && (long long)B * p.slabs * p.csplit * p.rsplit * 2 <= sm_count) p.rsplit *= 2;
+  p.rows = (S + p.rsplit - 1) / p.rsplit;
+  p.vpt = 1;
+  while ((long long)lanes * p.vpt < p.rows) p.vpt *= 2;
+  p.on_chip = true;
+  return p;
+}
