@@ -15,10 +15,15 @@ struct GnDims {
   int B, S, C, G, width;  // width = C / G
 };
 
+// 1 / (1 + exp(-z)) within 7 half steps: expf 4, the sum 1, the approximate division (1 ulp) 2.  IEEE division would
+// take some eight instructions more per element, a fifth of the forward kernel's.  Below -87.3, where the sum passes
+// 2^126, the division gives 0 (the logistic function is under 1.2e-38 there).
+__device__ __forceinline__ float logistic(float z) { return __fdividef(1.0f, 1.0f + expf(-z)); }
+
 template <int ACT>
 __device__ __forceinline__ float act(float z) {
   if (ACT == VTLB_ACT_RELU) return z < 0.0f ? 0.0f : z;
-  if (ACT == VTLB_ACT_SILU) return z / (1.0f + expf(-z));
+  if (ACT == VTLB_ACT_SILU) return z * logistic(z);
   return z;
 }
 
@@ -35,7 +40,7 @@ __device__ __forceinline__ float act_bwd(float g, float x, float mean, float rst
     }
     return z < 0.0f ? 0.0f : g;
   }
-  const float s = 1.0f / (1.0f + expf(-z));
+  const float s = logistic(z);
   return g * (s * (1.0f + z * (1.0f - s)));
 }
 
@@ -176,6 +181,7 @@ struct GnPlace {
   int col, lane;        // this thread's
   int r0, r1;           // rows of this CTA
   bool on;
+  bool even;            // pieces of a row fill a warp evenly: cols is a power of two up to 32
 };
 template <int VEC>
 __device__ __forceinline__ GnPlace gn_place(const GnTile& t, int rank, int cluster) {
@@ -195,11 +201,12 @@ __device__ __forceinline__ GnPlace gn_place(const GnTile& t, int rank, int clust
   p.r0 = min(t.d.S, (rank / t.csplit) * t.rows);
   p.r1 = min(t.d.S, p.r0 + t.rows);
   p.on = p.lane < p.lanes;
+  p.even = p.cols <= 32 && (p.cols & (p.cols - 1)) == 0;
   return p;
 }
 
 template <int ACT, int VEC, int VPT, bool GROUPED>
-__global__ void __launch_bounds__(kGnThreads) gn_fwd_tile_kernel(const float* x, const float* gamma, const float* beta,
+__global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 1024 / kGnThreads) gn_fwd_tile_kernel(const float* x, const float* gamma, const float* beta,
                                                                  GnTile t, double eps, float* y, float* mean_out,
                                                                  float* rstd_out) {
   namespace cg = cooperative_groups;
@@ -215,42 +222,77 @@ __global__ void __launch_bounds__(kGnThreads) gn_fwd_tile_kernel(const float* x,
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const size_t base = ((size_t)p.b * t.d.S + p.r0 + p.lane) * t.d.C + p.c0 + (size_t)p.col * VEC;
   const size_t step = (size_t)p.lanes * t.d.C;
+  const int rows = p.on ? min(VPT, max(0, (p.r1 - p.r0 - p.lane + p.lanes - 1) / p.lanes)) : 0;  // of this thread
   GnVec<VEC> v[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    if (p.on && p.r0 + p.lane + i * p.lanes < p.r1) {
+    if (i < rows) {
       v[i] = gn_load<VEC>(x + base + i * step);
     } else {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) v[i].e[k] = 0.0f;
     }
   }
-  // Sums of x and x^2 in f64, so that one pass over the registers does: the variance loses 2^-53 of the mean square.
-  double2 acc[PAIRS] = {};
+  // A thread's own mean K and squared distances from it in f32, then sums of x and x^2 in f64 from them: the variance
+  // loses 2^-53 of the mean square, not 2^-24, and few instructions are f64.
+  constexpr int PER = VEC / PAIRS;  // channels per pair
+  double2 acc[PAIRS];
 #pragma unroll
-  for (int i = 0; i < VPT; ++i)
+  for (int q = 0; q < PAIRS; ++q) {
+    const float n = (float)(rows * PER);
+    float sum = 0.0f, dist = 0.0f;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      const double e = (double)v[i].e[k];
-      acc[k % PAIRS].x += e;
-      acc[k % PAIRS].y = fma(e, e, acc[k % PAIRS].y);
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int k = 0; k < PER; ++k) sum += v[i].e[q * PER + k];
+    const float mean = rows ? __fdividef(sum, n) : 0.0f;  // any value near the mean serves
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (i < rows) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const float e = v[i].e[q * PER + k] - mean;
+          dist = fmaf(e, e, dist);
+        }
+      }
+    const double nm = (double)n * (double)mean;
+    acc[q] = make_double2(nm, fma(nm, (double)mean, (double)dist));
+  }
+  const int cq = width / PER;  // pairs per group and row
+  if (p.even && (PAIRS == 1) && (cq & (cq - 1)) == 0 && cq <= p.cols) {
+    // lanes of a warp that hold one group: the other rows' (steps of cols), then the other pieces of its channels
+    for (int o = 16; o; o >>= 1) {
+      if (o >= p.cols || o < cq) {
+        acc[0].x += __shfl_xor_sync(~0u, acc[0].x, o);
+        acc[0].y += __shfl_xor_sync(~0u, acc[0].y, o);
+      }
     }
+    const int lane = tid & 31;
+    if (lane < p.cols && lane % cq == 0) sm_pair[warp * p.groups + lane / cq] = acc[0];
+    __syncthreads();
+    if (tid < p.groups) {
+      double2 s = sm_pair[tid];
 #pragma unroll
-  for (int k = 0; k < PAIRS; ++k) sm_pair[tid * PAIRS + k] = acc[k];
-  __syncthreads();
-  // one warp per group of the slab: the entries of its channels in this CTA, all rows
-  constexpr int PER = VEC / PAIRS;  // channels per entry
-  for (int g = warp; g < p.groups; g += kGnThreads / 32) {
-    const int lo = max(g * width - p.in_slab, 0) / PER, hi = min((g + 1) * width - p.in_slab, p.channels) / PER;
-    double2 s = make_double2(0.0, 0.0);
-    const int n = hi > lo ? hi - lo : 0, entries = p.channels / PER;
-    for (int i = tid & 31; i < n * p.lanes; i += 32) {
-      const double2 e = sm_pair[(i / n) * entries + lo + i % n];
-      s.x += e.x, s.y += e.y;
+      for (int w = 1; w < kGnThreads / 32; ++w) s.x += sm_pair[w * p.groups + tid].x, s.y += sm_pair[w * p.groups + tid].y;
+      sm_sum[tid] = s;
     }
+  } else {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
-    if ((tid & 31) == 0) sm_sum[g] = s;
+    for (int q = 0; q < PAIRS; ++q) sm_pair[tid * PAIRS + q] = acc[q];
+    __syncthreads();
+    // one warp per group of the slab: the pairs of its channels in this CTA, all rows
+    for (int g = warp; g < p.groups; g += kGnThreads / 32) {
+      const int lo = max(g * width - p.in_slab, 0) / PER, hi = min((g + 1) * width - p.in_slab, p.channels) / PER;
+      double2 s = make_double2(0.0, 0.0);
+      const int n = hi > lo ? hi - lo : 0, entries = p.channels / PER;
+      for (int i = tid & 31; i < n * p.lanes; i += 32) {
+        const double2 e = sm_pair[(i / n) * entries + lo + i % n];
+        s.x += e.x, s.y += e.y;
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
+      if ((tid & 31) == 0) sm_sum[g] = s;
+    }
   }
   if (ctas > 1) cluster.sync(); else __syncthreads();
   if (tid < p.groups) {
@@ -270,27 +312,27 @@ __global__ void __launch_bounds__(kGnThreads) gn_fwd_tile_kernel(const float* x,
   }
   if (ctas > 1) cluster.sync(); else __syncthreads();  // (and no CTA leaves while another reads its sums)
   if (!p.on) return;
-  float mu[VEC], rs[VEC], ga[VEC], be[VEC];
+  float mu[VEC], a[VEC], be[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) {
     const int c = p.col * VEC + k;
-    const float2 st = sm_stat[(p.in_slab + c) / width];
-    mu[k] = st.x, rs[k] = st.y;
-    ga[k] = gamma ? __ldg(gamma + p.c0 + c) : 1.0f;
+    const float2 st = sm_stat[(p.in_slab + (GROUPED ? p.col * VEC : c)) / width];
+    mu[k] = st.x;
+    a[k] = gamma ? st.y * __ldg(gamma + p.c0 + c) : st.y;
     be[k] = beta ? __ldg(beta + p.c0 + c) : 0.0f;
   }
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    if (p.r0 + p.lane + i * p.lanes >= p.r1) break;
+    if (i >= rows) break;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) v[i].e[k] = act<ACT>(ga[k] * __fmul_rn(__fsub_rn(v[i].e[k], mu[k]), rs[k]) + be[k]);
+    for (int k = 0; k < VEC; ++k) v[i].e[k] = act<ACT>(fmaf(__fsub_rn(v[i].e[k], mu[k]), a[k], be[k]));
     gn_store<VEC>(y + base + i * step, v[i]);
   }
 }
 
 // Backward.  The channel sums of each CTA go to `sums` [B * rsplit][C] (dz * h, dz) for gn_params_kernel.
 template <int ACT, int VEC, int VPT>
-__global__ void __launch_bounds__(kGnThreads) gn_bwd_tile_kernel(const float* g, const float* x, const float* gamma,
+__global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 1024 / kGnThreads) gn_bwd_tile_kernel(const float* g, const float* x, const float* gamma,
                                                                  const float* beta, const float* mean, const float* rstd,
                                                                  GnTile t, float* dx, float2* sums) {
   namespace cg = cooperative_groups;
@@ -306,10 +348,11 @@ __global__ void __launch_bounds__(kGnThreads) gn_bwd_tile_kernel(const float* g,
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const size_t base = ((size_t)p.b * t.d.S + p.r0 + p.lane) * t.d.C + p.c0 + (size_t)p.col * VEC;
   const size_t step = (size_t)p.lanes * t.d.C;
+  const int rows = p.on ? min(VPT, max(0, (p.r1 - p.r0 - p.lane + p.lanes - 1) / p.lanes)) : 0;
   GnVec<VEC> vx[VPT], vg[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    if (p.on && p.r0 + p.lane + i * p.lanes < p.r1) {
+    if (i < rows) {
       vx[i] = gn_load<VEC>(x + base + i * step);
       vg[i] = gn_load<VEC>(g + base + i * step);
     } else {
@@ -331,7 +374,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_bwd_tile_kernel(const float* g,
   float2 acc[VEC] = {};
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    if (!(p.on && p.r0 + p.lane + i * p.lanes < p.r1)) break;
+    if (i >= rows) break;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
       const float h = __fmul_rn(__fsub_rn(vx[i].e[k], mu[k]), rs[k]);
@@ -341,21 +384,38 @@ __global__ void __launch_bounds__(kGnThreads) gn_bwd_tile_kernel(const float* g,
       vx[i].e[k] = h, vg[i].e[k] = dz;  // what dx is made of
     }
   }
-  if (p.on) {
+  int parts;  // rows of partial sums per channel in sm_chan
+  if (p.even) {
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) sm_part[p.lane * p.channels + p.col * VEC + k] = acc[k];
-  }
-  __syncthreads();
-  // per channel: `parts` threads take every parts-th row lane, then one adds theirs
-  const int parts = max(1, min(kGnThreads / p.channels, p.lanes));
-  for (int i = tid; i < parts * p.channels; i += kGnThreads) {
-    const int part = i / p.channels, c = i % p.channels;
-    float2 s = make_float2(0.f, 0.f);
-    for (int l = part; l < p.lanes; l += parts) {
-      const float2 e = sm_part[l * p.channels + c];
-      s.x += e.x, s.y += e.y;
+    for (int o = 16; o; o >>= 1) {
+      if (o < p.cols) break;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        acc[k].x += __shfl_xor_sync(~0u, acc[k].x, o);
+        acc[k].y += __shfl_xor_sync(~0u, acc[k].y, o);
+      }
     }
-    sm_chan[i] = s;
+    parts = kGnThreads / 32;
+    if ((tid & 31) < p.cols) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) sm_chan[warp * p.channels + p.col * VEC + k] = acc[k];
+    }
+  } else {
+    if (p.on) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) sm_part[p.lane * p.channels + p.col * VEC + k] = acc[k];
+    }
+    __syncthreads();
+    parts = max(1, min(kGnThreads / p.channels, p.lanes));
+    for (int i = tid; i < parts * p.channels; i += kGnThreads) {
+      const int part = i / p.channels, c = i % p.channels;
+      float2 s = make_float2(0.f, 0.f);
+      for (int l = part; l < p.lanes; l += parts) {
+        const float2 e = sm_part[l * p.channels + c];
+        s.x += e.x, s.y += e.y;
+      }
+      sm_chan[i] = s;
+    }
   }
   __syncthreads();
   for (int c = tid; c < p.channels; c += kGnThreads) {
@@ -395,7 +455,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_bwd_tile_kernel(const float* g,
   for (int k = 0; k < VEC; ++k) cf[k] = sm_coef[(p.in_slab + p.col * VEC + k) / width];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    if (p.r0 + p.lane + i * p.lanes >= p.r1) break;
+    if (i >= rows) break;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) vx[i].e[k] = rs[k] * (ga[k] * vg[i].e[k] - cf[k].y - vx[i].e[k] * cf[k].x);
     gn_store<VEC>(dx + base + i * step, vx[i]);
