@@ -28,7 +28,10 @@ def forward_bounds(x, G, gamma, beta, eps, kind, y, mean, rstd):
     d_h = per(rstd * d_mean) + np.abs(h) * (per(d_rstd / rstd) + 2 * U)
     ga, be = (1.0 if gamma is None else np.abs(gamma.astype(np.float64))), (0.0 if beta is None else np.abs(beta.astype(np.float64)))
     d_z = ga * d_h + U * (2 * ga * np.abs(h) + be)
-    return 1.01 * (1.1 * d_z + 8 * U * np.abs(y)) + 1e-37, 1.01 * d_mean + 1e-37, 1.01 * d_rstd
+    # the logistic function of SiLU is evaluated within |z| + 7 half steps (the argument of its power is rounded: |z|; the
+    # power 4, the sum 1, the reciprocal 2), its product with z rounds once more
+    z = np.abs(h * (1.0 if gamma is None else gamma) + (0.0 if beta is None else beta))
+    return 1.01 * (1.1 * d_z + (8 + z) * U * np.abs(y)) + 1e-37, 1.01 * d_mean + 1e-37, 1.01 * d_rstd
 
 
 def backward_bounds(r, g, gamma, kind, S):

@@ -8,6 +8,7 @@
 
 #include "common.cuh"
 #include "groupnorm_plan.h"
+#include "ptx.cuh"
 
 namespace {
 
@@ -15,10 +16,16 @@ struct GnDims {
   int B, S, C, G, width;  // width = C / G
 };
 
-// 1 / (1 + exp(-z)) within 7 half steps: expf 4, the sum 1, the approximate division (1 ulp) 2.  IEEE division would
-// take some eight instructions more per element, a fifth of the forward kernel's.  Below -87.3, where the sum passes
-// 2^126, the division gives 0 (the logistic function is under 1.2e-38 there).
-__device__ __forceinline__ float logistic(float z) { return __fdividef(1.0f, 1.0f + expf(-z)); }
+// 1 / (1 + exp(-z)) in four instructions; expf and IEEE division take some twenty, more than the rest of the forward
+// kernel per element.  In half steps (2^-24, relative): the product z * log2(e) is rounded, which weighs |z| in the
+// power, the approximate power and reciprocal are good to 2 ulp and 1 ulp: |z| + 4 + 1 + 2 together, less for z > 0.
+// Below z = -87.3, where the power passes 2^126, the result is 0 (the logistic function is under 1.2e-38 there).
+__device__ __forceinline__ float logistic(float z) {
+  float e, s;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + e));
+  return s;
+}
 
 template <int ACT>
 __device__ __forceinline__ float act(float z) {
@@ -42,6 +49,14 @@ __device__ __forceinline__ float act_bwd(float g, float x, float mean, float rst
   }
   const float s = logistic(z);
   return g * (s * (1.0f + z * (1.0f - s)));
+}
+
+// 1 / sqrt(v), v >= 0, rounded from a value good to 2^-40: an approximate root and one Newton step in f64, a tenth of the
+// time of f64 division and root, which every CTA would sit through between two barriers.
+__device__ __forceinline__ float inv_sqrt(double v) {
+  if (!(v > 1e-30 && v < 1e30)) return (float)(1.0 / sqrt(v));
+  const double r = (double)rsqrtf((float)v);
+  return (float)(r * fma(-0.5 * v * r, r, 1.5));
 }
 
 constexpr int kRows = 256;  // rows of x per CTA of the sums below
@@ -142,11 +157,13 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const float* x, const flo
 }
 
 // ---------------------------------------------------------------- groups that fit the registers of a cluster
-// x is read once: it stays in registers between the sums and the result (groupnorm_plan.h).  Bound by HBM, 8 bytes per
-// element forward, 12 backward.
+// x is read once: it stays in registers between the sums and the result (groupnorm_plan.h).  A cluster goes through
+// several units (a slab of groups of one sample), the next one's values on their way into shared memory while this
+// one's are worked on.  Bound by HBM, 8 bytes per element forward, 12 backward.
 struct GnTile {
   GnDims d;
   int groups, slabs, csplit, channels, rows;
+  unsigned units;  // B * slabs
 };
 
 template <int VEC>
@@ -172,294 +189,449 @@ __device__ __forceinline__ void gn_store(float* p, const GnVec<VEC>& v) {
     *p = v.e[0];
 }
 
-// Where this CTA and thread stand.
-struct GnPlace {
-  int b, grp0, groups;  // sample, first group of the slab, groups in it
-  int c0, channels;     // first channel and channels of this CTA
-  int in_slab;          // c0 minus the slab's first channel
-  int cols, lanes;      // pieces of VEC channels, rows per step
-  int col, lane;        // this thread's
-  int r0, r1;           // rows of this CTA
-  bool on;
-  bool even;            // pieces of a row fill a warp evenly: cols is a power of two up to 32
+// How a CTA's piece of a slab lies on its threads.  The same for all slabs but a narrower last one, so the divisions
+// are done once per kernel, not once per unit (where they took a third of all instructions).
+struct GnShape {
+  int groups;         // of the slab
+  int in_slab;        // first channel of this CTA, from the slab's first
+  int channels;       // of this CTA
+  int cols, lanes;    // pieces of VEC channels in a row, rows per step
+  int col, lane;      // this thread's
+  int rows;           // of this thread: lane, lane + lanes, ... of the CTA's
+  int group;          // of the thread's first channel, within the slab
+  size_t inside;      // the thread's first element, from the unit's (first position, first channel of the slab)
+  bool even;          // the pieces of a row fill a warp evenly: cols is a power of two up to 32
 };
 template <int VEC>
-__device__ __forceinline__ GnPlace gn_place(const GnTile& t, int rank, int cluster) {
-  GnPlace p;
-  const unsigned unit = blockIdx.x / cluster;
-  p.b = (int)(unit / t.slabs);
-  const int slab = (int)(unit % t.slabs);
-  p.grp0 = slab * t.groups;
-  p.groups = min(t.groups, t.d.G - p.grp0);
+__device__ __forceinline__ GnShape gn_shape(const GnTile& t, int groups, int rank) {
+  GnShape p;
+  p.groups = groups;
   p.in_slab = (rank % t.csplit) * t.channels;
-  p.c0 = p.grp0 * t.d.width + p.in_slab;
-  p.channels = min(t.channels, p.groups * t.d.width - p.in_slab);
+  p.channels = min(t.channels, groups * t.d.width - p.in_slab);
   p.cols = p.channels / VEC;
   p.lanes = kGnThreads / p.cols;
   p.col = threadIdx.x % p.cols;
   p.lane = threadIdx.x / p.cols;
-  p.r0 = min(t.d.S, (rank / t.csplit) * t.rows);
-  p.r1 = min(t.d.S, p.r0 + t.rows);
-  p.on = p.lane < p.lanes;
+  const int r0 = min(t.d.S, (rank / t.csplit) * t.rows), r1 = min(t.d.S, r0 + t.rows);
+  p.rows = p.lane < p.lanes ? max(0, (r1 - r0 - p.lane + p.lanes - 1) / p.lanes) : 0;
+  p.group = (p.in_slab + p.col * VEC) / t.d.width;
+  p.inside = (size_t)(r0 + p.lane) * t.d.C + p.in_slab + p.col * VEC;
   p.even = p.cols <= 32 && (p.cols & (p.cols - 1)) == 0;
   return p;
 }
 
-template <int ACT, int VEC, int VPT, bool GROUPED>
-__global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 1024 / kGnThreads) gn_fwd_tile_kernel(const float* x, const float* gamma, const float* beta,
-                                                                 GnTile t, double eps, float* y, float* mean_out,
-                                                                 float* rstd_out) {
-  namespace cg = cooperative_groups;
-  constexpr int PAIRS = GROUPED ? 1 : VEC;  // GROUPED: the channels of a thread's piece are all of one group
-  __shared__ double2 sm_pair[kGnThreads * PAIRS];
-  __shared__ double2 sm_sum[kGnMaxGroups];
-  __shared__ float2 sm_stat[kGnMaxGroups];
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
-  const GnPlace p = gn_place<VEC>(t, rank, ctas);
-  const int tid = threadIdx.x, warp = tid >> 5, width = t.d.width;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the kernel in front is done from here on
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const size_t base = ((size_t)p.b * t.d.S + p.r0 + p.lane) * t.d.C + p.c0 + (size_t)p.col * VEC;
+// A unit, and the way to the one that this cluster takes next.
+struct GnUnit {
+  unsigned unit, b, slab;
+};
+__device__ __forceinline__ GnUnit gn_first(const GnTile& t, unsigned unit) {
+  return GnUnit{unit, unit / t.slabs, unit % t.slabs};
+}
+__device__ __forceinline__ GnUnit gn_next(const GnTile& t, GnUnit u, const GnUnit& stride) {
+  u.unit += stride.unit, u.b += stride.b, u.slab += stride.slab;
+  if (u.slab >= (unsigned)t.slabs) u.slab -= t.slabs, u.b += 1;
+  return u;
+}
+__device__ __forceinline__ int gn_groups(const GnTile& t, const GnUnit& u) {
+  return min(t.groups, t.d.G - (int)u.slab * t.groups);
+}
+__device__ __forceinline__ size_t gn_base(const GnTile& t, const GnUnit& u) {
+  return (size_t)u.b * t.d.S * t.d.C + (size_t)u.slab * t.groups * t.d.width;
+}
+
+// The CTAs of a cluster send one another their sums: st.async into a box of the receiver, counted by an mbarrier there.
+// (A cluster barrier instead orders every earlier global store as well: each unit then waited for the results of the
+// unit before to reach L2.)  Two boxes in turn: a CTA sends for unit n + 2 only once it has everyone's sums of unit
+// n + 1, which they send after they have read those of unit n.
+template <typename T>
+struct GnMail {
+  T box[2][kGnMaxCluster][kGnMaxGroups];
+  uint64_t full[2];
+  uint32_t abort;
+};
+__device__ __forceinline__ uint32_t gn_remote(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void gn_post(uint32_t to, uint32_t bar, double2 v) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(to),
+               "l"(__double_as_longlong(v.x)), "l"(__double_as_longlong(v.y)), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void gn_post(uint32_t to, uint32_t bar, float2 v) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(to),
+               "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(bar)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void gn_mail_init(GnMail<T>& m) {
+  if (threadIdx.x == 0) {
+    ptx::mbar_init(ptx::smem_u32(&m.full[0]), 1);
+    ptx::mbar_init(ptx::smem_u32(&m.full[1]), 1);
+    m.abort = 0;
+    ptx::fence_barrier_init();
+  }
+}
+// One thread's sum of group g goes to every CTA of the cluster.
+template <typename T>
+__device__ __forceinline__ void gn_send(GnMail<T>& m, int turn, int rank, int ctas, int g, T v) {
+  if (ctas == 1) {
+    m.box[turn][0][g] = v;
+    return;
+  }
+  const uint32_t to = ptx::smem_u32(&m.box[turn][rank][g]), bar = ptx::smem_u32(&m.full[turn]);
+  for (int r = 0; r < ctas; ++r) gn_post(gn_remote(to, r), gn_remote(bar, r), v);
+}
+// The first warp waits for the sums of all CTAs (at most two seconds: then the status word says so, and the results
+// are not valid).  `round` counts the units of this CTA.
+template <typename T>
+__device__ __forceinline__ void gn_receive(GnMail<T>& m, int turn, unsigned round, int ctas, int groups, uint32_t* status) {
+  const uint32_t bar = ptx::smem_u32(&m.full[turn]);
+  if (threadIdx.x == 0) ptx::mbar_arrive_expect_tx(bar, (uint32_t)(ctas * groups * sizeof(T)));
+  __syncwarp();
+  if (!ptx::mbar_wait_bounded(bar, (round >> 1) & 1, &m.abort, 2000000000ull) && (threadIdx.x & 31) == 0)
+    atomicOr(status, VTLB_ST_GEMM_TIMEOUT);
+}
+
+// Each thread has slots of its own in shared memory, [i][thread], and reads back what it fetched itself.
+template <int VEC, int VPT>
+__device__ __forceinline__ void gn_fetch(float* slots, const float* src, const GnTile& t, const GnUnit& u, const GnShape& p) {
+  const float* from = src + gn_base(t, u) + p.inside;
   const size_t step = (size_t)p.lanes * t.d.C;
-  const int rows = p.on ? min(VPT, max(0, (p.r1 - p.r0 - p.lane + p.lanes - 1) / p.lanes)) : 0;  // of this thread
-  GnVec<VEC> v[VPT];
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(slots + threadIdx.x * VEC);
+#pragma unroll
+  for (int i = 0; i < VPT; ++i, from += step)
+    if (i < p.rows) {
+      if constexpr (VEC == 4)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * kGnThreads * 16), "l"(from) : "memory");
+      else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + i * kGnThreads * 4), "l"(from) : "memory");
+    }
+}
+template <int VEC, int VPT>
+__device__ __forceinline__ void gn_take(GnVec<VEC> (&v)[VPT], const float* slots, int rows) {
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     if (i < rows) {
-      v[i] = gn_load<VEC>(x + base + i * step);
+      v[i] = gn_load<VEC>(slots + (i * kGnThreads + threadIdx.x) * VEC);
     } else {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) v[i].e[k] = 0.0f;
     }
   }
-  // A thread's own mean K and squared distances from it in f32, then sums of x and x^2 in f64 from them: the variance
-  // loses 2^-53 of the mean square, not 2^-24, and few instructions are f64.
-  constexpr int PER = VEC / PAIRS;  // channels per pair
-  double2 acc[PAIRS];
-#pragma unroll
-  for (int q = 0; q < PAIRS; ++q) {
-    const float n = (float)(rows * PER);
-    float sum = 0.0f, dist = 0.0f;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-      for (int k = 0; k < PER; ++k) sum += v[i].e[q * PER + k];
-    const float mean = rows ? __fdividef(sum, n) : 0.0f;  // any value near the mean serves
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-      if (i < rows) {
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-          const float e = v[i].e[q * PER + k] - mean;
-          dist = fmaf(e, e, dist);
-        }
-      }
-    const double nm = (double)n * (double)mean;
-    acc[q] = make_double2(nm, fma(nm, (double)mean, (double)dist));
-  }
-  const int cq = width / PER;  // pairs per group and row
-  if (p.even && (PAIRS == 1) && (cq & (cq - 1)) == 0 && cq <= p.cols) {
-    // lanes of a warp that hold one group: the other rows' (steps of cols), then the other pieces of its channels
-    for (int o = 16; o; o >>= 1) {
-      if (o >= p.cols || o < cq) {
-        acc[0].x += __shfl_xor_sync(~0u, acc[0].x, o);
-        acc[0].y += __shfl_xor_sync(~0u, acc[0].y, o);
-      }
-    }
-    const int lane = tid & 31;
-    if (lane < p.cols && lane % cq == 0) sm_pair[warp * p.groups + lane / cq] = acc[0];
-    __syncthreads();
-    if (tid < p.groups) {
-      double2 s = sm_pair[tid];
-#pragma unroll
-      for (int w = 1; w < kGnThreads / 32; ++w) s.x += sm_pair[w * p.groups + tid].x, s.y += sm_pair[w * p.groups + tid].y;
-      sm_sum[tid] = s;
-    }
-  } else {
-#pragma unroll
-    for (int q = 0; q < PAIRS; ++q) sm_pair[tid * PAIRS + q] = acc[q];
-    __syncthreads();
-    // one warp per group of the slab: the pairs of its channels in this CTA, all rows
-    for (int g = warp; g < p.groups; g += kGnThreads / 32) {
-      const int lo = max(g * width - p.in_slab, 0) / PER, hi = min((g + 1) * width - p.in_slab, p.channels) / PER;
-      double2 s = make_double2(0.0, 0.0);
-      const int n = hi > lo ? hi - lo : 0, entries = p.channels / PER;
-      for (int i = tid & 31; i < n * p.lanes; i += 32) {
-        const double2 e = sm_pair[(i / n) * entries + lo + i % n];
-        s.x += e.x, s.y += e.y;
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
-      if ((tid & 31) == 0) sm_sum[g] = s;
-    }
-  }
-  if (ctas > 1) cluster.sync(); else __syncthreads();
-  if (tid < p.groups) {
-    double2 s = make_double2(0.0, 0.0);
-    for (int r = 0; r < ctas; ++r) {
-      const double2 e = *cluster.map_shared_rank(&sm_sum[tid], r);
-      s.x += e.x, s.y += e.y;
-    }
-    const double n = (double)t.d.S * width, mu = s.x / n, var = s.y / n - mu * mu;
-    const float2 st = make_float2((float)mu, (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + eps)));
-    sm_stat[tid] = st;
-    if (rank == 0) {
-      const size_t k = (size_t)p.b * t.d.G + p.grp0 + tid;
-      mean_out[k] = st.x;
-      rstd_out[k] = st.y;
-    }
-  }
-  if (ctas > 1) cluster.sync(); else __syncthreads();  // (and no CTA leaves while another reads its sums)
-  if (!p.on) return;
-  float mu[VEC], a[VEC], be[VEC];
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) {
-    const int c = p.col * VEC + k;
-    const float2 st = sm_stat[(p.in_slab + (GROUPED ? p.col * VEC : c)) / width];
-    mu[k] = st.x;
-    a[k] = gamma ? st.y * __ldg(gamma + p.c0 + c) : st.y;
-    be[k] = beta ? __ldg(beta + p.c0 + c) : 0.0f;
-  }
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    if (i >= rows) break;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) v[i].e[k] = act<ACT>(fmaf(__fsub_rn(v[i].e[k], mu[k]), a[k], be[k]));
-    gn_store<VEC>(y + base + i * step, v[i]);
-  }
 }
 
-// Backward.  The channel sums of each CTA go to `sums` [B * rsplit][C] (dz * h, dz) for gn_params_kernel.
-template <int ACT, int VEC, int VPT>
-__global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 1024 / kGnThreads) gn_bwd_tile_kernel(const float* g, const float* x, const float* gamma,
-                                                                 const float* beta, const float* mean, const float* rstd,
-                                                                 GnTile t, float* dx, float2* sums) {
+template <int ACT, int VEC, int VPT, bool GROUPED>
+__global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 1024 / kGnThreads)
+    gn_fwd_tile_kernel(const float* x, const float* gamma, const float* beta, GnTile t, double eps, float* y,
+                       float* mean_out, float* rstd_out, uint32_t* status) {
   namespace cg = cooperative_groups;
-  __shared__ float2 sm_part[kGnThreads * VEC];  // [lane][channel]
-  __shared__ float2 sm_chan[kGnThreads * VEC];
-  __shared__ float2 sm_sum[kGnMaxGroups];
-  __shared__ float2 sm_coef[kGnMaxGroups];
+  constexpr int PAIRS = GROUPED ? 1 : VEC;  // GROUPED: the channels of a thread's piece are all of one group
+  constexpr int PER = VEC / PAIRS;          // channels per pair of sums
+  __shared__ double2 sm_pair[kGnThreads * PAIRS];
+  __shared__ GnMail<double2> mail;
+  __shared__ float2 sm_stat[kGnMaxGroups];
+  extern __shared__ __align__(16) float slots[];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
-  const GnPlace p = gn_place<VEC>(t, rank, ctas);
   const int tid = threadIdx.x, warp = tid >> 5, width = t.d.width;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const GnUnit stride = gn_first(t, gridDim.x / ctas);
+  GnUnit u = gn_first(t, blockIdx.x / ctas);
+  GnShape p = gn_shape<VEC>(t, gn_groups(t, u), rank);
+  const int cq = width / PER;  // pairs per group and row
+  const bool cq_even = PAIRS == 1 && (cq & (cq - 1)) == 0;
+  const double part = 1.0 / ((double)t.d.S * width);
+  gn_mail_init(mail);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the kernel in front is done from here on
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const size_t base = ((size_t)p.b * t.d.S + p.r0 + p.lane) * t.d.C + p.c0 + (size_t)p.col * VEC;
-  const size_t step = (size_t)p.lanes * t.d.C;
-  const int rows = p.on ? min(VPT, max(0, (p.r1 - p.r0 - p.lane + p.lanes - 1) / p.lanes)) : 0;
-  GnVec<VEC> vx[VPT], vg[VPT];
+  gn_fetch<VEC, VPT>(slots, x, t, u, p);
+  if (ctas > 1) cluster.sync();  // everyone's boxes are ready
+  for (unsigned round = 0;; ++round) {
+    const int turn = round & 1;
+    GnVec<VEC> v[VPT];
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    gn_take(v, slots, p.rows);
+    // A thread's own mean K and squared distances from it in f32, then sums of x and x^2 in f64 from them: the variance
+    // loses 2^-53 of the mean square, not 2^-24, and few instructions are f64.
+    double2 acc[PAIRS];
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    if (i < rows) {
-      vx[i] = gn_load<VEC>(x + base + i * step);
-      vg[i] = gn_load<VEC>(g + base + i * step);
+    for (int q = 0; q < PAIRS; ++q) {
+      const float n = (float)(p.rows * PER);
+      float sum = 0.0f, dist = 0.0f;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int k = 0; k < PER; ++k) sum += v[i].e[q * PER + k];
+      const float mean = p.rows ? __fdividef(sum, n) : 0.0f;  // any value near the mean serves
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if (i < p.rows) {
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            const float e = v[i].e[q * PER + k] - mean;
+            dist = fmaf(e, e, dist);
+          }
+        }
+      const double nm = (double)n * (double)mean;
+      acc[q] = make_double2(nm, fma(nm, (double)mean, (double)dist));
+    }
+    const bool shuffle = p.even && cq_even && cq <= p.cols;
+    if (shuffle) {
+      // lanes of a warp that hold one group: the other rows' (steps of cols), then the other pieces of its channels
+#pragma unroll
+      for (int o = 16; o; o >>= 1) {
+        if (o >= p.cols || o < cq) {
+          acc[0].x += __shfl_xor_sync(~0u, acc[0].x, o);
+          acc[0].y += __shfl_xor_sync(~0u, acc[0].y, o);
+        }
+      }
+      const int lane = tid & 31;
+      if (lane < p.cols && (lane & (cq - 1)) == 0) sm_pair[warp * p.groups + p.group] = acc[0];
     } else {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) vx[i].e[k] = vg[i].e[k] = 0.0f;
+      for (int q = 0; q < PAIRS; ++q) sm_pair[tid * PAIRS + q] = acc[q];
     }
-  }
-  float mu[VEC], rs[VEC], ga[VEC], be[VEC];
-  if (p.on) {
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      const int c = p.col * VEC + k;
-      const size_t st = (size_t)p.b * t.d.G + p.grp0 + (p.in_slab + c) / width;
-      mu[k] = __ldg(mean + st), rs[k] = __ldg(rstd + st);
-      ga[k] = gamma ? __ldg(gamma + p.c0 + c) : 1.0f;
-      be[k] = beta ? __ldg(beta + p.c0 + c) : 0.0f;
+    __syncthreads();  // the sums are there, and every thread has used its slots
+    const GnUnit next = gn_next(t, u, stride);
+    if (next.unit < t.units) {
+      if (gn_groups(t, next) == p.groups)
+        gn_fetch<VEC, VPT>(slots, x, t, next, p);
+      else
+        gn_fetch<VEC, VPT>(slots, x, t, next, gn_shape<VEC>(t, gn_groups(t, next), rank));
     }
-  }
-  float2 acc[VEC] = {};
+    if (shuffle) {
+      if (tid < p.groups) {
+        double2 s = sm_pair[tid];
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    if (i >= rows) break;
+        for (int w = 1; w < kGnThreads / 32; ++w) s.x += sm_pair[w * p.groups + tid].x, s.y += sm_pair[w * p.groups + tid].y;
+        gn_send(mail, turn, rank, ctas, tid, s);
+      }
+    } else {
+      // one warp per group of the slab: the pairs of its channels in this CTA, all rows
+      for (int g = warp; g < p.groups; g += kGnThreads / 32) {
+        const int lo = max(g * width - p.in_slab, 0) / PER, hi = min((g + 1) * width - p.in_slab, p.channels) / PER;
+        double2 s = make_double2(0.0, 0.0);
+        const int n = hi > lo ? hi - lo : 0, entries = p.channels / PER;
+        for (int i = tid & 31; i < n * p.lanes; i += 32) {
+          const double2 e = sm_pair[(i / n) * entries + lo + i % n];
+          s.x += e.x, s.y += e.y;
+        }
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      const float h = __fmul_rn(__fsub_rn(vx[i].e[k], mu[k]), rs[k]);
-      const float dz = act_bwd<ACT>(vg[i].e[k], vx[i].e[k], mu[k], rs[k], ga[k], be[k], h);
-      acc[k].x = fmaf(dz, h, acc[k].x);
-      acc[k].y += dz;
-      vx[i].e[k] = h, vg[i].e[k] = dz;  // what dx is made of
+        for (int o = 16; o; o >>= 1) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
+        if ((tid & 31) == 0) gn_send(mail, turn, rank, ctas, g, s);
+      }
+      if (ctas == 1) __syncthreads();
     }
-  }
-  int parts;  // rows of partial sums per channel in sm_chan
-  if (p.even) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      if (o < p.cols) break;
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        acc[k].x += __shfl_xor_sync(~0u, acc[k].x, o);
-        acc[k].y += __shfl_xor_sync(~0u, acc[k].y, o);
+    if (warp == 0 && ctas > 1) gn_receive(mail, turn, round, ctas, p.groups, status);
+    if (tid < p.groups) {
+      double2 s = make_double2(0.0, 0.0);
+      for (int r = 0; r < ctas; ++r) s.x += mail.box[turn][r][tid].x, s.y += mail.box[turn][r][tid].y;
+      const double mu = s.x * part, var = s.y * part - mu * mu;
+      const float2 st = make_float2((float)mu, inv_sqrt((var < 0.0 ? 0.0 : var) + eps));
+      sm_stat[tid] = st;
+      if (rank == 0) {
+        const size_t k = (size_t)u.b * t.d.G + u.slab * t.groups + tid;
+        mean_out[k] = st.x;
+        rstd_out[k] = st.y;
       }
     }
-    parts = kGnThreads / 32;
-    if ((tid & 31) < p.cols) {
+    __syncthreads();
+    if (p.rows) {
+      const int c = (int)u.slab * t.groups * width + p.in_slab + p.col * VEC;
+      float mu[VEC], a[VEC], be[VEC];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) sm_chan[warp * p.channels + p.col * VEC + k] = acc[k];
+      for (int k = 0; k < VEC; ++k) {
+        const float2 st = sm_stat[GROUPED ? p.group : (p.in_slab + p.col * VEC + k) / width];
+        mu[k] = st.x;
+        a[k] = gamma ? st.y * __ldg(gamma + c + k) : st.y;
+        be[k] = beta ? __ldg(beta + c + k) : 0.0f;
+      }
+      float* to = y + gn_base(t, u) + p.inside;
+      const size_t step = (size_t)p.lanes * t.d.C;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i, to += step) {
+        if (i >= p.rows) break;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[i].e[k] = act<ACT>(fmaf(__fsub_rn(v[i].e[k], mu[k]), a[k], be[k]));
+        gn_store<VEC>(to, v[i]);
+      }
     }
-  } else {
-    if (p.on) {
+    if (next.unit >= t.units) break;
+    u = next;
+    if (gn_groups(t, u) != p.groups) p = gn_shape<VEC>(t, gn_groups(t, u), rank);
+  }
+  if (ctas > 1) cluster.sync();  // no CTA leaves while another may still send to it
+}
+
+// Backward.  The channel sums of each CTA go to `sums` [B * rsplit][C] (dz * h, dz) for gn_params_tile_kernel.
+template <int ACT, int VEC, int VPT>
+__global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 1024 / kGnThreads)
+    gn_bwd_tile_kernel(const float* g, const float* x, const float* gamma, const float* beta, const float* mean,
+                       const float* rstd, GnTile t, float* dx, float2* sums, uint32_t* status) {
+  namespace cg = cooperative_groups;
+  __shared__ float2 sm_part[kGnThreads * VEC];  // [lane][channel]
+  __shared__ float2 sm_chan[kGnThreads * VEC];  // [part][channel]
+  __shared__ GnMail<float2> mail;
+  __shared__ float2 sm_coef[kGnMaxGroups];
+  extern __shared__ __align__(16) float slots[];
+  float* slots_g = slots + VPT * kGnThreads * VEC;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
+  const int tid = threadIdx.x, warp = tid >> 5, width = t.d.width;
+  const GnUnit stride = gn_first(t, gridDim.x / ctas);
+  GnUnit u = gn_first(t, blockIdx.x / ctas);
+  GnShape p = gn_shape<VEC>(t, gn_groups(t, u), rank);
+  const float count = (float)t.d.S * (float)width;
+  const bool aligned_groups = width <= 32 && (width & (width - 1)) == 0 && t.csplit == 1;
+  gn_mail_init(mail);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  gn_fetch<VEC, VPT>(slots, x, t, u, p);
+  gn_fetch<VEC, VPT>(slots_g, g, t, u, p);
+  if (ctas > 1) cluster.sync();  // everyone's boxes are ready
+  for (unsigned round = 0;; ++round) {
+    const int turn = round & 1;
+    GnVec<VEC> vx[VPT], vg[VPT];
+    const int c = (int)u.slab * t.groups * width + p.in_slab + p.col * VEC;  // first channel of this thread
+    float rs[VEC], ga[VEC];
+    float2 acc[VEC] = {};
+    {
+      float mu[VEC], be[VEC];
+      if (p.rows) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const size_t st = (size_t)u.b * t.d.G + u.slab * t.groups + (p.in_slab + p.col * VEC + k) / width;
+          mu[k] = __ldg(mean + st), rs[k] = __ldg(rstd + st);
+          ga[k] = gamma ? __ldg(gamma + c + k) : 1.0f;
+          be[k] = beta ? __ldg(beta + c + k) : 0.0f;
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      gn_take(vx, slots, p.rows);
+      gn_take(vg, slots_g, p.rows);
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        if (i >= p.rows) break;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const float h = __fmul_rn(__fsub_rn(vx[i].e[k], mu[k]), rs[k]);
+          const float dz = act_bwd<ACT>(vg[i].e[k], vx[i].e[k], mu[k], rs[k], ga[k], be[k], h);
+          acc[k].x = fmaf(dz, h, acc[k].x);
+          acc[k].y += dz;
+          vx[i].e[k] = h, vg[i].e[k] = dz;  // what dx is made of
+        }
+      }
+    }
+    if (p.even) {
+#pragma unroll
+      for (int o = 16; o; o >>= 1) {
+        if (o < p.cols) break;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          acc[k].x += __shfl_xor_sync(~0u, acc[k].x, o);
+          acc[k].y += __shfl_xor_sync(~0u, acc[k].y, o);
+        }
+      }
+      if ((tid & 31) < p.cols) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) sm_chan[warp * p.channels + p.col * VEC + k] = acc[k];
+      }
+    } else if (p.lane < p.lanes) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) sm_part[p.lane * p.channels + p.col * VEC + k] = acc[k];
     }
-    __syncthreads();
-    parts = max(1, min(kGnThreads / p.channels, p.lanes));
-    for (int i = tid; i < parts * p.channels; i += kGnThreads) {
-      const int part = i / p.channels, c = i % p.channels;
-      float2 s = make_float2(0.f, 0.f);
-      for (int l = part; l < p.lanes; l += parts) {
-        const float2 e = sm_part[l * p.channels + c];
-        s.x += e.x, s.y += e.y;
+    __syncthreads();  // the sums are there, and every thread has used its slots
+    const GnUnit next = gn_next(t, u, stride);
+    if (next.unit < t.units) {
+      const int groups = gn_groups(t, next);
+      if (groups == p.groups) {
+        gn_fetch<VEC, VPT>(slots, x, t, next, p);
+        gn_fetch<VEC, VPT>(slots_g, g, t, next, p);
+      } else {
+        const GnShape q = gn_shape<VEC>(t, groups, rank);
+        gn_fetch<VEC, VPT>(slots, x, t, next, q);
+        gn_fetch<VEC, VPT>(slots_g, g, t, next, q);
       }
-      sm_chan[i] = s;
     }
-  }
-  __syncthreads();
-  for (int c = tid; c < p.channels; c += kGnThreads) {
-    float2 s = sm_chan[c];
-    for (int q = 1; q < parts; ++q) {
-      const float2 e = sm_chan[q * p.channels + c];
-      s.x += e.x, s.y += e.y;
+    int parts = kGnThreads / 32;  // rows of sums per channel in sm_chan
+    if (!p.even) {
+      parts = max(1, min(kGnThreads / p.channels, p.lanes));
+      for (int i = tid; i < parts * p.channels; i += kGnThreads) {
+        float2 s = make_float2(0.f, 0.f);
+        for (int l = i / p.channels; l < p.lanes; l += parts) {
+          const float2 e = sm_part[l * p.channels + i % p.channels];
+          s.x += e.x, s.y += e.y;
+        }
+        sm_chan[i] = s;
+      }
+      __syncthreads();
     }
-    if (sums) sums[((size_t)p.b * (ctas / t.csplit) + rank / t.csplit) * t.d.C + p.c0 + c] = s;
-    const float w = gamma ? __ldg(gamma + p.c0 + c) : 1.0f;
-    sm_part[c] = make_float2(w * s.x, w * s.y);
-  }
-  if (!dx) return;  // (all CTAs of the cluster alike: nobody reads another's shared memory)
-  __syncthreads();
-  for (int gr = warp; gr < p.groups; gr += kGnThreads / 32) {
-    const int lo = max(gr * width - p.in_slab, 0), hi = min((gr + 1) * width - p.in_slab, p.channels);
-    float2 s = make_float2(0.f, 0.f);
-    for (int c = lo + (tid & 31); c < hi; c += 32) s.x += sm_part[c].x, s.y += sm_part[c].y;
+    for (int c0 = warp * 32; c0 < p.channels; c0 += kGnThreads) {  // whole warps
+      const int ch = c0 + (tid & 31);
+      float2 s = make_float2(0.f, 0.f);
+      if (ch < p.channels) {
+        s = sm_chan[ch];
+        for (int q = 1; q < parts; ++q) {
+          const float2 e = sm_chan[q * p.channels + ch];
+          s.x += e.x, s.y += e.y;
+        }
+        const int at = (int)u.slab * t.groups * width + p.in_slab + ch;
+        if (sums) sums[((size_t)u.b * (ctas / t.csplit) + rank / t.csplit) * t.d.C + at] = s;
+        const float w = gamma ? __ldg(gamma + at) : 1.0f;
+        s = make_float2(w * s.x, w * s.y);
+      }
+      if (aligned_groups) {  // a group's channels are neighbouring lanes
 #pragma unroll
-    for (int o = 16; o; o >>= 1) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
-    if ((tid & 31) == 0) sm_sum[gr] = s;
-  }
-  if (ctas > 1) cluster.sync(); else __syncthreads();
-  if (tid < p.groups) {
-    float2 s = make_float2(0.f, 0.f);
-    for (int r = 0; r < ctas; ++r) {
-      const float2 e = *cluster.map_shared_rank(&sm_sum[tid], r);
-      s.x += e.x, s.y += e.y;
+        for (int o = 16; o; o >>= 1)
+          if (o < width) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
+        if (dx && ch < p.channels && (ch & (width - 1)) == 0) gn_send(mail, turn, rank, ctas, ch / width, s);
+      } else if (ch < p.channels) {
+        sm_part[ch] = s;
+      }
     }
-    const float n = (float)t.d.S * (float)width;
-    sm_coef[tid] = make_float2(s.x / n, s.y / n);
+    if (dx) {
+      if (!aligned_groups) {
+        __syncthreads();
+        for (int gr = warp; gr < p.groups; gr += kGnThreads / 32) {
+          const int lo = max(gr * width - p.in_slab, 0), hi = min((gr + 1) * width - p.in_slab, p.channels);
+          float2 s = make_float2(0.f, 0.f);
+          for (int ch = lo + (tid & 31); ch < hi; ch += 32) s.x += sm_part[ch].x, s.y += sm_part[ch].y;
+#pragma unroll
+          for (int o = 16; o; o >>= 1) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
+          if ((tid & 31) == 0) gn_send(mail, turn, rank, ctas, gr, s);
+        }
+      }
+      if (ctas == 1) __syncthreads();
+      if (warp == 0 && ctas > 1) gn_receive(mail, turn, round, ctas, p.groups, status);
+      if (tid < p.groups) {
+        float2 s = make_float2(0.f, 0.f);
+        for (int r = 0; r < ctas; ++r) s.x += mail.box[turn][r][tid].x, s.y += mail.box[turn][r][tid].y;
+        sm_coef[tid] = make_float2(s.x / count, s.y / count);
+      }
+      __syncthreads();
+      if (p.rows) {
+        float2 cf[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) cf[k] = sm_coef[(p.in_slab + p.col * VEC + k) / width];
+        float* to = dx + gn_base(t, u) + p.inside;
+        const size_t step = (size_t)p.lanes * t.d.C;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i, to += step) {
+          if (i >= p.rows) break;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) vx[i].e[k] = rs[k] * (ga[k] * vg[i].e[k] - cf[k].y - vx[i].e[k] * cf[k].x);
+          gn_store<VEC>(to, vx[i]);
+        }
+      }
+    } else {
+      __syncthreads();
+    }
+    if (next.unit >= t.units) break;
+    u = next;
+    if (gn_groups(t, u) != p.groups) p = gn_shape<VEC>(t, gn_groups(t, u), rank);
   }
-  if (ctas > 1) cluster.sync(); else __syncthreads();
-  if (!p.on) return;
-  float2 cf[VEC];
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) cf[k] = sm_coef[(p.in_slab + p.col * VEC + k) / width];
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    if (i >= rows) break;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) vx[i].e[k] = rs[k] * (ga[k] * vg[i].e[k] - cf[k].y - vx[i].e[k] * cf[k].x);
-    gn_store<VEC>(dx + base + i * step, vx[i]);
-  }
+  if (ctas > 1) cluster.sync();
 }
 
 // dgamma and dbeta from the channel sums: 32 channels and eight stretches of rows per CTA.
@@ -484,11 +656,14 @@ __global__ void __launch_bounds__(256) gn_params_tile_kernel(const float2* sums,
   if (dbeta) dbeta[c] = (float)s.y;
 }
 
+// Launches as many clusters as the GPU holds at a time (each goes on to further units), at most one per unit.
 template <typename... KArgs, typename... Args>
-cudaError_t cluster_launch(vtlb_ctx* ctx, void (*kern)(KArgs...), unsigned grid, int cluster, Args&&... args) {
+cudaError_t cluster_launch(vtlb_ctx* ctx, std::atomic<int>* resident, void (*kern)(KArgs...), unsigned units, int cluster,
+                           size_t smem, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = dim3(cluster);
   cfg.blockDim = dim3(kGnThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = ctx->stream;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -497,10 +672,35 @@ cudaError_t cluster_launch(vtlb_ctx* ctx, void (*kern)(KArgs...), unsigned grid,
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  unsigned clusters = units;
+  if (units > 8) {
+    int fit = resident[cluster].load(std::memory_order_relaxed);
+    if (!fit) {  // asked once per kernel and cluster size: the library runs on one kind of GPU
+      if ((e = cudaOccupancyMaxActiveClusters(&fit, kern, &cfg)) != cudaSuccess) return e;
+      if (fit < 1) fit = 1;
+      resident[cluster].store(fit, std::memory_order_relaxed);
+    }
+    if (clusters > (unsigned)fit) clusters = (unsigned)fit;
+  }
+  cfg.gridDim = dim3(clusters * cluster);
   return cudaLaunchKernelEx(&cfg, kern, static_cast<Args&&>(args)...);
 }
+template <int ACT, int VEC, int VPT, bool GROUPED, typename... Args>
+cudaError_t fwd_tile(vtlb_ctx* ctx, const GnTile& t, int cluster, Args... args) {
+  static std::atomic<int> resident[kGnMaxCluster + 1];
+  return cluster_launch(ctx, resident, gn_fwd_tile_kernel<ACT, VEC, VPT, GROUPED>, t.units, cluster,
+                        (size_t)kGnThreads * VPT * VEC * 4, args...);
+}
+template <int ACT, int VEC, int VPT, typename... Args>
+cudaError_t bwd_tile(vtlb_ctx* ctx, const GnTile& t, int cluster, Args... args) {
+  static std::atomic<int> resident[kGnMaxCluster + 1];
+  return cluster_launch(ctx, resident, gn_bwd_tile_kernel<ACT, VEC, VPT>, t.units, cluster,
+                        (size_t)kGnThreads * VPT * VEC * 8, args...);
+}
 
-GnTile tile_of(const GnDims& d, const GnPlan& p) { return GnTile{d, p.groups, p.slabs, p.csplit, p.channels, p.rows}; }
+GnTile tile_of(const GnDims& d, const GnPlan& p) { return GnTile{d, p.groups, p.slabs, p.csplit, p.channels, p.rows, (unsigned)d.B * (unsigned)p.slabs}; }
 
 int check_dims(vtlb_ctx* ctx, const char* fn, int B, int S, int C, int groups, int act_kind, GnDims* d) {
   if (B <= 0 || S <= 0 || C <= 0 || groups <= 0 || C % groups)
@@ -516,14 +716,13 @@ int check_dims(vtlb_ctx* ctx, const char* fn, int B, int S, int C, int groups, i
 template <int ACT>
 int gn_forward(vtlb_ctx* ctx, const float* x, GnDims d, const float* gamma, const float* beta, double eps, float* y,
                float* mean, float* rstd) {
-  const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, vtlb_aligned16(x) && vtlb_aligned16(y), 8, 16, ctx->sm_count);
+  const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, vtlb_aligned16(x) && vtlb_aligned16(y), 16, 16, ctx->sm_count);
   if (plan.on_chip) {
     const GnTile t = tile_of(d, plan);
     const int cluster = plan.csplit * plan.rsplit;
-    const unsigned grid = (unsigned)((size_t)d.B * plan.slabs * cluster);
     const bool grouped = plan.vec == 1 || d.width % 4 == 0;
 #define VTLB_GN_FWD(VEC, VPT, GROUPED) \
-  cluster_launch(ctx, gn_fwd_tile_kernel<ACT, VEC, VPT, GROUPED>, grid, cluster, x, gamma, beta, t, eps, y, mean, rstd)
+  fwd_tile<ACT, VEC, VPT, GROUPED>(ctx, t, cluster, x, gamma, beta, t, eps, y, mean, rstd, ctx->d_status)
 #define VTLB_GN_FWD_VPT(VPT) \
   case VPT:                  \
     VTLB_CUDA(ctx, plan.vec == 1 ? VTLB_GN_FWD(1, VPT, true) : grouped ? VTLB_GN_FWD(4, VPT, true) : VTLB_GN_FWD(4, VPT, false)); \
@@ -559,19 +758,18 @@ template <int ACT>
 int gn_backward(vtlb_ctx* ctx, const float* g, const float* x, GnDims d, const float* gamma, const float* beta,
                 const float* mean, const float* rstd, float* dx, float* dgamma, float* dbeta) {
   const bool aligned = vtlb_aligned16(x) && vtlb_aligned16(g) && vtlb_aligned16(dx);
-  const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, aligned, 4, 8, ctx->sm_count);
+  const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, aligned, 8, 8, ctx->sm_count);
   vtlb_workspace ws(ctx);
   void* scratch = nullptr;
   if (plan.on_chip) {
     const GnTile t = tile_of(d, plan);
     const int cluster = plan.csplit * plan.rsplit;
-    const unsigned grid = (unsigned)((size_t)d.B * plan.slabs * cluster);
     const int rows = d.B * plan.rsplit;
     if (dgamma || dbeta)
       if (int rc = ws.get((size_t)rows * d.C * sizeof(float2), &scratch)) return rc;
     float2* sums = (float2*)scratch;
 #define VTLB_GN_BWD(VEC, VPT) \
-  cluster_launch(ctx, gn_bwd_tile_kernel<ACT, VEC, VPT>, grid, cluster, g, x, gamma, beta, mean, rstd, t, dx, sums)
+  bwd_tile<ACT, VEC, VPT>(ctx, t, cluster, g, x, gamma, beta, mean, rstd, t, dx, sums, ctx->d_status)
 #define VTLB_GN_BWD_VPT(VPT) \
   case VPT:                  \
     VTLB_CUDA(ctx, plan.vec == 1 ? VTLB_GN_BWD(1, VPT) : VTLB_GN_BWD(4, VPT)); \

@@ -15,7 +15,7 @@ struct GnPlan {
   int rows;         // per CTA, the last stretch may have fewer
 };
 
-constexpr int kGnThreads = 512, kGnMaxGroups = 32, kGnMaxCluster = 8;
+constexpr int kGnThreads = 256, kGnMaxGroups = 32, kGnMaxCluster = 8;
 
 // `most`: the largest vpt of the kernel at hand (registers), `usual`: the one it runs best with.
 inline GnPlan gn_plan(int B, int S, int C, int G, bool aligned, int usual, int most, int sm_count) {
