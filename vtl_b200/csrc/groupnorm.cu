@@ -48,7 +48,7 @@ __device__ __forceinline__ float act_bwd(float g, float x, float mean, float rst
     return z < 0.0f ? 0.0f : g;
   }
   const float s = logistic(z);
-  return g * (s * (1.0f + z * (1.0f - s)));
+  return g * fmaf(s, fmaf(-z, s, z), s);  // s + s * (z - z * s)
 }
 
 // 1 / sqrt(v), v >= 0, rounded from a value good to 2^-40: an approximate root and one Newton step in f64, a tenth of the
@@ -164,6 +164,7 @@ struct GnTile {
   GnDims d;
   int groups, slabs, csplit, channels, rows;
   unsigned units;  // B * slabs
+  uint32_t zero;   // 0, unknown to the compiler (gn_after)
 };
 
 template <int VEC>
@@ -294,12 +295,24 @@ __device__ __forceinline__ void gn_receive(GnMail<T>& m, int turn, unsigned roun
     atomicOr(status, VTLB_ST_GEMM_TIMEOUT);
 }
 
-// Each thread has slots of its own in shared memory, [i][thread], and reads back what it fetched itself.
+// Each thread has slots of its own in shared memory, [i][thread], and reads back what it fetched itself.  A slot is
+// filled again as soon as it has been read: `after`, a zero made from the values read, is part of the address, so that
+// the copy cannot start before they are in registers.
 template <int VEC, int VPT>
-__device__ __forceinline__ void gn_fetch(float* slots, const float* src, const GnTile& t, const GnUnit& u, const GnShape& p) {
+__device__ __forceinline__ uint32_t gn_after(const GnTile& t, const GnVec<VEC> (&v)[VPT]) {
+  uint32_t all = 0;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) all |= __float_as_uint(v[i].e[k]);
+  return all & t.zero;
+}
+template <int VEC, int VPT>
+__device__ __forceinline__ void gn_fetch(float* slots, const float* src, const GnTile& t, const GnUnit& u, const GnShape& p,
+                                         uint32_t after = 0) {
   const float* from = src + gn_base(t, u) + p.inside;
   const size_t step = (size_t)p.lanes * t.d.C;
-  const uint32_t to = (uint32_t)__cvta_generic_to_shared(slots + threadIdx.x * VEC);
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(slots + threadIdx.x * VEC) + after;
 #pragma unroll
   for (int i = 0; i < VPT; ++i, from += step)
     if (i < p.rows) {
@@ -352,6 +365,14 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 
     GnVec<VEC> v[VPT];
     asm volatile("cp.async.wait_all;" ::: "memory");
     gn_take(v, slots, p.rows);
+    const GnUnit next = gn_next(t, u, stride);
+    if (next.unit < t.units) {
+      const uint32_t after = gn_after(t, v);
+      if (gn_groups(t, next) == p.groups)
+        gn_fetch<VEC, VPT>(slots, x, t, next, p, after);
+      else
+        gn_fetch<VEC, VPT>(slots, x, t, next, gn_shape<VEC>(t, gn_groups(t, next), rank), after);
+    }
     // A thread's own mean K and squared distances from it in f32, then sums of x and x^2 in f64 from them: the variance
     // loses 2^-53 of the mean square, not 2^-24, and few instructions are f64.
     double2 acc[PAIRS];
@@ -392,14 +413,7 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 
 #pragma unroll
       for (int q = 0; q < PAIRS; ++q) sm_pair[tid * PAIRS + q] = acc[q];
     }
-    __syncthreads();  // the sums are there, and every thread has used its slots
-    const GnUnit next = gn_next(t, u, stride);
-    if (next.unit < t.units) {
-      if (gn_groups(t, next) == p.groups)
-        gn_fetch<VEC, VPT>(slots, x, t, next, p);
-      else
-        gn_fetch<VEC, VPT>(slots, x, t, next, gn_shape<VEC>(t, gn_groups(t, next), rank));
-    }
+    __syncthreads();
     if (shuffle) {
       if (tid < p.groups) {
         double2 s = sm_pair[tid];
@@ -465,7 +479,7 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 
 }
 
 // Backward.  The channel sums of each CTA go to `sums` [B * rsplit][C] (dz * h, dz) for gn_params_tile_kernel.
-template <int ACT, int VEC, int VPT>
+template <int ACT, int VEC, int VPT, bool GROUPED>
 __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 1024 / kGnThreads)
     gn_bwd_tile_kernel(const float* g, const float* x, const float* gamma, const float* beta, const float* mean,
                        const float* rstd, GnTile t, float* dx, float2* sums, uint32_t* status) {
@@ -483,40 +497,64 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 
   GnUnit u = gn_first(t, blockIdx.x / ctas);
   GnShape p = gn_shape<VEC>(t, gn_groups(t, u), rank);
   const float count = (float)t.d.S * (float)width;
+  const int stretches = ctas / t.csplit, stretch = rank / t.csplit, shift = __ffs(width) - 1;
   const bool aligned_groups = width <= 32 && (width & (width - 1)) == 0 && t.csplit == 1;
   gn_mail_init(mail);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  gn_fetch<VEC, VPT>(slots, x, t, u, p);
-  gn_fetch<VEC, VPT>(slots_g, g, t, u, p);
+  // (the next unit's statistics, which nothing else brings nearer than HBM, come along with its values)
+  constexpr int NG = GROUPED ? 1 : VEC;
+  float mu_next[NG], rs_next[NG];
+  const auto fetch = [&](const GnUnit& w, const GnShape& q, uint32_t after) {
+    gn_fetch<VEC, VPT>(slots, x, t, w, q, after);
+    gn_fetch<VEC, VPT>(slots_g, g, t, w, q, after);
+    if (q.rows) {
+      const size_t st = (size_t)w.b * t.d.G + w.slab * t.groups;
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        const int gr = GROUPED ? q.group : (q.in_slab + q.col * VEC + k) / width;
+        mu_next[k] = __ldg(mean + st + gr), rs_next[k] = __ldg(rstd + st + gr);
+      }
+    }
+  };
+  fetch(u, p, 0);
   if (ctas > 1) cluster.sync();  // everyone's boxes are ready
   for (unsigned round = 0;; ++round) {
     const int turn = round & 1;
     GnVec<VEC> vx[VPT], vg[VPT];
-    const int c = (int)u.slab * t.groups * width + p.in_slab + p.col * VEC;  // first channel of this thread
-    float rs[VEC], ga[VEC];
+    const GnUnit next = gn_next(t, u, stride);
+    const int slab_c = (int)u.slab * t.groups * width + p.in_slab;  // first channel of this CTA
+    const float own_gamma = gamma && tid < p.channels ? __ldg(gamma + slab_c + tid) : 1.0f;  // of channel tid, for the sums
+    float rs[NG], ga[VEC];
     float2 acc[VEC] = {};
     {
-      float mu[VEC], be[VEC];
+      float mu[NG], be[VEC];
       if (p.rows) {
 #pragma unroll
+        for (int k = 0; k < NG; ++k) mu[k] = mu_next[k], rs[k] = rs_next[k];
+#pragma unroll
         for (int k = 0; k < VEC; ++k) {
-          const size_t st = (size_t)u.b * t.d.G + u.slab * t.groups + (p.in_slab + p.col * VEC + k) / width;
-          mu[k] = __ldg(mean + st), rs[k] = __ldg(rstd + st);
-          ga[k] = gamma ? __ldg(gamma + c + k) : 1.0f;
-          be[k] = beta ? __ldg(beta + c + k) : 0.0f;
+          ga[k] = gamma ? __ldg(gamma + slab_c + p.col * VEC + k) : 1.0f;
+          be[k] = beta ? __ldg(beta + slab_c + p.col * VEC + k) : 0.0f;
         }
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
       gn_take(vx, slots, p.rows);
       gn_take(vg, slots_g, p.rows);
+      if (next.unit < t.units) {
+        const uint32_t after = gn_after(t, vx) | gn_after(t, vg);
+        if (gn_groups(t, next) == p.groups)
+          fetch(next, p, after);
+        else
+          fetch(next, gn_shape<VEC>(t, gn_groups(t, next), rank), after);
+      }
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         if (i >= p.rows) break;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-          const float h = __fmul_rn(__fsub_rn(vx[i].e[k], mu[k]), rs[k]);
-          const float dz = act_bwd<ACT>(vg[i].e[k], vx[i].e[k], mu[k], rs[k], ga[k], be[k], h);
+          const float m = mu[k % NG], r = rs[k % NG], h = __fmul_rn(__fsub_rn(vx[i].e[k], m), r);
+          const float dz = act_bwd<ACT>(vg[i].e[k], vx[i].e[k], m, r, ga[k], be[k], h);
           acc[k].x = fmaf(dz, h, acc[k].x);
           acc[k].y += dz;
           vx[i].e[k] = h, vg[i].e[k] = dz;  // what dx is made of
@@ -541,19 +579,7 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 
 #pragma unroll
       for (int k = 0; k < VEC; ++k) sm_part[p.lane * p.channels + p.col * VEC + k] = acc[k];
     }
-    __syncthreads();  // the sums are there, and every thread has used its slots
-    const GnUnit next = gn_next(t, u, stride);
-    if (next.unit < t.units) {
-      const int groups = gn_groups(t, next);
-      if (groups == p.groups) {
-        gn_fetch<VEC, VPT>(slots, x, t, next, p);
-        gn_fetch<VEC, VPT>(slots_g, g, t, next, p);
-      } else {
-        const GnShape q = gn_shape<VEC>(t, groups, rank);
-        gn_fetch<VEC, VPT>(slots, x, t, next, q);
-        gn_fetch<VEC, VPT>(slots_g, g, t, next, q);
-      }
-    }
+    __syncthreads();
     int parts = kGnThreads / 32;  // rows of sums per channel in sm_chan
     if (!p.even) {
       parts = max(1, min(kGnThreads / p.channels, p.lanes));
@@ -576,16 +602,15 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 
           const float2 e = sm_chan[q * p.channels + ch];
           s.x += e.x, s.y += e.y;
         }
-        const int at = (int)u.slab * t.groups * width + p.in_slab + ch;
-        if (sums) sums[((size_t)u.b * (ctas / t.csplit) + rank / t.csplit) * t.d.C + at] = s;
-        const float w = gamma ? __ldg(gamma + at) : 1.0f;
+        if (sums) sums[((size_t)u.b * stretches + stretch) * t.d.C + slab_c + ch] = s;
+        const float w = ch == tid ? own_gamma : gamma ? __ldg(gamma + slab_c + ch) : 1.0f;
         s = make_float2(w * s.x, w * s.y);
       }
       if (aligned_groups) {  // a group's channels are neighbouring lanes
 #pragma unroll
         for (int o = 16; o; o >>= 1)
           if (o < width) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
-        if (dx && ch < p.channels && (ch & (width - 1)) == 0) gn_send(mail, turn, rank, ctas, ch / width, s);
+        if (dx && ch < p.channels && (ch & (width - 1)) == 0) gn_send(mail, turn, rank, ctas, ch >> shift, s);
       } else if (ch < p.channels) {
         sm_part[ch] = s;
       }
@@ -611,16 +636,21 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 
       }
       __syncthreads();
       if (p.rows) {
-        float2 cf[VEC];
+        float2 cf[NG];  // minus rstd times the two means
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) cf[k] = sm_coef[(p.in_slab + p.col * VEC + k) / width];
+        for (int k = 0; k < NG; ++k) {
+          const float2 m = sm_coef[GROUPED ? p.group : (p.in_slab + p.col * VEC + k) / width];
+          cf[k] = make_float2(-rs[k] * m.x, -rs[k] * m.y);
+        }
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) ga[k] *= rs[k % NG];
         float* to = dx + gn_base(t, u) + p.inside;
         const size_t step = (size_t)p.lanes * t.d.C;
 #pragma unroll
         for (int i = 0; i < VPT; ++i, to += step) {
           if (i >= p.rows) break;
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) vx[i].e[k] = rs[k] * (ga[k] * vg[i].e[k] - cf[k].y - vx[i].e[k] * cf[k].x);
+          for (int k = 0; k < VEC; ++k) vx[i].e[k] = fmaf(ga[k], vg[i].e[k], fmaf(vx[i].e[k], cf[k % NG].x, cf[k % NG].y));
           gn_store<VEC>(to, vx[i]);
         }
       }
@@ -634,24 +664,27 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 
   if (ctas > 1) cluster.sync();
 }
 
-// dgamma and dbeta from the channel sums: 32 channels and eight stretches of rows per CTA.
+// dgamma and dbeta from the channel sums: 8 channels and 32 stretches of rows per CTA, so that few loads of a thread
+// wait for one another (a few hundred rows as a rule: latency, not bytes).
 __global__ void __launch_bounds__(256) gn_params_tile_kernel(const float2* sums, int rows, int C, float* dgamma, float* dbeta) {
-  __shared__ double2 sm[8][32];
+  __shared__ double2 sm[8][8];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  const int cl = threadIdx.x & 7, c = blockIdx.x * 8 + cl, warp = threadIdx.x >> 5;
   double2 s = make_double2(0.0, 0.0);
   if (c < C) {
 #pragma unroll 8
-    for (int r = part; r < rows; r += 8) {
+    for (int r = threadIdx.x >> 3; r < rows; r += 32) {
       const float2 e = sums[(size_t)r * C + c];
       s.x += (double)e.x, s.y += (double)e.y;
     }
   }
-  sm[part][lane] = s;
+#pragma unroll
+  for (int o = 8; o < 32; o <<= 1) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
+  if ((threadIdx.x & 31) < 8) sm[warp][cl] = s;
   __syncthreads();
-  if (part || c >= C) return;
-  for (int q = 1; q < 8; ++q) s.x += sm[q][lane].x, s.y += sm[q][lane].y;
+  if (threadIdx.x >= 8 || c >= C) return;
+  for (int q = 1; q < 8; ++q) s.x += sm[q][cl].x, s.y += sm[q][cl].y;
   if (dgamma) dgamma[c] = (float)s.x;
   if (dbeta) dbeta[c] = (float)s.y;
 }
@@ -682,7 +715,9 @@ cudaError_t cluster_launch(vtlb_ctx* ctx, std::atomic<int>* resident, void (*ker
       if (fit < 1) fit = 1;
       resident[cluster].store(fit, std::memory_order_relaxed);
     }
-    if (clusters > (unsigned)fit) clusters = (unsigned)fit;
+    // as few as finish in the same number of rounds: a cluster that finds no room yet would run behind all others
+    const unsigned rounds = (units + fit - 1) / fit;
+    clusters = (units + rounds - 1) / rounds;
   }
   cfg.gridDim = dim3(clusters * cluster);
   return cudaLaunchKernelEx(&cfg, kern, static_cast<Args&&>(args)...);
@@ -693,14 +728,14 @@ cudaError_t fwd_tile(vtlb_ctx* ctx, const GnTile& t, int cluster, Args... args) 
   return cluster_launch(ctx, resident, gn_fwd_tile_kernel<ACT, VEC, VPT, GROUPED>, t.units, cluster,
                         (size_t)kGnThreads * VPT * VEC * 4, args...);
 }
-template <int ACT, int VEC, int VPT, typename... Args>
+template <int ACT, int VEC, int VPT, bool GROUPED, typename... Args>
 cudaError_t bwd_tile(vtlb_ctx* ctx, const GnTile& t, int cluster, Args... args) {
   static std::atomic<int> resident[kGnMaxCluster + 1];
-  return cluster_launch(ctx, resident, gn_bwd_tile_kernel<ACT, VEC, VPT>, t.units, cluster,
+  return cluster_launch(ctx, resident, gn_bwd_tile_kernel<ACT, VEC, VPT, GROUPED>, t.units, cluster,
                         (size_t)kGnThreads * VPT * VEC * 8, args...);
 }
 
-GnTile tile_of(const GnDims& d, const GnPlan& p) { return GnTile{d, p.groups, p.slabs, p.csplit, p.channels, p.rows, (unsigned)d.B * (unsigned)p.slabs}; }
+GnTile tile_of(const GnDims& d, const GnPlan& p) { return GnTile{d, p.groups, p.slabs, p.csplit, p.channels, p.rows, (unsigned)d.B * (unsigned)p.slabs, 0u}; }
 
 int check_dims(vtlb_ctx* ctx, const char* fn, int B, int S, int C, int groups, int act_kind, GnDims* d) {
   if (B <= 0 || S <= 0 || C <= 0 || groups <= 0 || C % groups)
@@ -768,11 +803,12 @@ int gn_backward(vtlb_ctx* ctx, const float* g, const float* x, GnDims d, const f
     if (dgamma || dbeta)
       if (int rc = ws.get((size_t)rows * d.C * sizeof(float2), &scratch)) return rc;
     float2* sums = (float2*)scratch;
-#define VTLB_GN_BWD(VEC, VPT) \
-  bwd_tile<ACT, VEC, VPT>(ctx, t, cluster, g, x, gamma, beta, mean, rstd, t, dx, sums, ctx->d_status)
+    const bool grouped = plan.vec == 1 || d.width % 4 == 0;
+#define VTLB_GN_BWD(VEC, VPT, GROUPED) \
+  bwd_tile<ACT, VEC, VPT, GROUPED>(ctx, t, cluster, g, x, gamma, beta, mean, rstd, t, dx, sums, ctx->d_status)
 #define VTLB_GN_BWD_VPT(VPT) \
   case VPT:                  \
-    VTLB_CUDA(ctx, plan.vec == 1 ? VTLB_GN_BWD(1, VPT) : VTLB_GN_BWD(4, VPT)); \
+    VTLB_CUDA(ctx, plan.vec == 1 ? VTLB_GN_BWD(1, VPT, true) : grouped ? VTLB_GN_BWD(4, VPT, true) : VTLB_GN_BWD(4, VPT, false)); \
     break
     switch (plan.vpt) {
       VTLB_GN_BWD_VPT(1);
@@ -784,7 +820,7 @@ int gn_backward(vtlb_ctx* ctx, const float* g, const float* x, GnDims d, const f
 #undef VTLB_GN_BWD
     VTLB_LAUNCHED(ctx);
     if (sums) {
-      VTLB_CUDA(ctx, vtlb_launch_early(gn_params_tile_kernel, dim3((d.C + 31) / 32), dim3(256), 0, ctx->stream,
+      VTLB_CUDA(ctx, vtlb_launch_early(gn_params_tile_kernel, dim3((d.C + 7) / 8), dim3(256), 0, ctx->stream,
                                        (const float2*)sums, rows, d.C, dgamma, dbeta));
       VTLB_LAUNCHED(ctx);
     }
