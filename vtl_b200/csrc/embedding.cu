@@ -7,26 +7,62 @@
 
 namespace {
 
-// one thread per four consecutive elements of y
-template <bool DROP>
+// Four consecutive elements of y per step, U steps at a time: bound by HBM (a row of W in, a row of y out), so what counts is
+// that every thread has U loads in flight.  VEC: D is a multiple of four and both arrays are 16-byte aligned, so that
+// the four lie in one row.
+template <bool VEC, bool DROP, int U>
 __global__ void __launch_bounds__(256) embedding_fwd_kernel(const float* __restrict__ W, int V, uint32_t D,
                                                             const int32_t* __restrict__ ids, size_t total, float scale,
-                                                            float* __restrict__ y, vtlb_mask m, uint32_t* bad) {
-  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; 4 * i < total; i += (size_t)gridDim.x * blockDim.x) {
-    uint4 r = make_uint4(0, 0, 0, 0);
-    if (DROP) r = vtlb_philox(m, i);
-    const uint32_t word[4] = {r.x, r.y, r.z, r.w};
+                                                            float* __restrict__ y, int y_aligned, vtlb_mask m,
+                                                            uint32_t* bad) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the kernel in front is done from here on
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const size_t first = (size_t)blockIdx.x * (256 * 4 * U);  // element of y
+  const size_t row0 = first / D;
+  const uint32_t col0 = (uint32_t)(first - row0 * D);  // D + 4096 * U fits 32 bits: D < 2^31
+  float v[U][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const size_t e = 4 * i + k;
-      if (e >= total) break;
-      const size_t j = e / D;
-      const int id = ids[j];
-      const bool in = id >= 0 && id < V;
-      if (!in && bad) atomicOr(bad, 1u);
-      float v = in ? __fmul_rn(W[(size_t)id * D + (e - j * D)], scale) : 0.0f;
-      if (DROP) v = vtlb_drop(m, word[k], v);
-      y[e] = v;
+  for (int u = 0; u < U; ++u) {
+    const uint32_t off = col0 + (u * 256 + threadIdx.x) * 4;
+    uint32_t row = off / D, col = off - row * D;
+    size_t j = row0 + row;
+    if (first + (size_t)(u * 256 + threadIdx.x) * 4 >= total) {
+      v[u][0] = v[u][1] = v[u][2] = v[u][3] = 0.0f;
+      continue;
+    }
+    int id = __ldg(ids + j);
+    bool in = id >= 0 && id < V;
+    if (!in && bad) atomicOr(bad, 1u);
+    if (VEC) {
+      const float4 f = in ? __ldg(reinterpret_cast<const float4*>(W + (size_t)id * D + col)) : make_float4(0, 0, 0, 0);
+      v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[u][k] = in && j * D + col < total ? __ldg(W + (size_t)id * D + col) : 0.0f;
+        if (++col == D && j * D + col < total) {  // the next row
+          col = 0;
+          id = __ldg(ids + ++j);
+          in = id >= 0 && id < V;
+          if (!in && bad) atomicOr(bad, 1u);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const size_t e = first + (size_t)(u * 256 + threadIdx.x) * 4;
+    if (e >= total) return;
+    float4 o = make_float4(__fmul_rn(v[u][0], scale), __fmul_rn(v[u][1], scale), __fmul_rn(v[u][2], scale),
+                           __fmul_rn(v[u][3], scale));
+    if (DROP) o = vtlb_drop4(m, e / 4, o);
+    if (VEC || (y_aligned && e + 4 <= total)) {
+      *reinterpret_cast<float4*>(y + e) = o;
+    } else {
+      const float q[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (e + k < total) y[e + k] = q[k];
     }
   }
 }
@@ -34,12 +70,56 @@ __global__ void __launch_bounds__(256) embedding_fwd_kernel(const float* __restr
 // ---------------------------------------------------------------- gradient
 // The positions are sorted by token (stable: those of a token stay in order), then read in that order, so that a sum is
 // a run of consecutive rows and no two threads add to one place: no atomics, the same bits every time.  Three launches:
-//   sort   one thread-block cluster; the pairs (token, position) stay in its shared memory over all passes
-//   sums   the sorted positions in tiles of equal length whatever the tokens are; a run inside a tile is written to dW,
-//          a run that crosses a tile's edge leaves a partial row per tile.  Rows of tokens that do not occur are
-//          zeroed by further CTAs of the same launch
-//   join   the partial rows of each run that crosses edges, in order
+//   sort   pairs (token, position); tokens outside [0, V) take the key V and end up behind all others
+//   sums   the sorted positions in tiles of equal length whatever the tokens are.  A run that ends within a tile's
+//          length of the tile it starts in is summed there as a whole; a longer one leaves a partial row per tile.
+//          Rows of tokens that do not occur are zeroed by further CTAs of this launch, which need nothing of the sort and
+//          start while it runs
+//   join   the partial rows of each long run, in order
 // Bound by HBM: the rows of g that count are read once and dW is written once.
+
+// Sort of up to kRankMax positions: a warp finds the ranks of four of them by comparing with all.  n^2 comparisons, two
+// instructions each, spread over the whole GPU, against two or three passes of a few microseconds each on one cluster.
+constexpr int kRankMax = 2048;
+__global__ void __launch_bounds__(256) token_rank_kernel(const int32_t* __restrict__ ids, int n, int V, int2* __restrict__ sorted) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31, j0 = (int)(blockIdx.x * 8 + (threadIdx.x >> 5)) * 4;
+  if (j0 >= n) return;
+  const auto key_at = [&](int i) {
+    const int id = i < n ? __ldg(ids + i) : -1;
+    return id >= 0 && id < V ? (uint32_t)id : (uint32_t)V;
+  };
+  uint32_t key[4];
+  int rank[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) key[q] = key_at(j0 + q);
+  const int own = j0 & ~31;  // the 32 positions around j0 .. j0 + 3
+#pragma unroll 4
+  for (int i = lane; i < own; i += 32) {
+    const uint32_t k = key_at(i);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) rank[q] += k <= key[q];
+  }
+  {
+    const int i = own + lane;
+    const uint32_t k = key_at(i);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) rank[q] += i < n && (k < key[q] || (k == key[q] && i < j0 + q));
+  }
+#pragma unroll 4
+  for (int i = own + 32 + lane; i < n; i += 32) {
+    const uint32_t k = key_at(i);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) rank[q] += k < key[q];
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int r = __reduce_add_sync(0xffffffffu, rank[q]);
+    if (lane == q && j0 + q < n) sorted[r] = make_int2((int)key[q], j0 + q);
+  }
+}
+
 constexpr int kSortThreads = 1024, kSortItemsMax = 16, kSortCtas = 8;
 constexpr int kSortMax = kSortThreads * kSortItemsMax * kSortCtas;  // positions per batch; longer calls take several
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
@@ -48,13 +128,11 @@ size_t sort_smem(int items) {
   return (size_t)items * kSortThreads * 8 + (size_t)32 * kDigits * 4 + (size_t)kDigits * 8 + 32 * 4;
 }
 
-// Radix sort of (token, position), least significant digit first.  CTA r of the cluster holds elements
-// [r, r + 1) * 1024 * ITEMS of the current order, a warp 32 * ITEMS consecutive ones of them.  Tokens outside [0, V)
-// take the key V and end up behind all others.  `present`, where given, gets 1 for each token that occurs.
+// Radix sort of more positions, least significant digit first, in the shared memory of one thread-block cluster: CTA r
+// holds elements [r, r + 1) * 1024 * ITEMS of the current order, a warp 32 * ITEMS consecutive ones of them.
 template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const int32_t* __restrict__ ids, int n, int V, int passes,
-                                                                  int bits, int32_t* __restrict__ sorted_id,
-                                                                  int32_t* __restrict__ sorted_pos, uint8_t* present) {
+                                                                  int bits, int2* __restrict__ sorted) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   constexpr int kChunk = kSortThreads * ITEMS;
@@ -67,30 +145,22 @@ __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const int32_t*
   uint32_t* sm_scan = sm_base + kDigits;       // [32]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int me = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
-  const int first = warp * 32 * ITEMS + lane;
+  const int first = warp * 32 * ITEMS + lane, digits = 1 << bits;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the kernel in front is done from here on
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (present) {
-    for (size_t i = (size_t)me * kSortThreads + tid; i < ((size_t)V + 15) / 16; i += (size_t)ctas * kSortThreads)
-      reinterpret_cast<uint4*>(present)[i] = make_uint4(0, 0, 0, 0);
-    __threadfence();
-    cluster.sync();
-  }
   uint32_t key[ITEMS], pos[ITEMS], rank[ITEMS];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
     const int j = me * kChunk + first + 32 * i;
-    const int id = j < n ? ids[j] : -1;
-    const bool in = id >= 0 && id < V;
-    key[i] = in ? (uint32_t)id : (uint32_t)V;
+    const int id = j < n ? __ldg(ids + j) : -1;
+    key[i] = id >= 0 && id < V ? (uint32_t)id : (uint32_t)V;
     pos[i] = (uint32_t)j;
-    if (in && present) present[id] = 1;
   }
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * bits;
-    const uint32_t mask = (1u << bits) - 1u;
+    const uint32_t mask = (uint32_t)digits - 1u;
     uint32_t* cnt = sm_cnt + warp * kDigits;
-    for (int d = lane; d < kDigits; d += 32) cnt[d] = 0;
+    for (int d = lane; d < digits; d += 32) cnt[d] = 0;
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
@@ -103,20 +173,23 @@ __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const int32_t*
       __syncwarp();
     }
     __syncthreads();
-    uint32_t total = 0;
-    if (tid < kDigits) {
+    if (tid < digits) {
+      uint32_t c[32], total = 0;
+#pragma unroll
+      for (int w = 0; w < 32; ++w) c[w] = sm_cnt[w * kDigits + tid];
+#pragma unroll
       for (int w = 0; w < 32; ++w) {
-        const uint32_t c = sm_cnt[w * kDigits + tid];
         sm_cnt[w * kDigits + tid] = total;
-        total += c;
+        total += c[w];
       }
       sm_tot[tid] = total;
     }
     cluster.sync();  // the totals of all CTAs are there, and nobody reads its elements from shared memory any more
     uint32_t in_front = 0, all = 0;
-    if (tid < kDigits) {
-      for (int r = 0; r < ctas; ++r) {
-        const uint32_t c = cluster.map_shared_rank(sm_tot, r)[tid];
+    if (tid < digits) {
+#pragma unroll
+      for (int r = 0; r < kSortCtas; ++r) {
+        const uint32_t c = r < ctas ? cluster.map_shared_rank(sm_tot, r)[tid] : 0u;
         if (r < me) in_front += c;
         all += c;
       }
@@ -129,17 +202,10 @@ __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const int32_t*
     }
     if (lane == 31) sm_scan[warp] = incl;
     __syncthreads();
-    if (warp == 0) {
-      uint32_t v = sm_scan[lane];
+    uint32_t base = 0;  // of the digits of earlier warps; at most kDigits / 32 hold any
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
-      }
-      sm_scan[lane] = v;
-    }
-    __syncthreads();
-    if (tid < kDigits) sm_base[tid] = (warp ? sm_scan[warp - 1] : 0u) + incl - all + in_front;
+    for (int w = 0; w < kDigits / 32; ++w) base += w < warp ? sm_scan[w] : 0u;
+    if (tid < digits) sm_base[tid] = base + incl - all + in_front;
     __syncthreads();
     const bool out = pass == passes - 1;
 #pragma unroll
@@ -147,7 +213,7 @@ __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const int32_t*
       const uint32_t d = (key[i] >> shift) & mask;
       const uint32_t to = sm_base[d] + cnt[d] + rank[i];
       if (out) {
-        if (to < (uint32_t)n) sorted_id[to] = (int32_t)key[i], sorted_pos[to] = (int32_t)pos[i];
+        if (to < (uint32_t)n) sorted[to] = make_int2((int)key[i], (int)pos[i]);
       } else {
         const int r = (int)(to / kChunk);
         cluster.map_shared_rank(sm_key, r)[to % kChunk] = key[i];
@@ -164,8 +230,8 @@ __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const int32_t*
 
 struct EmbGrad {
   const float* g;
-  const int32_t *sorted_id, *sorted_pos;
-  const uint8_t* present;  // null: rows of absent tokens are left alone
+  const int32_t* ids;
+  const int2* sorted;  // (token, position)
   float* dW;
   float* partial;  // [tiles][2][cols * 4]
   size_t first_pos;  // position 0 of this batch in the whole call (the mask's index)
@@ -220,114 +286,161 @@ __device__ __forceinline__ float4 mul4(float4 a, float s) {
   return make_float4(__fmul_rn(a.x, s), __fmul_rn(a.y, s), __fmul_rn(a.z, s), __fmul_rn(a.w, s));
 }
 
-constexpr int kZeroPerThread = 16;  // columns of four zeroed per thread
-
-template <bool VEC, bool DROP>
-__global__ void __launch_bounds__(256) embedding_sums_kernel(EmbGrad p, vtlb_mask m, unsigned sum_ctas) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (blockIdx.x >= sum_ctas) {  // zeros: blocks of four elements of dW, 16-byte aligned where VEC
-    const size_t total = (size_t)p.V * p.D;
-    const size_t base = (size_t)(blockIdx.x - sum_ctas) * blockDim.x * kZeroPerThread * 4;
-    const size_t row0 = base / p.D;
-    const uint32_t col0 = (uint32_t)(base - row0 * p.D);
+// Zeros in the rows [row0, row1) of dW whose token does not occur, kZeroRows of them at a time: which do occur is seen from
+// all of the ids, by every CTA for itself.
+constexpr int kZeroRows = 8192;
+__device__ __forceinline__ void zero_absent(const EmbGrad& p, size_t row0, size_t row1) {
+  __shared__ uint32_t met[kZeroRows / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (size_t r0 = row0; r0 < row1; r0 += kZeroRows) {
+    const int rows = (int)(row1 - r0 < kZeroRows ? row1 - r0 : kZeroRows);
+    for (int i = threadIdx.x; i < (rows + 31) / 32; i += blockDim.x) met[i] = 0;
+    __syncthreads();
+    const auto mark = [&](int id) {
+      const int64_t r = (int64_t)id - (int64_t)r0;
+      if (r >= 0 && r < rows && !(met[r >> 5] >> (r & 31) & 1u)) atomicOr(&met[r >> 5], 1u << (r & 31));
+    };
+    // 16-byte pieces of the ids, several in flight: this is latency, during which nothing is written
+    const int lead = min(p.n, (int)((16 - ((uintptr_t)p.ids & 15)) & 15) / 4), quads = (p.n - lead) / 4;
+    const int4* ids4 = reinterpret_cast<const int4*>(p.ids + lead);
+#pragma unroll 8
+    for (int i = threadIdx.x; i < quads; i += blockDim.x) {
+      const int4 q = __ldg(ids4 + i);
+      mark(q.x), mark(q.y), mark(q.z), mark(q.w);
+    }
+    if ((int)threadIdx.x < lead) mark(__ldg(p.ids + threadIdx.x));
+    if ((int)threadIdx.x < p.n - lead - 4 * quads) mark(__ldg(p.ids + lead + 4 * quads + threadIdx.x));
+    __syncthreads();
+    if (p.cols >= 32) {  // a warp per row, 16 bytes per lane but for the row's unaligned ends
+      for (int r = warp; r < rows; r += blockDim.x >> 5) {
+        if (met[r >> 5] >> (r & 31) & 1u) continue;
+        float* row = p.dW + (r0 + r) * p.D;
+        const int head = (int)((16 - ((uintptr_t)row & 15)) & 15) / 4, body = (p.D - head) / 4, end = head + 4 * body;
+        float4* out = reinterpret_cast<float4*>(row + head);
 #pragma unroll 4
-    for (int i = 0; i < kZeroPerThread; ++i) {
-      const uint32_t off = (i * blockDim.x + threadIdx.x) * 4;
-      const size_t e = base + off;
-      if (e >= total) return;
-      if (VEC) {
-        if (!p.present[row0 + ((uint64_t)col0 + off) / (uint32_t)p.D]) *reinterpret_cast<float4*>(p.dW + e) = make_float4(0, 0, 0, 0);
-      } else {
-        for (int k = 0; k < 4 && e + k < total; ++k)
-          if (!p.present[row0 + ((uint64_t)col0 + off + k) / (uint32_t)p.D]) p.dW[e + k] = 0.0f;
+        for (int c = lane; c < body; c += 32) out[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (lane < head) row[lane] = 0.0f;
+        if (end + lane < p.D) row[end + lane] = 0.0f;
+      }
+    } else {  // element by element, a warp's 32 next to one another
+      float* out = p.dW + r0 * p.D;
+      const uint32_t D = (uint32_t)p.D, total = (uint32_t)rows * D, dr = blockDim.x / D, dc = blockDim.x - dr * D;
+      uint32_t r = threadIdx.x / D, c = threadIdx.x - r * D;
+      for (uint32_t e = threadIdx.x; e < total; e += blockDim.x) {
+        if (!(met[r >> 5] >> (r & 31) & 1u)) out[e] = 0.0f;
+        r += dr, c += dc;
+        if (c >= D) c -= D, ++r;
       }
     }
+    __syncthreads();
+  }
+}
+
+template <bool VEC, bool DROP>
+__global__ void __launch_bounds__(256) embedding_sums_kernel(EmbGrad p, vtlb_mask m, unsigned zero_ctas) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (blockIdx.x < zero_ctas) {
+    // No wait for the sort: nothing of it is read here, and it started only when everything in front of it was done.
+    const size_t each = ((size_t)p.V + zero_ctas - 1) / zero_ctas, row0 = blockIdx.x * each;
+    zero_absent(p, row0, row0 + each < (size_t)p.V ? row0 + each : (size_t)p.V);
     return;
   }
-  const int group = threadIdx.x / p.slab, c = (int)(blockIdx.x % p.slabs) * p.slab + threadIdx.x % p.slab;
-  const int t = (int)(blockIdx.x / p.slabs) * p.per_cta + group;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const unsigned cta = blockIdx.x - zero_ctas;
+  const int group = threadIdx.x / p.slab, c = (int)(cta % p.slabs) * p.slab + threadIdx.x % p.slab;
+  const int t = (int)(cta / p.slabs) * p.per_cta + group;
   if (group >= p.per_cta || t >= p.tiles || c >= p.cols) return;
-  const int k0 = t * p.tile, k1 = min(p.n, k0 + p.tile);
-  int cur = __ldg(p.sorted_id + k0);
+  const int T = p.tile, k0 = t * T, k1 = min(p.n, k0 + T);
+  const auto id_at = [&](int k) { return k >= 0 && k < p.n ? __ldg(&p.sorted[k].x) : -1; };
+  int cur = id_at(k0);
   if (cur >= p.V) return;
-  bool starts = k0 == 0 || __ldg(p.sorted_id + k0 - 1) != cur;
+  // The run that comes in from an earlier tile: long if it started before the last tile or goes on into the next one.
+  const bool comes_in = id_at(k0 - 1) == cur;
+  const bool lead = comes_in && (id_at(k0 - T - 1) == cur || id_at(k0 + T) == cur);
+  const int skip = comes_in && !lead ? cur : -1;  // its first tile sums it
+  // The run that starts here and goes on into the next tile: short if it ends in that one.
+  const int last = id_at(k1 - 1);
+  const bool goes_on = last < p.V && id_at(k1) == last && !(comes_in && last == cur);
+  const bool tail = goes_on && id_at(k1 + T) == last;
+  const int end = goes_on && !tail ? min(p.n, k1 + T) : k1;
+  bool first = lead;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const auto flush = [&] {
+    if (first)
+      reinterpret_cast<float4*>(p.partial)[(size_t)t * 2 * p.cols + c] = acc;
+    else if (tail && cur == last)
+      reinterpret_cast<float4*>(p.partial)[((size_t)t * 2 + 1) * p.cols + c] = acc;
+    else if (cur != skip)
+      row_store<VEC>(p.dW + (size_t)cur * p.D, c, p.D, mul4(acc, p.scale), p.accumulate);
+    first = false;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  };
   constexpr int U = 8;
-  for (int k = k0; k < k1; k += U) {
+  for (int k = k0; k < end; k += U) {
     int id[U];
     float4 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      id[u] = k + u < k1 ? __ldg(p.sorted_id + k + u) : p.V;
-      if (id[u] < p.V) {
-        const size_t j = (size_t)__ldg(p.sorted_pos + k + u);
+      const int2 s = k + u < end ? __ldg(p.sorted + k + u) : make_int2(p.V, 0);
+      id[u] = k + u < k1 || s.x == last ? s.x : p.V;
+      if (id[u] < p.V && id[u] != skip) {
+        const size_t j = (size_t)s.y;
         v[u] = row_load<VEC>(p.g + j * p.D, c, p.D);
         if (DROP) v[u] = drop_at<VEC>(m, (p.first_pos + j) * p.D + 4 * (size_t)c, v[u]);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (id[u] != cur && cur < p.V) {  // the run ends at k + u
-        // (at the end of the tile it may go on in the next one)
-        const bool ends = k + u < k1 || k1 == p.n || __ldg(p.sorted_id + k1) != cur;
-        if (starts && ends)
-          row_store<VEC>(p.dW + (size_t)cur * p.D, c, p.D, mul4(acc, p.scale), p.accumulate);
-        else
-          reinterpret_cast<float4*>(p.partial)[((size_t)t * 2 + starts) * p.cols + c] = acc;
+      if (id[u] != cur) {
+        if (cur < p.V) flush();
         cur = id[u];
-        starts = true;
-        acc = make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      if (id[u] < p.V) add4(acc, v[u]);
+      if (id[u] < p.V && id[u] != skip) add4(acc, v[u]);
     }
   }
-  if (cur < p.V) {  // a tile whose length is a multiple of U
-    const bool ends = k1 == p.n || __ldg(p.sorted_id + k1) != cur;
-    if (starts && ends)
-      row_store<VEC>(p.dW + (size_t)cur * p.D, c, p.D, mul4(acc, p.scale), p.accumulate);
-    else
-      reinterpret_cast<float4*>(p.partial)[((size_t)t * 2 + starts) * p.cols + c] = acc;
-  }
+  if (cur < p.V) flush();
 }
 
-// One CTA per tile and 32 columns of four: where a run starts in tile t and goes on in tile t + 1, its partial rows are
-// added up, eight stretches of them at a time, and the stretches in order.
+// Where a long run starts in tile t, its partial rows (slot 1 of tile t, slot 0 of the following ones) are added up: eight
+// stretches of them at a time, and the stretches in order.
 template <bool VEC>
-__global__ void __launch_bounds__(256) embedding_join_kernel(EmbGrad p) {
+__global__ void __launch_bounds__(256) embedding_join_kernel(EmbGrad p, int split) {
   __shared__ float4 sm[8][32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int wide = (p.cols + 31) / 32;
-  const int t = (int)(blockIdx.x / wide), k0 = t * p.tile, k1 = k0 + p.tile;
-  if (k1 >= p.n) return;
-  const int id = __ldg(p.sorted_id + k1 - 1);
-  if (id >= p.V || __ldg(p.sorted_id + k1) != id) return;
-  if (__ldg(p.sorted_id + k0) == id && k0 > 0 && __ldg(p.sorted_id + k0 - 1) == id) return;  // it started before tile t
-  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, c = (int)(blockIdx.x % wide) * 32 + lane;
-  int more = 1;  // tiles t + 1 .. t + more hold partial rows of it
+  const int T = p.tile, t = (int)(blockIdx.x / split), k0 = t * T, k1 = k0 + T;
+  const auto id_at = [&](int k) { return k >= 0 && k < p.n ? __ldg(&p.sorted[k].x) : -1; };
+  const int id = id_at(k1 - 1);
+  if (id >= p.V || id_at(k1 + T) != id || id_at(k0 - 1) == id) return;
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+  int more = 2;  // tiles t + 1 .. t + more hold partial rows of it
   for (;;) {
-    const size_t k = (size_t)(t + more + 1 + lane) * p.tile;
-    const uint32_t differs = __ballot_sync(0xffffffffu, k >= (size_t)p.n || __ldg(p.sorted_id + k) != id);
+    const long long k = (long long)(t + more + 1 + lane) * T;
+    const uint32_t differs = __ballot_sync(0xffffffffu, k >= p.n || id_at((int)k) != id);
     if (differs) {
       more += __ffs(differs) - 1;
       break;
     }
     more += 32;
   }
-  const float4* rows = reinterpret_cast<const float4*>(p.partial) + (size_t)t * 2 * p.cols + c;
-  const int share = (more + 8) / 8;  // of more + 1 rows: the start in slot 1 of tile t, then slot 0 of the others
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (c < p.cols) {
+  const int share = (more + 8) / 8;  // of more + 1 rows
+  for (int c0 = (int)(blockIdx.x % split) * 32; c0 < p.cols; c0 += split * 32) {
+    const int c = c0 + lane;
+    const float4* rows = reinterpret_cast<const float4*>(p.partial) + (size_t)t * 2 * p.cols + c;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c < p.cols) {
 #pragma unroll 4
-    for (int r = part * share; r < min(more + 1, (part + 1) * share); ++r)
-      add4(acc, rows[((size_t)r * 2 + (r == 0)) * p.cols]);
+      for (int r = part * share; r < min(more + 1, (part + 1) * share); ++r)
+        add4(acc, rows[((size_t)r * 2 + (r == 0)) * p.cols]);
+    }
+    __syncthreads();
+    sm[part][lane] = acc;
+    __syncthreads();
+    if (part == 0 && c < p.cols) {
+      for (int q = 1; q * share <= more; ++q) add4(acc, sm[q][lane]);
+      row_store<VEC>(p.dW + (size_t)id * p.D, c, p.D, mul4(acc, p.scale), p.accumulate);
+    }
   }
-  sm[part][lane] = acc;
-  __syncthreads();
-  if (part || c >= p.cols) return;
-  for (int q = 1; q * share <= more; ++q) add4(acc, sm[q][lane]);
-  row_store<VEC>(p.dW + (size_t)id * p.D, c, p.D, mul4(acc, p.scale), p.accumulate);
 }
 
 __global__ void __launch_bounds__(256) ids_from_f32_kernel(const float* __restrict__ src, size_t n, int32_t* __restrict__ ids) {
@@ -350,8 +463,7 @@ int check_sizes(vtlb_ctx* ctx, const char* fn, int V, int D, size_t n, double p)
 }
 
 template <int ITEMS>
-cudaError_t sort_launch(vtlb_ctx* ctx, int ctas, const int32_t* ids, int n, int V, int passes, int bits, int32_t* sorted_id,
-                        int32_t* sorted_pos, uint8_t* present) {
+cudaError_t sort_launch(vtlb_ctx* ctx, int ctas, const int32_t* ids, int n, int V, int passes, int bits, int2* sorted) {
   auto kern = token_sort_kernel<ITEMS>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sort_smem(ITEMS));
   if (e != cudaSuccess) return e;
@@ -367,58 +479,65 @@ cudaError_t sort_launch(vtlb_ctx* ctx, int ctas, const int32_t* ids, int n, int 
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kern, ids, n, V, passes, bits, sorted_id, sorted_pos, present);
+  return cudaLaunchKernelEx(&cfg, kern, ids, n, V, passes, bits, sorted);
+}
+
+cudaError_t sort_positions(vtlb_ctx* ctx, const int32_t* ids, int n, int V, int2* sorted) {
+  if (n <= kRankMax) return vtlb_launch_early(token_rank_kernel, dim3((n + 31) / 32), dim3(256), 0, ctx->stream, ids, n, V, sorted);
+  int key_bits = 1;
+  while (key_bits < 31 && (V >> key_bits)) ++key_bits;  // keys 0 .. V
+  const int passes = (key_bits + kDigitBits - 1) / kDigitBits, bits = (key_bits + passes - 1) / passes;
+  int items = 1, ctas = 1;
+  while (items * kSortThreads * kSortCtas < n) items *= 2;
+  while (ctas * items * kSortThreads < n) ctas *= 2;
+  switch (items) {
+    case 1: return sort_launch<1>(ctx, ctas, ids, n, V, passes, bits, sorted);
+    case 2: return sort_launch<2>(ctx, ctas, ids, n, V, passes, bits, sorted);
+    case 4: return sort_launch<4>(ctx, ctas, ids, n, V, passes, bits, sorted);
+    case 8: return sort_launch<8>(ctx, ctas, ids, n, V, passes, bits, sorted);
+    default: return sort_launch<16>(ctx, ctas, ids, n, V, passes, bits, sorted);
+  }
 }
 
 int embedding_bwd_batch(vtlb_ctx* ctx, vtlb_workspace& ws, const float* g, const int32_t* ids, size_t first_pos, int n, int V,
                         int D, float scale, const vtlb_mask& m, float* dW, int accumulate) {
   EmbGrad p = {};
-  p.g = g, p.dW = dW, p.first_pos = first_pos, p.n = n, p.V = V, p.D = D, p.scale = scale, p.accumulate = accumulate;
+  p.g = g, p.ids = ids, p.dW = dW, p.first_pos = first_pos, p.n = n, p.V = V, p.D = D, p.scale = scale, p.accumulate = accumulate;
   p.cols = (D + 3) / 4;
   p.slabs = (p.cols + 255) / 256;
   p.slab = (p.cols + p.slabs - 1) / p.slabs;
   p.per_cta = 256 / p.slab;
-  const int threads = (p.slab * p.per_cta + 31) / 32 * 32;
-  p.tile = 32;
+  // Tiles of 4 to 64 positions: long enough that few runs are cut, short enough for eight CTAs per SM.
+  p.tile = 4;
+  while (p.tile < 64 && (long long)n * p.slabs > (long long)p.tile * p.per_cta * 8 * ctx->sm_count) p.tile *= 2;
   p.tiles = (n + p.tile - 1) / p.tile;
-  const size_t list = vtlb_round_up((size_t)n * 4, 256), flags = accumulate ? 0 : vtlb_round_up((size_t)V, 256);
+  const size_t list = vtlb_round_up((size_t)n * sizeof(int2), 256);
   void* scr = nullptr;
-  if (int rc = ws.get(2 * list + flags + (size_t)p.tiles * 2 * p.cols * 16, &scr)) return rc;
-  char* at = (char*)scr;
-  int32_t *sorted_id = (int32_t*)at, *sorted_pos = (int32_t*)(at + list);
-  uint8_t* present = accumulate ? nullptr : (uint8_t*)(at + 2 * list);
-  p.sorted_id = sorted_id, p.sorted_pos = sorted_pos, p.present = present;
-  p.partial = (float*)(at + 2 * list + flags);
+  if (int rc = ws.get(list + (size_t)p.tiles * 2 * p.cols * 16, &scr)) return rc;
+  int2* sorted = (int2*)scr;
+  p.sorted = sorted;
+  p.partial = (float*)((char*)scr + list);
 
-  int key_bits = 1;
-  while (key_bits < 31 && (V >> key_bits)) ++key_bits;  // keys 0 .. V
-  const int passes = (key_bits + kDigitBits - 1) / kDigitBits, bits = (key_bits + passes - 1) / passes;
-  int items = 1;
-  while (items * kSortThreads * kSortCtas < n) items *= 2;
-  int ctas = 1;
-  while (ctas * items * kSortThreads < n) ctas *= 2;
-  cudaError_t e;
-  switch (items) {
-    case 1: e = sort_launch<1>(ctx, ctas, ids, n, V, passes, bits, sorted_id, sorted_pos, present); break;
-    case 2: e = sort_launch<2>(ctx, ctas, ids, n, V, passes, bits, sorted_id, sorted_pos, present); break;
-    case 4: e = sort_launch<4>(ctx, ctas, ids, n, V, passes, bits, sorted_id, sorted_pos, present); break;
-    case 8: e = sort_launch<8>(ctx, ctas, ids, n, V, passes, bits, sorted_id, sorted_pos, present); break;
-    default: e = sort_launch<16>(ctx, ctas, ids, n, V, passes, bits, sorted_id, sorted_pos, present); break;
-  }
-  VTLB_CUDA(ctx, e);
+  VTLB_CUDA(ctx, sort_positions(ctx, ids, n, V, sorted));
   VTLB_LAUNCHED(ctx);
 
   const bool vec = D % 4 == 0 && vtlb_aligned16(g) && vtlb_aligned16(dW);
   const unsigned sum_ctas = (unsigned)((p.tiles + p.per_cta - 1) / p.per_cta) * p.slabs;
-  const size_t per_zero = (size_t)threads * kZeroPerThread * 4, table = (size_t)V * D;
-  const size_t zero_ctas = accumulate ? 0 : (table + per_zero - 1) / per_zero;
+  // Each zeroing CTA reads all ids, so they are no more than write four times what all of them read, but two per SM
+  // where there are 32 KB to write for each.
+  const size_t table = (size_t)V * D * 4;
+  size_t want = table / ((size_t)n * 16), least = (size_t)2 * ctx->sm_count;
+  want = want < least ? least : want;
+  if (want > table / 32768 + 1) want = table / 32768 + 1;
+  const unsigned zero_ctas = accumulate ? 0u : (unsigned)(want < (size_t)V ? want : (size_t)V);
   auto sums = vec ? (m.any ? embedding_sums_kernel<true, true> : embedding_sums_kernel<true, false>)
                   : (m.any ? embedding_sums_kernel<false, true> : embedding_sums_kernel<false, false>);
-  VTLB_CUDA(ctx, vtlb_launch_early(sums, dim3((unsigned)(sum_ctas + zero_ctas)), dim3(threads), 0, ctx->stream, p, m, sum_ctas));
+  VTLB_CUDA(ctx, vtlb_launch_early(sums, dim3(sum_ctas + zero_ctas), dim3(256), 0, ctx->stream, p, m, zero_ctas));
   VTLB_LAUNCHED(ctx);
-  if (p.tiles > 1) {
+  if (p.tiles > 2) {
     auto join = vec ? embedding_join_kernel<true> : embedding_join_kernel<false>;
-    VTLB_CUDA(ctx, vtlb_launch_early(join, dim3((unsigned)(p.tiles - 1) * ((p.cols + 31) / 32)), dim3(256), 0, ctx->stream, p));
+    const int wide = (p.cols + 31) / 32, split = wide < 8 ? wide : 8;
+    VTLB_CUDA(ctx, vtlb_launch_early(join, dim3((unsigned)(p.tiles - 2) * split), dim3(256), 0, ctx->stream, p, split));
     VTLB_LAUNCHED(ctx);
   }
   return VTLB_OK;
@@ -448,9 +567,17 @@ VTLB_API int vtlb_embedding_fwd_f32(vtlb_ctx* ctx, const void* d_W, int V, int D
     VTLB_CUDA(ctx, cudaMemsetAsync(bad, 0, sizeof(uint32_t), ctx->stream));
   }
   const vtlb_mask m = vtlb_make_mask(p, seed, step);
-  auto kern = m.any ? embedding_fwd_kernel<true> : embedding_fwd_kernel<false>;
-  kern<<<grid_for(ctx, (total + 3) / 4), 256, 0, ctx->stream>>>((const float*)d_W, V, (uint32_t)D, (const int32_t*)d_ids_i32,
-                                                                total, scale, (float*)d_Y, m, bad);
+  const bool y_aligned = vtlb_aligned16(d_Y), vec = D % 4 == 0 && vtlb_aligned16(d_W) && y_aligned;
+  // Four loads in flight per thread where that still leaves work for every SM.
+  const int U = total >= (size_t)ctx->sm_count * 2 * 256 * 4 * 4 ? 4 : 1;
+  auto kern = U == 4 ? (vec ? (m.any ? embedding_fwd_kernel<true, true, 4> : embedding_fwd_kernel<true, false, 4>)
+                            : (m.any ? embedding_fwd_kernel<false, true, 4> : embedding_fwd_kernel<false, false, 4>))
+                     : (vec ? (m.any ? embedding_fwd_kernel<true, true, 1> : embedding_fwd_kernel<true, false, 1>)
+                            : (m.any ? embedding_fwd_kernel<false, true, 1> : embedding_fwd_kernel<false, false, 1>));
+  const size_t ctas = (total + 1024 * U - 1) / (1024 * U);
+  if (ctas > 0x7fffffffu) return vtlb_fail(ctx, VTLB_EINVAL, "vtlb_embedding_fwd_f32: n * D is beyond 2^43 elements");
+  VTLB_CUDA(ctx, vtlb_launch_early(kern, dim3((unsigned)ctas), dim3(256), 0, ctx->stream, (const float*)d_W, V, (uint32_t)D,
+                                   (const int32_t*)d_ids_i32, total, scale, (float*)d_Y, (int)y_aligned, m, bad));
   VTLB_LAUNCHED(ctx);
   if (check) {
     uint32_t flag = 0;
