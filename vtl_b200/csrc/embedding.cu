@@ -236,19 +236,11 @@ struct EmbGrad {
   float* partial;  // [tiles][2][cols * 4]
   size_t first_pos;  // position 0 of this batch in the whole call (the mask's index)
   int n, V, D, cols, tile, tiles;  // cols = ceil(D / 4)
-  int slab, slabs, per_cta;        // columns of four per slab, slabs, tiles per CTA
+  int slab, slabs, per_cta;        // columns of four (else: warps) per slab, slabs, tiles per CTA
   float scale;
   int accumulate;
 };
 
-// Four consecutive values of a row from column 4 * c on; VEC: the rows are 16-byte aligned.
-template <bool VEC>
-__device__ __forceinline__ float4 row_load(const float* row, int c, int D) {
-  if (VEC) return __ldg(reinterpret_cast<const float4*>(row) + c);
-  const float* p = row + 4 * c;
-  const int left = D - 4 * c;
-  return make_float4(__ldg(p), left > 1 ? __ldg(p + 1) : 0.f, left > 2 ? __ldg(p + 2) : 0.f, left > 3 ? __ldg(p + 3) : 0.f);
-}
 template <bool VEC>
 __device__ __forceinline__ void row_store(float* row, int c, int D, float4 v, int accumulate) {
   if (VEC) {
@@ -266,18 +258,27 @@ __device__ __forceinline__ void row_store(float* row, int c, int D, float4 v, in
   for (int k = 0; k < 4; ++k)
     if (4 * c + k < D) p[k] = accumulate ? __fadd_rn(p[k], e[k]) : e[k];
 }
-// The mask on four consecutive elements from flat index e on (e % 4 = 0 where VEC).
-template <bool VEC>
-__device__ __forceinline__ float4 drop_at(const vtlb_mask& m, size_t e, float4 v) {
-  if (VEC) return vtlb_drop4(m, e / 4, v);
-  const uint4 a = vtlb_philox(m, e / 4);
-  const int o = (int)(e & 3);
-  uint4 w = a;
-  if (o) {
-    const uint4 b = vtlb_philox(m, e / 4 + 1);
-    w = o == 1 ? make_uint4(a.y, a.z, a.w, b.x) : o == 2 ? make_uint4(a.z, a.w, b.x, b.y) : make_uint4(a.w, b.x, b.y, b.z);
-  }
-  return make_float4(vtlb_drop(m, w.x, v.x), vtlb_drop(m, w.y, v.y), vtlb_drop(m, w.z, v.z), vtlb_drop(m, w.w, v.w));
+// Rows that are not 16-byte aligned (D % 4 = o > 0 from one row to the next, or a displaced g): a lane takes the aligned
+// block of four elements of g that starts `o` columns before column 4 * c, draws one block of the mask for it, and hands
+// its first o elements to the lane before it.  (Four single loads and two blocks of the mask otherwise.)  The last lane
+// of a warp only helps the one before it.
+__device__ __forceinline__ float4 block_load(const float* g, size_t e, size_t total, bool aligned) {
+  if (aligned && e + 4 <= total) return __ldg(reinterpret_cast<const float4*>(g + e));
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (e < total) v.x = __ldg(g + e);
+  if (e + 1 < total) v.y = __ldg(g + e + 1);
+  if (e + 2 < total) v.z = __ldg(g + e + 2);
+  if (e + 3 < total) v.w = __ldg(g + e + 3);
+  return v;
+}
+__device__ __forceinline__ float4 shift_down(float4 v, int o) {  // o is the same in all lanes
+  if (o == 0) return v;
+  const float x = __shfl_down_sync(0xffffffffu, v.x, 1);
+  if (o == 1) return make_float4(v.y, v.z, v.w, x);
+  const float y = __shfl_down_sync(0xffffffffu, v.y, 1);
+  if (o == 2) return make_float4(v.z, v.w, x, y);
+  const float z = __shfl_down_sync(0xffffffffu, v.z, 1);
+  return make_float4(v.w, x, y, z);
 }
 __device__ __forceinline__ void add4(float4& a, float4 v) {
   a = make_float4(__fadd_rn(a.x, v.x), __fadd_rn(a.y, v.y), __fadd_rn(a.z, v.z), __fadd_rn(a.w, v.w));
@@ -336,8 +337,10 @@ __device__ __forceinline__ void zero_absent(const EmbGrad& p, size_t row0, size_
   }
 }
 
+constexpr int kTileMax = 64, kCtaPositions = 2048;  // positions per tile and per CTA
 template <bool VEC, bool DROP>
-__global__ void __launch_bounds__(256) embedding_sums_kernel(EmbGrad p, vtlb_mask m, unsigned zero_ctas) {
+__global__ void __launch_bounds__(256, 3) embedding_sums_kernel(EmbGrad p, vtlb_mask m, unsigned zero_ctas) {
+  __shared__ int2 window[kCtaPositions + 2 * kTileMax + 2];  // the sorted positions of this CTA's tiles and a tile around them
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x < zero_ctas) {
     // No wait for the sort: nothing of it is read here, and it started only when everything in front of it was done.
@@ -347,11 +350,20 @@ __global__ void __launch_bounds__(256) embedding_sums_kernel(EmbGrad p, vtlb_mas
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const unsigned cta = blockIdx.x - zero_ctas;
-  const int group = threadIdx.x / p.slab, c = (int)(cta % p.slabs) * p.slab + threadIdx.x % p.slab;
-  const int t = (int)(cta / p.slabs) * p.per_cta + group;
-  if (group >= p.per_cta || t >= p.tiles || c >= p.cols) return;
-  const int T = p.tile, k0 = t * T, k1 = min(p.n, k0 + T);
-  const auto id_at = [&](int k) { return k >= 0 && k < p.n ? __ldg(&p.sorted[k].x) : -1; };
+  const int T = p.tile, t0 = (int)(cta / p.slabs) * p.per_cta, w0 = (t0 - 1) * T - 1;
+  for (int i = threadIdx.x; i < (p.per_cta + 2) * T + 2; i += blockDim.x)
+    window[i] = w0 + i >= 0 && w0 + i < p.n ? __ldg(p.sorted + w0 + i) : make_int2(-1, 0);
+  __syncthreads();
+  const int unit = VEC ? threadIdx.x : threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = unit / p.slab, at = (int)(cta % p.slabs) * p.slab + unit % p.slab;
+  const int c = VEC ? at : at * 31 + lane;
+  const int t = t0 + group;
+  if (group >= p.per_cta || t >= p.tiles || (VEC ? c : at * 31) >= p.cols) return;  // (whole warps where they shuffle)
+  const bool own = VEC || (lane < 31 && c < p.cols);
+  const size_t total = (size_t)p.n * p.D;
+  const bool aligned = ((uintptr_t)p.g & 15) == 0;
+  const int k0 = t * T, k1 = min(p.n, k0 + T);
+  const auto id_at = [&](int k) { return window[k - w0].x; };  // -1 before the first and behind the last position
   int cur = id_at(k0);
   if (cur >= p.V) return;
   // The run that comes in from an earlier tile: long if it started before the last tile or goes on into the next one.
@@ -366,27 +378,33 @@ __global__ void __launch_bounds__(256) embedding_sums_kernel(EmbGrad p, vtlb_mas
   bool first = lead;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   const auto flush = [&] {
-    if (first)
+    if (!own) {
+    } else if (first) {
       reinterpret_cast<float4*>(p.partial)[(size_t)t * 2 * p.cols + c] = acc;
-    else if (tail && cur == last)
+    } else if (tail && cur == last) {
       reinterpret_cast<float4*>(p.partial)[((size_t)t * 2 + 1) * p.cols + c] = acc;
-    else if (cur != skip)
+    } else if (cur != skip) {
       row_store<VEC>(p.dW + (size_t)cur * p.D, c, p.D, mul4(acc, p.scale), p.accumulate);
+    }
     first = false;
     acc = make_float4(0.f, 0.f, 0.f, 0.f);
   };
-  constexpr int U = 8;
+  constexpr int U = DROP ? 4 : 8;  // (the mask's block takes the registers of four more rows)
   for (int k = k0; k < end; k += U) {
-    int id[U];
+    int id[U], pos[U];
     float4 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int2 s = k + u < end ? __ldg(p.sorted + k + u) : make_int2(p.V, 0);
+      const int2 s = k + u < end ? window[k + u - w0] : make_int2(p.V, 0);
       id[u] = k + u < k1 || s.x == last ? s.x : p.V;
+      pos[u] = s.y;
       if (id[u] < p.V && id[u] != skip) {
-        const size_t j = (size_t)s.y;
-        v[u] = row_load<VEC>(p.g + j * p.D, c, p.D);
-        if (DROP) v[u] = drop_at<VEC>(m, (p.first_pos + j) * p.D + 4 * (size_t)c, v[u]);
+        const size_t e = (size_t)s.y * p.D;
+        if (VEC)
+          v[u] = __ldg(reinterpret_cast<const float4*>(p.g + e) + c);
+        else
+          v[u] = 4 * c - (int)(e & 3) < p.D ? block_load(p.g, (e & ~(size_t)3) + 4 * (size_t)c, total, aligned)
+                                            : make_float4(0.f, 0.f, 0.f, 0.f);
       }
     }
 #pragma unroll
@@ -395,7 +413,13 @@ __global__ void __launch_bounds__(256) embedding_sums_kernel(EmbGrad p, vtlb_mas
         if (cur < p.V) flush();
         cur = id[u];
       }
-      if (id[u] < p.V && id[u] != skip) add4(acc, v[u]);
+      if (id[u] < p.V && id[u] != skip) {
+        const size_t e = (p.first_pos + pos[u]) * p.D;
+        float4 w = v[u];
+        if (DROP) w = vtlb_drop4(m, e / 4 + c, w);
+        if (!VEC) w = shift_down(w, (int)(e & 3));
+        add4(acc, w);
+      }
     }
   }
   if (cur < p.V) flush();
@@ -504,12 +528,14 @@ int embedding_bwd_batch(vtlb_ctx* ctx, vtlb_workspace& ws, const float* g, const
   EmbGrad p = {};
   p.g = g, p.ids = ids, p.dW = dW, p.first_pos = first_pos, p.n = n, p.V = V, p.D = D, p.scale = scale, p.accumulate = accumulate;
   p.cols = (D + 3) / 4;
-  p.slabs = (p.cols + 255) / 256;
-  p.slab = (p.cols + p.slabs - 1) / p.slabs;
-  p.per_cta = 256 / p.slab;
+  const bool vec = D % 4 == 0 && vtlb_aligned16(g) && vtlb_aligned16(dW);
+  const int units = vec ? p.cols : (p.cols + 30) / 31, most = vec ? 256 : 8;  // threads, or warps, per row and per CTA
+  p.slabs = (units + most - 1) / most;
+  p.slab = (units + p.slabs - 1) / p.slabs;
+  p.per_cta = most / p.slab;
   // Tiles of 4 to 64 positions: long enough that few runs are cut, short enough for eight CTAs per SM.
   p.tile = 4;
-  while (p.tile < 64 && (long long)n * p.slabs > (long long)p.tile * p.per_cta * 8 * ctx->sm_count) p.tile *= 2;
+  while (p.tile < kTileMax && p.tile * p.per_cta < kCtaPositions && (long long)n * p.slabs > (long long)p.tile * p.per_cta * 8 * ctx->sm_count) p.tile *= 2;
   p.tiles = (n + p.tile - 1) / p.tile;
   const size_t list = vtlb_round_up((size_t)n * sizeof(int2), 256);
   void* scr = nullptr;
@@ -521,7 +547,6 @@ int embedding_bwd_batch(vtlb_ctx* ctx, vtlb_workspace& ws, const float* g, const
   VTLB_CUDA(ctx, sort_positions(ctx, ids, n, V, sorted));
   VTLB_LAUNCHED(ctx);
 
-  const bool vec = D % 4 == 0 && vtlb_aligned16(g) && vtlb_aligned16(dW);
   const unsigned sum_ctas = (unsigned)((p.tiles + p.per_cta - 1) / p.per_cta) * p.slabs;
   // Each zeroing CTA reads all ids, so they are no more than write four times what all of them read, but two per SM
   // where there are 32 KB to write for each.
