@@ -389,80 +389,93 @@ __global__ void __launch_bounds__(256, 3) embedding_sums_kernel(EmbGrad p, vtlb_
     first = false;
     acc = make_float4(0.f, 0.f, 0.f, 0.f);
   };
+  // token of sorted position k of this tile (V: none)
+  const auto token = [&](int k) {
+    const int id = k < end ? window[k - w0].x : p.V;
+    return k < k1 || id == last ? id : p.V;
+  };
   constexpr int U = DROP ? 4 : 8;  // (the mask's block takes the registers of four more rows)
   for (int k = k0; k < end; k += U) {
-    int id[U], pos[U];
     float4 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int2 s = k + u < end ? window[k + u - w0] : make_int2(p.V, 0);
-      id[u] = k + u < k1 || s.x == last ? s.x : p.V;
-      pos[u] = s.y;
-      if (id[u] < p.V && id[u] != skip) {
-        const size_t e = (size_t)s.y * p.D;
+      const int id = token(k + u);
+      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (id < p.V && id != skip) {
+        const size_t row = (size_t)window[k + u - w0].y * p.D;
         if (VEC)
-          v[u] = __ldg(reinterpret_cast<const float4*>(p.g + e) + c);
-        else
-          v[u] = 4 * c - (int)(e & 3) < p.D ? block_load(p.g, (e & ~(size_t)3) + 4 * (size_t)c, total, aligned)
-                                            : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[u] = __ldg(reinterpret_cast<const float4*>(p.g + row) + c);
+        else if (4 * c - (int)(row & 3) < p.D)
+          v[u] = block_load(p.g, (row & ~(size_t)3) + 4 * (size_t)c, total, aligned);
+      }
+    }
+    // (all U rows, valid or not, without a branch between them: a block of the mask is a chain of some 150 cycles)
+    if (DROP || !VEC) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const size_t e = (p.first_pos + (size_t)window[min(k + u, end - 1) - w0].y) * p.D;
+        if (DROP) v[u] = vtlb_drop4(m, e / 4 + c, v[u]);
+        if (!VEC) v[u] = shift_down(v[u], (int)(e & 3));
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (id[u] != cur) {
+      const int id = token(k + u);
+      if (id != cur) {
         if (cur < p.V) flush();
-        cur = id[u];
+        cur = id;
       }
-      if (id[u] < p.V && id[u] != skip) {
-        const size_t e = (p.first_pos + pos[u]) * p.D;
-        float4 w = v[u];
-        if (DROP) w = vtlb_drop4(m, e / 4 + c, w);
-        if (!VEC) w = shift_down(w, (int)(e & 3));
-        add4(acc, w);
-      }
+      if (id < p.V && id != skip) add4(acc, v[u]);
     }
   }
   if (cur < p.V) flush();
 }
 
 // Where a long run starts in tile t, its partial rows (slot 1 of tile t, slot 0 of the following ones) are added up: eight
-// stretches of them at a time, and the stretches in order.
+// stretches of them at a time, and the stretches in order.  A CTA looks after eight tiles (most start no long run, and
+// a CTA per tile costs more than the sums) and one of `split` shares of the columns.
+constexpr int kJoinTiles = 8;
 template <bool VEC>
 __global__ void __launch_bounds__(256) embedding_join_kernel(EmbGrad p, int split) {
   __shared__ float4 sm[8][32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int T = p.tile, t = (int)(blockIdx.x / split), k0 = t * T, k1 = k0 + T;
-  const auto id_at = [&](int k) { return k >= 0 && k < p.n ? __ldg(&p.sorted[k].x) : -1; };
-  const int id = id_at(k1 - 1);
-  if (id >= p.V || id_at(k1 + T) != id || id_at(k0 - 1) == id) return;
+  const int T = p.tile, t0 = (int)(blockIdx.x / split) * kJoinTiles;
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
-  int more = 2;  // tiles t + 1 .. t + more hold partial rows of it
-  for (;;) {
-    const long long k = (long long)(t + more + 1 + lane) * T;
-    const uint32_t differs = __ballot_sync(0xffffffffu, k >= p.n || id_at((int)k) != id);
-    if (differs) {
-      more += __ffs(differs) - 1;
-      break;
+  const auto id_at = [&](long long k) { return k >= 0 && k < p.n ? __ldg(&p.sorted[k].x) : -1; };
+  const int own = t0 + (lane & (kJoinTiles - 1));  // every warp sees the starts of all eight tiles
+  const int own_id = own < p.tiles ? id_at((long long)own * T + T - 1) : -1;
+  const bool starts = own_id >= 0 && own_id < p.V && id_at((long long)own * T + 2 * T) == own_id &&
+                      id_at((long long)own * T - 1) != own_id;
+  uint32_t todo = __ballot_sync(0xffffffffu, starts) & ((1u << kJoinTiles) - 1u);
+  for (; todo; todo &= todo - 1) {
+    const int t = t0 + __ffs(todo) - 1, id = __shfl_sync(0xffffffffu, own_id, t - t0);
+    int more = 2;  // tiles t + 1 .. t + more hold partial rows of it
+    for (;;) {
+      const uint32_t differs = __ballot_sync(0xffffffffu, id_at((long long)(t + more + 1 + lane) * T) != id);
+      if (differs) {
+        more += __ffs(differs) - 1;
+        break;
+      }
+      more += 32;
     }
-    more += 32;
-  }
-  const int share = (more + 8) / 8;  // of more + 1 rows
-  for (int c0 = (int)(blockIdx.x % split) * 32; c0 < p.cols; c0 += split * 32) {
-    const int c = c0 + lane;
-    const float4* rows = reinterpret_cast<const float4*>(p.partial) + (size_t)t * 2 * p.cols + c;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (c < p.cols) {
+    const int share = (more + 8) / 8;  // of more + 1 rows
+    for (int c0 = (int)(blockIdx.x % split) * 32; c0 < p.cols; c0 += split * 32) {
+      const int c = c0 + lane;
+      const float4* rows = reinterpret_cast<const float4*>(p.partial) + (size_t)t * 2 * p.cols + c;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c < p.cols) {
 #pragma unroll 4
-      for (int r = part * share; r < min(more + 1, (part + 1) * share); ++r)
-        add4(acc, rows[((size_t)r * 2 + (r == 0)) * p.cols]);
-    }
-    __syncthreads();
-    sm[part][lane] = acc;
-    __syncthreads();
-    if (part == 0 && c < p.cols) {
-      for (int q = 1; q * share <= more; ++q) add4(acc, sm[q][lane]);
-      row_store<VEC>(p.dW + (size_t)id * p.D, c, p.D, mul4(acc, p.scale), p.accumulate);
+        for (int r = part * share; r < min(more + 1, (part + 1) * share); ++r)
+          add4(acc, rows[((size_t)r * 2 + (r == 0)) * p.cols]);
+      }
+      __syncthreads();
+      sm[part][lane] = acc;
+      __syncthreads();
+      if (part == 0 && c < p.cols) {
+        for (int q = 1; q * share <= more; ++q) add4(acc, sm[q][lane]);
+        row_store<VEC>(p.dW + (size_t)id * p.D, c, p.D, mul4(acc, p.scale), p.accumulate);
+      }
     }
   }
 }
@@ -533,9 +546,10 @@ int embedding_bwd_batch(vtlb_ctx* ctx, vtlb_workspace& ws, const float* g, const
   p.slabs = (units + most - 1) / most;
   p.slab = (units + p.slabs - 1) / p.slabs;
   p.per_cta = most / p.slab;
-  // Tiles of 4 to 64 positions: long enough that few runs are cut, short enough for eight CTAs per SM.
+  const int threads = vec ? (p.slab * p.per_cta + 31) / 32 * 32 : p.slab * p.per_cta * 32;
+  // Tiles of 4 to 64 positions: long enough that few runs are cut, short enough for eight to sixteen CTAs per SM.
   p.tile = 4;
-  while (p.tile < kTileMax && p.tile * p.per_cta < kCtaPositions && (long long)n * p.slabs > (long long)p.tile * p.per_cta * 8 * ctx->sm_count) p.tile *= 2;
+  while (p.tile < kTileMax && p.tile * p.per_cta < kCtaPositions && (long long)n * p.slabs > (long long)p.tile * p.per_cta * 16 * ctx->sm_count) p.tile *= 2;
   p.tiles = (n + p.tile - 1) / p.tile;
   const size_t list = vtlb_round_up((size_t)n * sizeof(int2), 256);
   void* scr = nullptr;
@@ -557,12 +571,13 @@ int embedding_bwd_batch(vtlb_ctx* ctx, vtlb_workspace& ws, const float* g, const
   const unsigned zero_ctas = accumulate ? 0u : (unsigned)(want < (size_t)V ? want : (size_t)V);
   auto sums = vec ? (m.any ? embedding_sums_kernel<true, true> : embedding_sums_kernel<true, false>)
                   : (m.any ? embedding_sums_kernel<false, true> : embedding_sums_kernel<false, false>);
-  VTLB_CUDA(ctx, vtlb_launch_early(sums, dim3(sum_ctas + zero_ctas), dim3(256), 0, ctx->stream, p, m, zero_ctas));
+  VTLB_CUDA(ctx, vtlb_launch_early(sums, dim3(sum_ctas + zero_ctas), dim3(threads), 0, ctx->stream, p, m, zero_ctas));
   VTLB_LAUNCHED(ctx);
   if (p.tiles > 2) {
     auto join = vec ? embedding_join_kernel<true> : embedding_join_kernel<false>;
-    const int wide = (p.cols + 31) / 32, split = wide < 8 ? wide : 8;
-    VTLB_CUDA(ctx, vtlb_launch_early(join, dim3((unsigned)(p.tiles - 2) * split), dim3(256), 0, ctx->stream, p, split));
+    const int wide = (p.cols + 31) / 32, blocks = (p.tiles - 2 + kJoinTiles - 1) / kJoinTiles;
+    const int split = wide < 8 ? wide : 8;
+    VTLB_CUDA(ctx, vtlb_launch_early(join, dim3((unsigned)blocks * split), dim3(256), 0, ctx->stream, p, split));
     VTLB_LAUNCHED(ctx);
   }
   return VTLB_OK;
