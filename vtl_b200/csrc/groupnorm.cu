@@ -7,6 +7,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "gemm_tc.cuh"
 #include "groupnorm_plan.h"
 #include "ptx.cuh"
 
@@ -165,6 +166,7 @@ struct GnTile {
   int groups, slabs, csplit, channels, rows;
   unsigned units;  // B * slabs
   uint32_t zero;   // 0, unknown to the compiler (gn_after)
+  int boxes, box_rows;  // of a CTA's piece as the tensor map cuts it
 };
 
 template <int VEC>
@@ -200,6 +202,8 @@ struct GnShape {
   int col, lane;      // this thread's
   int rows;           // of this thread: lane, lane + lanes, ... of the CTA's
   int group;          // of the thread's first channel, within the slab
+  bool any;           // whether the CTA has rows at all
+  int r0;             // the CTA's first
   size_t inside;      // the thread's first element, from the unit's (first position, first channel of the slab)
   bool even;          // the pieces of a row fill a warp evenly: cols is a power of two up to 32
 };
@@ -214,6 +218,8 @@ __device__ __forceinline__ GnShape gn_shape(const GnTile& t, int groups, int ran
   p.col = threadIdx.x % p.cols;
   p.lane = threadIdx.x / p.cols;
   const int r0 = min(t.d.S, (rank / t.csplit) * t.rows), r1 = min(t.d.S, r0 + t.rows);
+  p.any = r0 < r1;
+  p.r0 = r0;
   p.rows = p.lane < p.lanes ? max(0, (r1 - r0 - p.lane + p.lanes - 1) / p.lanes) : 0;
   p.group = (p.in_slab + p.col * VEC) / t.d.width;
   p.inside = (size_t)(r0 + p.lane) * t.d.C + p.in_slab + p.col * VEC;
@@ -248,6 +254,7 @@ template <typename T>
 struct GnMail {
   T box[2][kGnMaxCluster][kGnMaxGroups];
   uint64_t full[2];
+  uint64_t data;  // the slots are filled (TMA)
   uint32_t abort;
 };
 __device__ __forceinline__ uint32_t gn_remote(uint32_t addr, int rank) {
@@ -270,6 +277,7 @@ __device__ __forceinline__ void gn_mail_init(GnMail<T>& m) {
   if (threadIdx.x == 0) {
     ptx::mbar_init(ptx::smem_u32(&m.full[0]), 1);
     ptx::mbar_init(ptx::smem_u32(&m.full[1]), 1);
+    ptx::mbar_init(ptx::smem_u32(&m.data), 1);
     m.abort = 0;
     ptx::fence_barrier_init();
   }
@@ -292,6 +300,13 @@ __device__ __forceinline__ void gn_receive(GnMail<T>& m, int turn, unsigned roun
   if (threadIdx.x == 0) ptx::mbar_arrive_expect_tx(bar, (uint32_t)(ctas * groups * sizeof(T)));
   __syncwarp();
   if (!ptx::mbar_wait_bounded(bar, (round >> 1) & 1, &m.abort, 2000000000ull) && (threadIdx.x & 31) == 0)
+    atomicOr(status, VTLB_ST_GEMM_TIMEOUT);
+}
+
+// Waits, for at most two seconds, until the slots are filled for unit number `round` of this CTA.
+template <typename T>
+__device__ __forceinline__ void gn_wait_data(GnMail<T>& m, unsigned round, uint32_t* status) {
+  if (!ptx::mbar_wait_bounded(ptx::smem_u32(&m.data), round & 1, &m.abort, 2000000000ull) && threadIdx.x == 0)
     atomicOr(status, VTLB_ST_GEMM_TIMEOUT);
 }
 
@@ -322,6 +337,36 @@ __device__ __forceinline__ void gn_fetch(float* slots, const float* src, const G
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + i * kGnThreads * 4), "l"(from) : "memory");
     }
 }
+// The same piece by TMA: one thread asks for it, and the threads are spared the requests (16 per thread and unit, a fifth
+// of the backward kernel's time).  Rows lie t.channels apart; rows behind S and channels behind C arrive as zeros.
+__device__ __forceinline__ void gn_fetch_box(float* slots, const CUtensorMap* map, const GnTile& t, const GnUnit& u,
+                                             const GnShape& p, uint32_t bar) {
+  const int c = (int)u.slab * t.groups * t.d.width + p.in_slab;
+  for (int i = 0; i < t.boxes; ++i)
+    ptx::tma_load_3d(ptx::smem_u32(slots + (size_t)i * t.box_rows * t.channels), map, c, p.r0 + i * t.box_rows, (int)u.b, bar);
+}
+template <int VEC, int VPT>
+__device__ __forceinline__ void gn_take_box(GnVec<VEC> (&v)[VPT], const float* slots, const GnTile& t, const GnShape& p) {
+  const float* from = slots + p.lane * t.channels + p.col * VEC;
+  const int step = p.lanes * t.channels;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i, from += step) {
+    if (i < p.rows) {
+      v[i] = gn_load<VEC>(from);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) v[i].e[k] = 0.0f;
+    }
+  }
+}
+// The threads have read their slots: the first warp goes on when all have.
+__device__ __forceinline__ void gn_slots_free() {
+  if (threadIdx.x < 32)
+    asm volatile("bar.sync 1, %0;" ::"n"(kGnThreads) : "memory");
+  else
+    asm volatile("bar.arrive 1, %0;" ::"n"(kGnThreads) : "memory");
+}
+
 template <int VEC, int VPT>
 __device__ __forceinline__ void gn_take(GnVec<VEC> (&v)[VPT], const float* slots, int rows) {
 #pragma unroll
@@ -335,9 +380,9 @@ __device__ __forceinline__ void gn_take(GnVec<VEC> (&v)[VPT], const float* slots
   }
 }
 
-template <int ACT, int VEC, int VPT, bool GROUPED>
+template <int ACT, int VEC, int VPT, bool GROUPED, bool TMA>
 __global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 1024 / kGnThreads)
-    gn_fwd_tile_kernel(const float* x, const float* gamma, const float* beta, GnTile t, double eps, float* y,
+    gn_fwd_tile_kernel(const __grid_constant__ CUtensorMap map, const float* x, const float* gamma, const float* beta, GnTile t, double eps, float* y,
                        float* mean_out, float* rstd_out, uint32_t* status) {
   namespace cg = cooperative_groups;
   constexpr int PAIRS = GROUPED ? 1 : VEC;  // GROUPED: the channels of a thread's piece are all of one group
@@ -345,7 +390,7 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 
   __shared__ double2 sm_pair[kGnThreads * PAIRS];
   __shared__ GnMail<double2> mail;
   __shared__ float2 sm_stat[kGnMaxGroups];
-  extern __shared__ __align__(16) float slots[];
+  extern __shared__ __align__(128) float slots[];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
   const int tid = threadIdx.x, warp = tid >> 5, width = t.d.width;
@@ -358,20 +403,39 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 
   gn_mail_init(mail);
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the kernel in front is done from here on
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  gn_fetch<VEC, VPT>(slots, x, t, u, p);
+  const uint32_t bar = ptx::smem_u32(&mail.data), box_bytes = (uint32_t)(t.boxes * t.box_rows * t.channels * 4);
+  if constexpr (TMA) {
+    if (tid == 0 && p.any) {
+      ptx::mbar_arrive_expect_tx(bar, box_bytes);
+      gn_fetch_box(slots, &map, t, u, p, bar);
+    }
+    if (ctas == 1) __syncthreads();  // (the barrier is ready)
+  } else {
+    gn_fetch<VEC, VPT>(slots, x, t, u, p);
+  }
   if (ctas > 1) cluster.sync();  // everyone's boxes are ready
   for (unsigned round = 0;; ++round) {
     const int turn = round & 1;
     GnVec<VEC> v[VPT];
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    gn_take(v, slots, p.rows);
     const GnUnit next = gn_next(t, u, stride);
-    if (next.unit < t.units) {
-      const uint32_t after = gn_after(t, v);
-      if (gn_groups(t, next) == p.groups)
-        gn_fetch<VEC, VPT>(slots, x, t, next, p, after);
-      else
-        gn_fetch<VEC, VPT>(slots, x, t, next, gn_shape<VEC>(t, gn_groups(t, next), rank), after);
+    if constexpr (TMA) {
+      if (p.any) gn_wait_data(mail, round, status);
+      gn_take_box(v, slots, t, p);
+      gn_slots_free();
+      if (tid == 0 && p.any && next.unit < t.units) {
+        ptx::mbar_arrive_expect_tx(bar, box_bytes);
+        gn_fetch_box(slots, &map, t, next, p, bar);  // (in_slab and r0 are those of every slab)
+      }
+    } else {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      gn_take(v, slots, p.rows);
+      if (next.unit < t.units) {
+        const uint32_t after = gn_after(t, v);
+        if (gn_groups(t, next) == p.groups)
+          gn_fetch<VEC, VPT>(slots, x, t, next, p, after);
+        else
+          gn_fetch<VEC, VPT>(slots, x, t, next, gn_shape<VEC>(t, gn_groups(t, next), rank), after);
+      }
     }
     // A thread's own mean K and squared distances from it in f32, then sums of x and x^2 in f64 from them: the variance
     // loses 2^-53 of the mean square, not 2^-24, and few instructions are f64.
@@ -479,17 +543,18 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 
 }
 
 // Backward.  The channel sums of each CTA go to `sums` [B * rsplit][C] (dz * h, dz) for gn_params_tile_kernel.
-template <int ACT, int VEC, int VPT, bool GROUPED>
+template <int ACT, int VEC, int VPT, bool GROUPED, bool TMA>
 __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 1024 / kGnThreads)
-    gn_bwd_tile_kernel(const float* g, const float* x, const float* gamma, const float* beta, const float* mean,
+    gn_bwd_tile_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_x, const float* g, const float* x, const float* gamma, const float* beta, const float* mean,
                        const float* rstd, GnTile t, float* dx, float2* sums, uint32_t* status) {
   namespace cg = cooperative_groups;
   __shared__ float2 sm_part[kGnThreads * VEC];  // [lane][channel]
   __shared__ float2 sm_chan[kGnThreads * VEC];  // [part][channel]
   __shared__ GnMail<float2> mail;
   __shared__ float2 sm_coef[kGnMaxGroups];
-  extern __shared__ __align__(16) float slots[];
-  float* slots_g = slots + VPT * kGnThreads * VEC;
+  extern __shared__ __align__(128) float slots[];
+  const uint32_t bar = ptx::smem_u32(&mail.data), box_bytes = (uint32_t)(t.boxes * t.box_rows * t.channels * 4);
+  float* slots_g = slots + (TMA ? box_bytes / 4 : VPT * kGnThreads * VEC);
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
   const int tid = threadIdx.x, warp = tid >> 5, width = t.d.width;
@@ -506,8 +571,16 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 
   constexpr int NG = GROUPED ? 1 : VEC;
   float mu_next[NG], rs_next[NG];
   const auto fetch = [&](const GnUnit& w, const GnShape& q, uint32_t after) {
-    gn_fetch<VEC, VPT>(slots, x, t, w, q, after);
-    gn_fetch<VEC, VPT>(slots_g, g, t, w, q, after);
+    if constexpr (TMA) {
+      if (tid == 0 && q.any) {
+        ptx::mbar_arrive_expect_tx(bar, 2 * box_bytes);
+        gn_fetch_box(slots, &map_x, t, w, q, bar);
+        gn_fetch_box(slots_g, &map_g, t, w, q, bar);
+      }
+    } else {
+      gn_fetch<VEC, VPT>(slots, x, t, w, q, after);
+      gn_fetch<VEC, VPT>(slots_g, g, t, w, q, after);
+    }
     if (q.rows) {
       const size_t st = (size_t)w.b * t.d.G + w.slab * t.groups;
 #pragma unroll
@@ -518,6 +591,7 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 
     }
   };
   fetch(u, p, 0);
+  if (TMA && ctas == 1) __syncthreads();  // (the barrier is ready)
   if (ctas > 1) cluster.sync();  // everyone's boxes are ready
   for (unsigned round = 0;; ++round) {
     const int turn = round & 1;
@@ -538,11 +612,19 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 
           be[k] = beta ? __ldg(beta + slab_c + p.col * VEC + k) : 0.0f;
         }
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      gn_take(vx, slots, p.rows);
-      gn_take(vg, slots_g, p.rows);
+      uint32_t after = 0;
+      if constexpr (TMA) {
+        if (p.any) gn_wait_data(mail, round, status);
+        gn_take_box(vx, slots, t, p);
+        gn_take_box(vg, slots_g, t, p);
+        gn_slots_free();
+      } else {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        gn_take(vx, slots, p.rows);
+        gn_take(vg, slots_g, p.rows);
+        after = gn_after(t, vx) | gn_after(t, vg);
+      }
       if (next.unit < t.units) {
-        const uint32_t after = gn_after(t, vx) | gn_after(t, vg);
         if (gn_groups(t, next) == p.groups)
           fetch(next, p, after);
         else
@@ -722,20 +804,21 @@ cudaError_t cluster_launch(vtlb_ctx* ctx, std::atomic<int>* resident, void (*ker
   cfg.gridDim = dim3(clusters * cluster);
   return cudaLaunchKernelEx(&cfg, kern, static_cast<Args&&>(args)...);
 }
-template <int ACT, int VEC, int VPT, bool GROUPED, typename... Args>
+template <int ACT, int VEC, int VPT, bool GROUPED, bool TMA, typename... Args>
 cudaError_t fwd_tile(vtlb_ctx* ctx, const GnTile& t, int cluster, Args... args) {
   static std::atomic<int> resident[kGnMaxCluster + 1];
-  return cluster_launch(ctx, resident, gn_fwd_tile_kernel<ACT, VEC, VPT, GROUPED>, t.units, cluster,
-                        (size_t)kGnThreads * VPT * VEC * 4, args...);
+  const size_t smem = TMA ? (size_t)t.boxes * t.box_rows * t.channels * 4 : (size_t)kGnThreads * VPT * VEC * 4;
+  return cluster_launch(ctx, resident, gn_fwd_tile_kernel<ACT, VEC, VPT, GROUPED, TMA>, t.units, cluster, smem, args...);
 }
-template <int ACT, int VEC, int VPT, bool GROUPED, typename... Args>
+template <int ACT, int VEC, int VPT, bool GROUPED, bool TMA, typename... Args>
 cudaError_t bwd_tile(vtlb_ctx* ctx, const GnTile& t, int cluster, Args... args) {
   static std::atomic<int> resident[kGnMaxCluster + 1];
-  return cluster_launch(ctx, resident, gn_bwd_tile_kernel<ACT, VEC, VPT, GROUPED>, t.units, cluster,
-                        (size_t)kGnThreads * VPT * VEC * 8, args...);
+  const size_t smem = TMA ? (size_t)t.boxes * t.box_rows * t.channels * 8 : (size_t)kGnThreads * VPT * VEC * 8;
+  return cluster_launch(ctx, resident, gn_bwd_tile_kernel<ACT, VEC, VPT, GROUPED, TMA>, t.units, cluster, smem, args...);
 }
 
-GnTile tile_of(const GnDims& d, const GnPlan& p) { return GnTile{d, p.groups, p.slabs, p.csplit, p.channels, p.rows, (unsigned)d.B * (unsigned)p.slabs, 0u}; }
+GnTile tile_of(const GnDims& d, const GnPlan& p) { return GnTile{d, p.groups, p.slabs, p.csplit, p.channels, p.rows, (unsigned)d.B * (unsigned)p.slabs, 0u,
+                p.boxes, p.box_rows}; }
 
 int check_dims(vtlb_ctx* ctx, const char* fn, int B, int S, int C, int groups, int act_kind, GnDims* d) {
   if (B <= 0 || S <= 0 || C <= 0 || groups <= 0 || C % groups)
@@ -751,22 +834,26 @@ int check_dims(vtlb_ctx* ctx, const char* fn, int B, int S, int C, int groups, i
 template <int ACT>
 int gn_forward(vtlb_ctx* ctx, const float* x, GnDims d, const float* gamma, const float* beta, double eps, float* y,
                float* mean, float* rstd) {
-  const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, vtlb_aligned16(x) && vtlb_aligned16(y), 16, 16, ctx->sm_count);
+  const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, vtlb_aligned16(x) && vtlb_aligned16(y), 4, 16, ctx->sm_count);
   if (plan.on_chip) {
     const GnTile t = tile_of(d, plan);
     const int cluster = plan.csplit * plan.rsplit;
-    const bool grouped = plan.vec == 1 || d.width % 4 == 0;
-#define VTLB_GN_FWD(VEC, VPT, GROUPED) \
-  fwd_tile<ACT, VEC, VPT, GROUPED>(ctx, t, cluster, x, gamma, beta, t, eps, y, mean, rstd, ctx->d_status)
-#define VTLB_GN_FWD_VPT(VPT) \
-  case VPT:                  \
-    VTLB_CUDA(ctx, plan.vec == 1 ? VTLB_GN_FWD(1, VPT, true) : grouped ? VTLB_GN_FWD(4, VPT, true) : VTLB_GN_FWD(4, VPT, false)); \
+    const bool grouped = d.width % 4 == 0;
+    CUtensorMap map = {};
+    if (plan.tma)
+      if (int rc = gemm::encode_tmap_3d_f32_plain(ctx, &map, x, d.C, d.S, d.B, plan.channels, plan.box_rows)) return rc;
+#define VTLB_GN_FWD(VEC, VPT, GROUPED, TMA) \
+  fwd_tile<ACT, VEC, VPT, GROUPED, TMA>(ctx, t, cluster, map, x, gamma, beta, t, eps, y, mean, rstd, ctx->d_status)
+#define VTLB_GN_FWD_VPT(VPT)                                                      \
+  case VPT:                                                                       \
+    VTLB_CUDA(ctx, plan.vec == 1 ? VTLB_GN_FWD(1, VPT, true, false)               \
+                   : !plan.tma   ? VTLB_GN_FWD(4, VPT, false, false)              \
+                   : grouped     ? VTLB_GN_FWD(4, VPT, true, true)                \
+                                 : VTLB_GN_FWD(4, VPT, false, true));             \
     break
     switch (plan.vpt) {
       VTLB_GN_FWD_VPT(1);
-      VTLB_GN_FWD_VPT(2);
       VTLB_GN_FWD_VPT(4);
-      VTLB_GN_FWD_VPT(8);
       VTLB_GN_FWD_VPT(16);
     }
 #undef VTLB_GN_FWD_VPT
@@ -793,7 +880,7 @@ template <int ACT>
 int gn_backward(vtlb_ctx* ctx, const float* g, const float* x, GnDims d, const float* gamma, const float* beta,
                 const float* mean, const float* rstd, float* dx, float* dgamma, float* dbeta) {
   const bool aligned = vtlb_aligned16(x) && vtlb_aligned16(g) && vtlb_aligned16(dx);
-  const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, aligned, 8, 8, ctx->sm_count);
+  const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, aligned, 4, 8, ctx->sm_count);
   vtlb_workspace ws(ctx);
   void* scratch = nullptr;
   if (plan.on_chip) {
@@ -803,16 +890,24 @@ int gn_backward(vtlb_ctx* ctx, const float* g, const float* x, GnDims d, const f
     if (dgamma || dbeta)
       if (int rc = ws.get((size_t)rows * d.C * sizeof(float2), &scratch)) return rc;
     float2* sums = (float2*)scratch;
-    const bool grouped = plan.vec == 1 || d.width % 4 == 0;
-#define VTLB_GN_BWD(VEC, VPT, GROUPED) \
-  bwd_tile<ACT, VEC, VPT, GROUPED>(ctx, t, cluster, g, x, gamma, beta, mean, rstd, t, dx, sums, ctx->d_status)
-#define VTLB_GN_BWD_VPT(VPT) \
-  case VPT:                  \
-    VTLB_CUDA(ctx, plan.vec == 1 ? VTLB_GN_BWD(1, VPT, true) : grouped ? VTLB_GN_BWD(4, VPT, true) : VTLB_GN_BWD(4, VPT, false)); \
+    const bool grouped = d.width % 4 == 0;
+    CUtensorMap map_g = {}, map_x = {};
+    if (plan.tma) {
+      if (int rc = gemm::encode_tmap_3d_f32_plain(ctx, &map_g, g, d.C, d.S, d.B, plan.channels, plan.box_rows)) return rc;
+      if (int rc = gemm::encode_tmap_3d_f32_plain(ctx, &map_x, x, d.C, d.S, d.B, plan.channels, plan.box_rows)) return rc;
+    }
+#define VTLB_GN_BWD(VEC, VPT, GROUPED, TMA)                                                                        \
+  bwd_tile<ACT, VEC, VPT, GROUPED, TMA>(ctx, t, cluster, map_g, map_x, g, x, gamma, beta, mean, rstd, t, dx, sums, \
+                                        ctx->d_status)
+#define VTLB_GN_BWD_VPT(VPT)                                                      \
+  case VPT:                                                                       \
+    VTLB_CUDA(ctx, plan.vec == 1 ? VTLB_GN_BWD(1, VPT, true, false)               \
+                   : !plan.tma   ? VTLB_GN_BWD(4, VPT, false, false)              \
+                   : grouped     ? VTLB_GN_BWD(4, VPT, true, true)                \
+                                 : VTLB_GN_BWD(4, VPT, false, true));             \
     break
     switch (plan.vpt) {
       VTLB_GN_BWD_VPT(1);
-      VTLB_GN_BWD_VPT(2);
       VTLB_GN_BWD_VPT(4);
       VTLB_GN_BWD_VPT(8);
     }

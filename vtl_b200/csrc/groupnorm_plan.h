@@ -7,18 +7,20 @@
 struct GnPlan {
   bool on_chip;     // false: the group does not fit a cluster's registers; x is read twice
   int vec;          // channels per load: 4 (16-byte aligned rows) or 1
-  int vpt;          // rows per thread: 1, 2, 4, 8, 16
+  int vpt;          // rows per thread: 1, the middle or the largest number that the kernel at hand has
   int groups;       // per slab; the last slab may have fewer
   int slabs;
   int csplit, rsplit;
   int channels;     // per CTA (a multiple of vec), the last piece of a slab may have fewer
   int rows;         // per CTA, the last stretch may have fewer
+  bool tma;         // the pieces are fetched by TMA, in `boxes` boxes of `box_rows` rows (a multiple of eight) each
+  int boxes, box_rows;
 };
 
 constexpr int kGnThreads = 256, kGnMaxGroups = 32, kGnMaxCluster = 8;
 
-// `most`: the largest vpt of the kernel at hand (registers), `usual`: the one it runs best with.
-inline GnPlan gn_plan(int B, int S, int C, int G, bool aligned, int usual, int most, int sm_count) {
+// The kernels have `middle` and `most` rows per thread to choose from, and one.
+inline GnPlan gn_plan(int B, int S, int C, int G, bool aligned, int middle, int most, int sm_count) {
   GnPlan p = {};
   const int width = C / G;
   p.vec = aligned && C % 4 == 0 ? 4 : 1;
@@ -39,13 +41,16 @@ inline GnPlan gn_plan(int B, int S, int C, int G, bool aligned, int usual, int m
   const auto fits = [&](int vpt, int rsplit) { return (long long)lanes * vpt * rsplit >= S; };
   const int max_r = kGnMaxCluster / p.csplit;
   p.rsplit = 1;
-  while (p.rsplit < max_r && !fits(usual, p.rsplit)) p.rsplit *= 2;
+  while (p.rsplit < max_r && !fits(most, p.rsplit)) p.rsplit *= 2;
   if (!fits(most, p.rsplit)) return p;
   // Too few CTAs for the SMs: shorter stretches.
   while (p.rsplit < max_r && !fits(1, p.rsplit) && (long long)B * p.slabs * p.csplit * p.rsplit * 2 <= sm_count) p.rsplit *= 2;
   p.rows = (S + p.rsplit - 1) / p.rsplit;
-  p.vpt = 1;
-  while ((long long)lanes * p.vpt < p.rows) p.vpt *= 2;
+  p.vpt = p.rows <= lanes ? 1 : p.rows <= lanes * middle ? middle : most;
+  // TMA boxes are at most 256 by 256; rows of less than 64 bytes are not worth one.
+  p.tma = p.vec == 4 && p.channels >= 16 && p.channels <= 256;
+  p.boxes = (p.rows + 255) / 256;
+  p.box_rows = ((p.rows + p.boxes - 1) / p.boxes + 7) / 8 * 8;
   p.on_chip = true;
   return p;
 }
