@@ -207,14 +207,14 @@ struct GnShape {
   size_t inside;      // the thread's first element, from the unit's (first position, first channel of the slab)
   bool even;          // the pieces of a row fill a warp evenly: cols is a power of two up to 32
 };
-template <int VEC>
+template <int T, int VEC>
 __device__ __forceinline__ GnShape gn_shape(const GnTile& t, int groups, int rank) {
   GnShape p;
   p.groups = groups;
   p.in_slab = (rank % t.csplit) * t.channels;
   p.channels = min(t.channels, groups * t.d.width - p.in_slab);
   p.cols = p.channels / VEC;
-  p.lanes = kGnThreads / p.cols;
+  p.lanes = T / p.cols;
   p.col = threadIdx.x % p.cols;
   p.lane = threadIdx.x / p.cols;
   const int r0 = min(t.d.S, (rank / t.csplit) * t.rows), r1 = min(t.d.S, r0 + t.rows);
@@ -301,6 +301,7 @@ __device__ __forceinline__ void gn_receive(GnMail<T>& m, int turn, unsigned roun
   __syncwarp();
   if (!ptx::mbar_wait_bounded(bar, (round >> 1) & 1, &m.abort, 2000000000ull) && (threadIdx.x & 31) == 0)
     atomicOr(status, VTLB_ST_GEMM_TIMEOUT);
+  __syncwarp();  // lanes leave the wait one by one
 }
 
 // Waits, for at most two seconds, until the slots are filled for unit number `round` of this CTA.
@@ -308,6 +309,7 @@ template <typename T>
 __device__ __forceinline__ void gn_wait_data(GnMail<T>& m, unsigned round, uint32_t* status) {
   if (!ptx::mbar_wait_bounded(ptx::smem_u32(&m.data), round & 1, &m.abort, 2000000000ull) && threadIdx.x == 0)
     atomicOr(status, VTLB_ST_GEMM_TIMEOUT);
+  __syncwarp();  // lanes leave the wait one by one, and a warp that is not whole counts as a whole one at a barrier
 }
 
 // Each thread has slots of its own in shared memory, [i][thread], and reads back what it fetched itself.  A slot is
@@ -322,7 +324,7 @@ __device__ __forceinline__ uint32_t gn_after(const GnTile& t, const GnVec<VEC> (
     for (int k = 0; k < VEC; ++k) all |= __float_as_uint(v[i].e[k]);
   return all & t.zero;
 }
-template <int VEC, int VPT>
+template <int T, int VEC, int VPT>
 __device__ __forceinline__ void gn_fetch(float* slots, const float* src, const GnTile& t, const GnUnit& u, const GnShape& p,
                                          uint32_t after = 0) {
   const float* from = src + gn_base(t, u) + p.inside;
@@ -332,9 +334,9 @@ __device__ __forceinline__ void gn_fetch(float* slots, const float* src, const G
   for (int i = 0; i < VPT; ++i, from += step)
     if (i < p.rows) {
       if constexpr (VEC == 4)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * kGnThreads * 16), "l"(from) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * T * 16), "l"(from) : "memory");
       else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + i * kGnThreads * 4), "l"(from) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + i * T * 4), "l"(from) : "memory");
     }
 }
 // The same piece by TMA: one thread asks for it, and the threads are spared the requests (16 per thread and unit, a fifth
@@ -359,20 +361,19 @@ __device__ __forceinline__ void gn_take_box(GnVec<VEC> (&v)[VPT], const float* s
     }
   }
 }
-// The threads have read their slots: the first warp goes on when all have.
-__device__ __forceinline__ void gn_slots_free() {
-  if (threadIdx.x < 32)
-    asm volatile("bar.sync 1, %0;" ::"n"(kGnThreads) : "memory");
-  else
-    asm volatile("bar.arrive 1, %0;" ::"n"(kGnThreads) : "memory");
+// Every thread has read its slots, and the copy engine may write them.  The proxy fence is what holds the copies back: a
+// barrier alone orders the reads' issue, and a read can wait in a busy shared memory for longer than a copy takes.
+__device__ __forceinline__ void gn_slots_read() {
+  ptx::fence_proxy_async();
+  __syncthreads();
 }
 
-template <int VEC, int VPT>
+template <int T, int VEC, int VPT>
 __device__ __forceinline__ void gn_take(GnVec<VEC> (&v)[VPT], const float* slots, int rows) {
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     if (i < rows) {
-      v[i] = gn_load<VEC>(slots + (i * kGnThreads + threadIdx.x) * VEC);
+      v[i] = gn_load<VEC>(slots + (i * T + threadIdx.x) * VEC);
     } else {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) v[i].e[k] = 0.0f;
@@ -381,13 +382,14 @@ __device__ __forceinline__ void gn_take(GnVec<VEC> (&v)[VPT], const float* slots
 }
 
 template <int ACT, int VEC, int VPT, bool GROUPED, bool TMA>
-__global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 1024 / kGnThreads)
+__global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads : 1024 / kGnFwdThreads)
     gn_fwd_tile_kernel(const __grid_constant__ CUtensorMap map, const float* x, const float* gamma, const float* beta, GnTile t, double eps, float* y,
                        float* mean_out, float* rstd_out, uint32_t* status) {
   namespace cg = cooperative_groups;
+  constexpr int T = kGnFwdThreads;
   constexpr int PAIRS = GROUPED ? 1 : VEC;  // GROUPED: the channels of a thread's piece are all of one group
   constexpr int PER = VEC / PAIRS;          // channels per pair of sums
-  __shared__ double2 sm_pair[kGnThreads * PAIRS];
+  __shared__ double2 sm_pair[T * PAIRS];
   __shared__ GnMail<double2> mail;
   __shared__ float2 sm_stat[kGnMaxGroups];
   extern __shared__ __align__(128) float slots[];
@@ -396,7 +398,7 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 
   const int tid = threadIdx.x, warp = tid >> 5, width = t.d.width;
   const GnUnit stride = gn_first(t, gridDim.x / ctas);
   GnUnit u = gn_first(t, blockIdx.x / ctas);
-  GnShape p = gn_shape<VEC>(t, gn_groups(t, u), rank);
+  GnShape p = gn_shape<T, VEC>(t, gn_groups(t, u), rank);
   const int cq = width / PER;  // pairs per group and row
   const bool cq_even = PAIRS == 1 && (cq & (cq - 1)) == 0;
   const double part = 1.0 / ((double)t.d.S * width);
@@ -411,7 +413,7 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 
     }
     if (ctas == 1) __syncthreads();  // (the barrier is ready)
   } else {
-    gn_fetch<VEC, VPT>(slots, x, t, u, p);
+    gn_fetch<T, VEC, VPT>(slots, x, t, u, p);
   }
   if (ctas > 1) cluster.sync();  // everyone's boxes are ready
   for (unsigned round = 0;; ++round) {
@@ -421,20 +423,20 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 
     if constexpr (TMA) {
       if (p.any) gn_wait_data(mail, round, status);
       gn_take_box(v, slots, t, p);
-      gn_slots_free();
+      gn_slots_read();
       if (tid == 0 && p.any && next.unit < t.units) {
         ptx::mbar_arrive_expect_tx(bar, box_bytes);
         gn_fetch_box(slots, &map, t, next, p, bar);  // (in_slab and r0 are those of every slab)
       }
     } else {
       asm volatile("cp.async.wait_all;" ::: "memory");
-      gn_take(v, slots, p.rows);
+      gn_take<T>(v, slots, p.rows);
       if (next.unit < t.units) {
         const uint32_t after = gn_after(t, v);
         if (gn_groups(t, next) == p.groups)
-          gn_fetch<VEC, VPT>(slots, x, t, next, p, after);
+          gn_fetch<T, VEC, VPT>(slots, x, t, next, p, after);
         else
-          gn_fetch<VEC, VPT>(slots, x, t, next, gn_shape<VEC>(t, gn_groups(t, next), rank), after);
+          gn_fetch<T, VEC, VPT>(slots, x, t, next, gn_shape<T, VEC>(t, gn_groups(t, next), rank), after);
       }
     }
     // A thread's own mean K and squared distances from it in f32, then sums of x and x^2 in f64 from them: the variance
@@ -482,12 +484,12 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 
       if (tid < p.groups) {
         double2 s = sm_pair[tid];
 #pragma unroll
-        for (int w = 1; w < kGnThreads / 32; ++w) s.x += sm_pair[w * p.groups + tid].x, s.y += sm_pair[w * p.groups + tid].y;
+        for (int w = 1; w < T / 32; ++w) s.x += sm_pair[w * p.groups + tid].x, s.y += sm_pair[w * p.groups + tid].y;
         gn_send(mail, turn, rank, ctas, tid, s);
       }
     } else {
       // one warp per group of the slab: the pairs of its channels in this CTA, all rows
-      for (int g = warp; g < p.groups; g += kGnThreads / 32) {
+      for (int g = warp; g < p.groups; g += T / 32) {
         const int lo = max(g * width - p.in_slab, 0) / PER, hi = min((g + 1) * width - p.in_slab, p.channels) / PER;
         double2 s = make_double2(0.0, 0.0);
         const int n = hi > lo ? hi - lo : 0, entries = p.channels / PER;
@@ -537,30 +539,31 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 8 ? 1024 / kGnThreads / 2 : 
     }
     if (next.unit >= t.units) break;
     u = next;
-    if (gn_groups(t, u) != p.groups) p = gn_shape<VEC>(t, gn_groups(t, u), rank);
+    if (gn_groups(t, u) != p.groups) p = gn_shape<T, VEC>(t, gn_groups(t, u), rank);
   }
   if (ctas > 1) cluster.sync();  // no CTA leaves while another may still send to it
 }
 
 // Backward.  The channel sums of each CTA go to `sums` [B * rsplit][C] (dz * h, dz) for gn_params_tile_kernel.
 template <int ACT, int VEC, int VPT, bool GROUPED, bool TMA>
-__global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 1024 / kGnThreads)
+__global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads : 1024 / kGnBwdThreads)
     gn_bwd_tile_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_x, const float* g, const float* x, const float* gamma, const float* beta, const float* mean,
                        const float* rstd, GnTile t, float* dx, float2* sums, uint32_t* status) {
   namespace cg = cooperative_groups;
-  __shared__ float2 sm_part[kGnThreads * VEC];  // [lane][channel]
-  __shared__ float2 sm_chan[kGnThreads * VEC];  // [part][channel]
+  constexpr int T = kGnBwdThreads;
+  __shared__ float2 sm_part[T * VEC];  // [lane][channel]
+  __shared__ float2 sm_chan[T * VEC];  // [part][channel]
   __shared__ GnMail<float2> mail;
   __shared__ float2 sm_coef[kGnMaxGroups];
   extern __shared__ __align__(128) float slots[];
   const uint32_t bar = ptx::smem_u32(&mail.data), box_bytes = (uint32_t)(t.boxes * t.box_rows * t.channels * 4);
-  float* slots_g = slots + (TMA ? box_bytes / 4 : VPT * kGnThreads * VEC);
+  float* slots_g = slots + (TMA ? box_bytes / 4 : VPT * T * VEC);
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
   const int tid = threadIdx.x, warp = tid >> 5, width = t.d.width;
   const GnUnit stride = gn_first(t, gridDim.x / ctas);
   GnUnit u = gn_first(t, blockIdx.x / ctas);
-  GnShape p = gn_shape<VEC>(t, gn_groups(t, u), rank);
+  GnShape p = gn_shape<T, VEC>(t, gn_groups(t, u), rank);
   const float count = (float)t.d.S * (float)width;
   const int stretches = ctas / t.csplit, stretch = rank / t.csplit, shift = __ffs(width) - 1;
   const bool aligned_groups = width <= 32 && (width & (width - 1)) == 0 && t.csplit == 1;
@@ -578,8 +581,8 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 
         gn_fetch_box(slots_g, &map_g, t, w, q, bar);
       }
     } else {
-      gn_fetch<VEC, VPT>(slots, x, t, w, q, after);
-      gn_fetch<VEC, VPT>(slots_g, g, t, w, q, after);
+      gn_fetch<T, VEC, VPT>(slots, x, t, w, q, after);
+      gn_fetch<T, VEC, VPT>(slots_g, g, t, w, q, after);
     }
     if (q.rows) {
       const size_t st = (size_t)w.b * t.d.G + w.slab * t.groups;
@@ -617,18 +620,18 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 
         if (p.any) gn_wait_data(mail, round, status);
         gn_take_box(vx, slots, t, p);
         gn_take_box(vg, slots_g, t, p);
-        gn_slots_free();
+        gn_slots_read();
       } else {
         asm volatile("cp.async.wait_all;" ::: "memory");
-        gn_take(vx, slots, p.rows);
-        gn_take(vg, slots_g, p.rows);
+        gn_take<T>(vx, slots, p.rows);
+        gn_take<T>(vg, slots_g, p.rows);
         after = gn_after(t, vx) | gn_after(t, vg);
       }
       if (next.unit < t.units) {
         if (gn_groups(t, next) == p.groups)
           fetch(next, p, after);
         else
-          fetch(next, gn_shape<VEC>(t, gn_groups(t, next), rank), after);
+          fetch(next, gn_shape<T, VEC>(t, gn_groups(t, next), rank), after);
       }
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
@@ -662,10 +665,10 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 
       for (int k = 0; k < VEC; ++k) sm_part[p.lane * p.channels + p.col * VEC + k] = acc[k];
     }
     __syncthreads();
-    int parts = kGnThreads / 32;  // rows of sums per channel in sm_chan
+    int parts = T / 32;  // rows of sums per channel in sm_chan
     if (!p.even) {
-      parts = max(1, min(kGnThreads / p.channels, p.lanes));
-      for (int i = tid; i < parts * p.channels; i += kGnThreads) {
+      parts = max(1, min(T / p.channels, p.lanes));
+      for (int i = tid; i < parts * p.channels; i += T) {
         float2 s = make_float2(0.f, 0.f);
         for (int l = i / p.channels; l < p.lanes; l += parts) {
           const float2 e = sm_part[l * p.channels + i % p.channels];
@@ -675,7 +678,7 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 
       }
       __syncthreads();
     }
-    for (int c0 = warp * 32; c0 < p.channels; c0 += kGnThreads) {  // whole warps
+    for (int c0 = warp * 32; c0 < p.channels; c0 += T) {  // whole warps
       const int ch = c0 + (tid & 31);
       float2 s = make_float2(0.f, 0.f);
       if (ch < p.channels) {
@@ -700,7 +703,7 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 
     if (dx) {
       if (!aligned_groups) {
         __syncthreads();
-        for (int gr = warp; gr < p.groups; gr += kGnThreads / 32) {
+        for (int gr = warp; gr < p.groups; gr += T / 32) {
           const int lo = max(gr * width - p.in_slab, 0), hi = min((gr + 1) * width - p.in_slab, p.channels);
           float2 s = make_float2(0.f, 0.f);
           for (int ch = lo + (tid & 31); ch < hi; ch += 32) s.x += sm_part[ch].x, s.y += sm_part[ch].y;
@@ -741,7 +744,7 @@ __global__ void __launch_bounds__(kGnThreads, VPT > 4 ? 1024 / kGnThreads / 2 : 
     }
     if (next.unit >= t.units) break;
     u = next;
-    if (gn_groups(t, u) != p.groups) p = gn_shape<VEC>(t, gn_groups(t, u), rank);
+    if (gn_groups(t, u) != p.groups) p = gn_shape<T, VEC>(t, gn_groups(t, u), rank);
   }
   if (ctas > 1) cluster.sync();
 }
@@ -773,11 +776,11 @@ __global__ void __launch_bounds__(256) gn_params_tile_kernel(const float2* sums,
 
 // Launches as many clusters as the GPU holds at a time (each goes on to further units), at most one per unit.
 template <typename... KArgs, typename... Args>
-cudaError_t cluster_launch(vtlb_ctx* ctx, std::atomic<int>* resident, void (*kern)(KArgs...), unsigned units, int cluster,
-                           size_t smem, Args&&... args) {
+cudaError_t cluster_launch(vtlb_ctx* ctx, std::atomic<int>* resident, void (*kern)(KArgs...), int threads, unsigned units,
+                           int cluster, size_t smem, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cluster);
-  cfg.blockDim = dim3(kGnThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = ctx->stream;
   cudaLaunchAttribute at[2];
@@ -807,14 +810,14 @@ cudaError_t cluster_launch(vtlb_ctx* ctx, std::atomic<int>* resident, void (*ker
 template <int ACT, int VEC, int VPT, bool GROUPED, bool TMA, typename... Args>
 cudaError_t fwd_tile(vtlb_ctx* ctx, const GnTile& t, int cluster, Args... args) {
   static std::atomic<int> resident[kGnMaxCluster + 1];
-  const size_t smem = TMA ? (size_t)t.boxes * t.box_rows * t.channels * 4 : (size_t)kGnThreads * VPT * VEC * 4;
-  return cluster_launch(ctx, resident, gn_fwd_tile_kernel<ACT, VEC, VPT, GROUPED, TMA>, t.units, cluster, smem, args...);
+  const size_t smem = TMA ? (size_t)t.boxes * t.box_rows * t.channels * 4 : (size_t)kGnFwdThreads * VPT * VEC * 4;
+  return cluster_launch(ctx, resident, gn_fwd_tile_kernel<ACT, VEC, VPT, GROUPED, TMA>, kGnFwdThreads, t.units, cluster, smem, args...);
 }
 template <int ACT, int VEC, int VPT, bool GROUPED, bool TMA, typename... Args>
 cudaError_t bwd_tile(vtlb_ctx* ctx, const GnTile& t, int cluster, Args... args) {
   static std::atomic<int> resident[kGnMaxCluster + 1];
-  const size_t smem = TMA ? (size_t)t.boxes * t.box_rows * t.channels * 8 : (size_t)kGnThreads * VPT * VEC * 8;
-  return cluster_launch(ctx, resident, gn_bwd_tile_kernel<ACT, VEC, VPT, GROUPED, TMA>, t.units, cluster, smem, args...);
+  const size_t smem = TMA ? (size_t)t.boxes * t.box_rows * t.channels * 8 : (size_t)kGnBwdThreads * VPT * VEC * 8;
+  return cluster_launch(ctx, resident, gn_bwd_tile_kernel<ACT, VEC, VPT, GROUPED, TMA>, kGnBwdThreads, t.units, cluster, smem, args...);
 }
 
 GnTile tile_of(const GnDims& d, const GnPlan& p) { return GnTile{d, p.groups, p.slabs, p.csplit, p.channels, p.rows, (unsigned)d.B * (unsigned)p.slabs, 0u,
@@ -834,7 +837,7 @@ int check_dims(vtlb_ctx* ctx, const char* fn, int B, int S, int C, int groups, i
 template <int ACT>
 int gn_forward(vtlb_ctx* ctx, const float* x, GnDims d, const float* gamma, const float* beta, double eps, float* y,
                float* mean, float* rstd) {
-  const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, vtlb_aligned16(x) && vtlb_aligned16(y), 4, 16, ctx->sm_count);
+  const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, vtlb_aligned16(x) && vtlb_aligned16(y), kGnFwdThreads, 4, 16, ctx->sm_count);
   if (plan.on_chip) {
     const GnTile t = tile_of(d, plan);
     const int cluster = plan.csplit * plan.rsplit;
@@ -880,7 +883,7 @@ template <int ACT>
 int gn_backward(vtlb_ctx* ctx, const float* g, const float* x, GnDims d, const float* gamma, const float* beta,
                 const float* mean, const float* rstd, float* dx, float* dgamma, float* dbeta) {
   const bool aligned = vtlb_aligned16(x) && vtlb_aligned16(g) && vtlb_aligned16(dx);
-  const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, aligned, 4, 8, ctx->sm_count);
+  const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, aligned, kGnBwdThreads, 4, 8, ctx->sm_count);
   vtlb_workspace ws(ctx);
   void* scratch = nullptr;
   if (plan.on_chip) {

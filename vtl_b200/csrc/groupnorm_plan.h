@@ -17,10 +17,10 @@ struct GnPlan {
   int boxes, box_rows;
 };
 
-constexpr int kGnThreads = 256, kGnMaxGroups = 32, kGnMaxCluster = 8;
+constexpr int kGnFwdThreads = 512, kGnBwdThreads = 256, kGnMaxGroups = 32, kGnMaxCluster = 8;
 
 // The kernels have `middle` and `most` rows per thread to choose from, and one.
-inline GnPlan gn_plan(int B, int S, int C, int G, bool aligned, int middle, int most, int sm_count) {
+inline GnPlan gn_plan(int B, int S, int C, int G, bool aligned, int threads, int middle, int most, int sm_count) {
   GnPlan p = {};
   const int width = C / G;
   p.vec = aligned && C % 4 == 0 ? 4 : 1;
@@ -33,11 +33,11 @@ inline GnPlan gn_plan(int B, int S, int C, int G, bool aligned, int middle, int 
   p.slabs = (G + p.groups - 1) / p.groups;
   const int slab = p.groups * width, cols = slab / p.vec;
   p.csplit = 1;
-  while ((cols + p.csplit - 1) / p.csplit > kGnThreads && p.csplit < kGnMaxCluster) p.csplit *= 2;
+  while ((cols + p.csplit - 1) / p.csplit > threads && p.csplit < kGnMaxCluster) p.csplit *= 2;
   const int cols_cta = (cols + p.csplit - 1) / p.csplit;
   p.channels = cols_cta * p.vec;
-  if (cols_cta > kGnThreads || p.groups > kGnMaxGroups) return p;
-  const int lanes = kGnThreads / cols_cta;  // rows that a CTA takes in one step
+  if (cols_cta > threads || p.groups > kGnMaxGroups) return p;
+  const int lanes = threads / cols_cta;  // rows that a CTA takes in one step
   const auto fits = [&](int vpt, int rsplit) { return (long long)lanes * vpt * rsplit >= S; };
   const int max_r = kGnMaxCluster / p.csplit;
   p.rsplit = 1;
