@@ -60,115 +60,6 @@ __device__ __forceinline__ float inv_sqrt(double v) {
   return (float)(r * fma(-0.5 * v * r, r, 1.5));
 }
 
-constexpr int kRows = 256;  // rows of x per CTA of the sums below
-
-// Sums of one column of [chunk of rows] in f64 into partial[b][chunk][c]: of x and x^2 (forward), of dz and dz * h.
-template <int ACT, bool BWD>
-__global__ void __launch_bounds__(256) gn_sums_kernel(const float* x, const float* g, const float* gamma,
-                                                      const float* beta, const float* mean, const float* rstd, GnDims d,
-                                                      double2* partial) {
-  __shared__ double2 sm[8][32];
-  const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + cl, chunk = blockIdx.y, b = blockIdx.z;
-  const int r1 = min(d.S, (chunk + 1) * kRows);
-  double2 acc = make_double2(0.0, 0.0);
-  if (c < d.C) {
-    float mu = 0.f, rs = 0.f, ga = 1.f, be = 0.f;
-    if (BWD) {
-      mu = mean[b * d.G + c / d.width], rs = rstd[b * d.G + c / d.width];
-      if (gamma) ga = gamma[c];
-      if (beta) be = beta[c];
-    }
-    for (int r = chunk * kRows + rl; r < r1; r += 8) {
-      const size_t i = ((size_t)b * d.S + r) * d.C + c;
-      const float v = x[i];
-      if (BWD) {
-        const float h = __fmul_rn(__fsub_rn(v, mu), rs), dz = act_bwd<ACT>(g[i], v, mu, rs, ga, be, h);
-        acc.x += (double)dz;
-        acc.y += (double)dz * (double)h;
-      } else {
-        acc.x += (double)v;
-        acc.y += (double)v * (double)v;
-      }
-    }
-  }
-  sm[rl][cl] = acc;
-  __syncthreads();
-  if (rl == 0 && c < d.C) {
-    for (int k = 1; k < 8; ++k) acc.x += sm[k][cl].x, acc.y += sm[k][cl].y;
-    partial[((size_t)b * gridDim.y + chunk) * d.C + c] = acc;
-  }
-}
-
-// One warp per (sample, group): the sums over chunks and channels, in a fixed order.
-template <bool BWD>
-__global__ void __launch_bounds__(256) gn_groups_kernel(const double2* partial, int chunks, GnDims d, const float* gamma,
-                                                        double eps, float* mean, float* rstd, float2* coef) {
-  const int lane = threadIdx.x & 31;
-  const size_t k = (blockIdx.x * (size_t)blockDim.x + threadIdx.x) >> 5;
-  if (k >= (size_t)d.B * d.G) return;
-  const int b = (int)(k / d.G), grp = (int)(k % d.G);
-  double s0 = 0.0, s1 = 0.0;
-  for (int i = lane; i < chunks * d.width; i += 32) {
-    const int c = grp * d.width + i % d.width;
-    const double2 p = partial[((size_t)b * chunks + i / d.width) * d.C + c];
-    const double w = BWD && gamma ? (double)gamma[c] : 1.0;
-    s0 += w * p.x, s1 += w * p.y;
-  }
-  for (int o = 16; o; o >>= 1) s0 += __shfl_xor_sync(~0u, s0, o), s1 += __shfl_xor_sync(~0u, s1, o);
-  if (lane) return;
-  const double n = (double)d.S * d.width;
-  if (BWD) {
-    coef[k] = make_float2((float)(s0 / n), (float)(s1 / n));
-  } else {
-    const double mu = s0 / n, var = s1 / n - mu * mu;
-    mean[k] = (float)mu;
-    rstd[k] = (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + eps));
-  }
-}
-
-// dgamma and dbeta: one thread per channel sums over samples and chunks.
-__global__ void __launch_bounds__(64) gn_params_kernel(const double2* partial, int rows, int C, float* dgamma, float* dbeta) {
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= C) return;
-  double s0 = 0.0, s1 = 0.0;
-  for (int r = 0; r < rows; ++r) s0 += partial[(size_t)r * C + c].x, s1 += partial[(size_t)r * C + c].y;
-  if (dbeta) dbeta[c] = (float)s0;
-  if (dgamma) dgamma[c] = (float)s1;
-}
-
-template <int ACT, bool BWD>
-__global__ void __launch_bounds__(256) gn_apply_kernel(const float* x, const float* g, const float* gamma,
-                                                       const float* beta, const float* mean, const float* rstd,
-                                                       const float2* coef, GnDims d, float* out) {
-  const size_t total = (size_t)d.B * d.S * d.C;
-  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < total; i += (size_t)gridDim.x * blockDim.x) {
-    const int c = (int)(i % d.C);
-    const size_t k = i / ((size_t)d.S * d.C) * d.G + c / d.width;
-    const float mu = mean[k], rs = rstd[k], ga = gamma ? gamma[c] : 1.0f, be = beta ? beta[c] : 0.0f, v = x[i];
-    const float h = __fmul_rn(__fsub_rn(v, mu), rs);
-    if (BWD) {
-      const float dz = act_bwd<ACT>(g[i], v, mu, rs, ga, be, h);
-      const float2 cf = coef[k];
-      out[i] = rs * (ga * dz - cf.x - h * cf.y);
-    } else {
-      out[i] = act<ACT>(ga * h + be);
-    }
-  }
-}
-
-// ---------------------------------------------------------------- groups that fit the registers of a cluster
-// x is read once: it stays in registers between the sums and the result (groupnorm_plan.h).  A cluster goes through
-// several units (a slab of groups of one sample), the next one's values on their way into shared memory while this
-// one's are worked on.  Bound by HBM, 8 bytes per element forward, 12 backward.
-struct GnTile {
-  GnDims d;
-  int groups, slabs, csplit, channels, rows;
-  unsigned units;  // B * slabs
-  uint32_t zero;   // 0, unknown to the compiler (gn_after)
-  int boxes, box_rows;  // of a CTA's piece as the tensor map cuts it
-};
-
 template <int VEC>
 struct GnVec {
   float e[VEC];
@@ -192,20 +83,192 @@ __device__ __forceinline__ void gn_store(float* p, const GnVec<VEC>& v) {
     *p = v.e[0];
 }
 
+// ---------------------------------------------------------------- groups of any size
+// Two passes over x (and g): sums per channel and chunk of kRows positions, then the result.  CTAs take 256 threads as
+// `cols` pieces of VEC channels by 256 / cols rows.
+constexpr int kRows = 256;
+
+struct GnGrid {
+  GnDims d;
+  int shift;  // log2 of the pieces per CTA
+};
+
+template <int ACT, bool BWD, int VEC>
+__global__ void __launch_bounds__(256) gn_sums_kernel(const float* x, const float* g, const float* gamma,
+                                                      const float* beta, const float* mean, const float* rstd, GnGrid t,
+                                                      double2* partial) {
+  __shared__ double2 sm[256 * VEC];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const GnDims d = t.d;
+  const int cols = 1 << t.shift, lanes = 256 >> t.shift, col = threadIdx.x & (cols - 1), lane = threadIdx.x >> t.shift;
+  const int c = (blockIdx.x * cols + col) * VEC, chunk = blockIdx.y, b = blockIdx.z;
+  const int r1 = min(d.S, (chunk + 1) * kRows);
+  double2 acc[VEC] = {};
+  if (c < d.C) {
+    float mu[VEC], rs[VEC], ga[VEC], be[VEC];
+    if (BWD) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const size_t st = (size_t)b * d.G + (c + k) / d.width;
+        mu[k] = mean[st], rs[k] = rstd[st];
+        ga[k] = gamma ? gamma[c + k] : 1.0f, be[k] = beta ? beta[c + k] : 0.0f;
+      }
+    }
+    const size_t base = (size_t)b * d.S * d.C + c;
+#pragma unroll 4
+    for (int r = chunk * kRows + lane; r < r1; r += lanes) {
+      const GnVec<VEC> v = gn_load<VEC>(x + base + (size_t)r * d.C);
+      GnVec<VEC> w = {};
+      if (BWD) w = gn_load<VEC>(g + base + (size_t)r * d.C);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        if (BWD) {
+          const float h = __fmul_rn(__fsub_rn(v.e[k], mu[k]), rs[k]);
+          const float dz = act_bwd<ACT>(w.e[k], v.e[k], mu[k], rs[k], ga[k], be[k], h);
+          acc[k].x += (double)dz;
+          acc[k].y = fma((double)dz, (double)h, acc[k].y);
+        } else {
+          acc[k].x += (double)v.e[k];
+          acc[k].y = fma((double)v.e[k], (double)v.e[k], acc[k].y);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) sm[threadIdx.x * VEC + k] = acc[k];
+  __syncthreads();
+  for (int i = threadIdx.x; i < cols * VEC; i += 256) {
+    const int ch = blockIdx.x * cols * VEC + i;
+    if (ch >= d.C) break;
+    double2 s = sm[i];
+    for (int l = 1; l < lanes; ++l) s.x += sm[l * cols * VEC + i].x, s.y += sm[l * cols * VEC + i].y;
+    partial[((size_t)b * gridDim.y + chunk) * d.C + ch] = s;
+  }
+}
+
+// One warp per (sample, group): the sums over chunks and channels, in a fixed order.
+template <bool BWD>
+__global__ void __launch_bounds__(256) gn_groups_kernel(const double2* partial, int chunks, GnDims d, const float* gamma,
+                                                        double eps, float* mean, float* rstd, float2* coef) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const size_t k = (blockIdx.x * (size_t)blockDim.x + threadIdx.x) >> 5;
+  if (k >= (size_t)d.B * d.G) return;
+  const int b = (int)(k / d.G), grp = (int)(k % d.G);
+  double s0 = 0.0, s1 = 0.0;
+  for (int i = lane; i < chunks * d.width; i += 32) {
+    const int c = grp * d.width + i % d.width;
+    const double2 p = partial[((size_t)b * chunks + i / d.width) * d.C + c];
+    const double w = BWD && gamma ? (double)gamma[c] : 1.0;
+    s0 += w * p.x, s1 += w * p.y;
+  }
+  for (int o = 16; o; o >>= 1) s0 += __shfl_xor_sync(~0u, s0, o), s1 += __shfl_xor_sync(~0u, s1, o);
+  if (lane) return;
+  const double n = (double)d.S * d.width;
+  if (BWD) {
+    coef[k] = make_float2((float)(s0 / n), (float)(s1 / n));
+  } else {
+    const double mu = s0 / n, var = s1 / n - mu * mu;
+    mean[k] = (float)mu;
+    rstd[k] = (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + eps));
+  }
+}
+
+// dgamma and dbeta from the channel sums (dz, dz * h): 8 channels and 32 stretches of rows per CTA, so that few loads of a thread
+// wait for one another (a few hundred rows as a rule: latency, not bytes).
+template <typename PAIR>
+__global__ void __launch_bounds__(256) gn_params_kernel(const PAIR* sums, int rows, int C, float* dgamma, float* dbeta) {
+  __shared__ double2 sm[8][8];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int cl = threadIdx.x & 7, c = blockIdx.x * 8 + cl, warp = threadIdx.x >> 5;
+  double2 s = make_double2(0.0, 0.0);
+  if (c < C) {
+#pragma unroll 8
+    for (int r = threadIdx.x >> 3; r < rows; r += 32) {
+      const PAIR e = sums[(size_t)r * C + c];
+      s.x += (double)e.x, s.y += (double)e.y;
+    }
+  }
+#pragma unroll
+  for (int o = 8; o < 32; o <<= 1) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
+  if ((threadIdx.x & 31) < 8) sm[warp][cl] = s;
+  __syncthreads();
+  if (threadIdx.x >= 8 || c >= C) return;
+  for (int q = 1; q < 8; ++q) s.x += sm[q][cl].x, s.y += sm[q][cl].y;
+  if (dbeta) dbeta[c] = (float)s.x;
+  if (dgamma) dgamma[c] = (float)s.y;
+}
+
+template <int ACT, bool BWD, int VEC>
+__global__ void __launch_bounds__(256) gn_apply_kernel(const float* x, const float* g, const float* gamma,
+                                                       const float* beta, const float* mean, const float* rstd,
+                                                       const float2* coef, GnGrid t, float* out) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const GnDims d = t.d;
+  const int cols = 1 << t.shift, lanes = 256 >> t.shift, col = threadIdx.x & (cols - 1), lane = threadIdx.x >> t.shift;
+  const int c = (blockIdx.x * cols + col) * VEC, chunk = blockIdx.y, b = blockIdx.z;
+  const int r1 = min(d.S, (chunk + 1) * kRows);
+  if (c >= d.C) return;
+  float mu[VEC], rs[VEC], ga[VEC], be[VEC];
+  float2 cf[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    const size_t st = (size_t)b * d.G + (c + k) / d.width;
+    mu[k] = mean[st], rs[k] = rstd[st];
+    ga[k] = gamma ? gamma[c + k] : 1.0f, be[k] = beta ? beta[c + k] : 0.0f;
+    if (BWD) cf[k] = coef[st];
+  }
+  const size_t base = (size_t)b * d.S * d.C + c;
+#pragma unroll 4
+  for (int r = chunk * kRows + lane; r < r1; r += lanes) {
+    const size_t i = base + (size_t)r * d.C;
+    GnVec<VEC> v = gn_load<VEC>(x + i), w = {};
+    if (BWD) w = gn_load<VEC>(g + i);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const float h = __fmul_rn(__fsub_rn(v.e[k], mu[k]), rs[k]);
+      if (BWD) {
+        const float dz = act_bwd<ACT>(w.e[k], v.e[k], mu[k], rs[k], ga[k], be[k], h);
+        v.e[k] = rs[k] * (ga[k] * dz - cf[k].x - h * cf[k].y);
+      } else {
+        v.e[k] = act<ACT>(fmaf(ga[k], h, be[k]));
+      }
+    }
+    gn_store<VEC>(out + i, v);
+  }
+}
+
+// ---------------------------------------------------------------- groups that fit the registers of a cluster
+// x is read once: it stays in registers between the sums and the result (groupnorm_plan.h).  A cluster goes through
+// several units (a slab of groups of one sample), the next one's values on their way into shared memory while this
+// one's are worked on.  Bound by HBM, 8 bytes per element forward, 12 backward.
+struct GnTile {
+  GnDims d;
+  int groups, slabs, csplit, channels, rows;
+  unsigned units;  // B * slabs
+  uint32_t zero;   // 0, unknown to the compiler (gn_after)
+  int boxes, box_rows;  // of a CTA's piece as the tensor map cuts it
+};
+
 // How a CTA's piece of a slab lies on its threads.  The same for all slabs but a narrower last one, so the divisions
 // are done once per kernel, not once per unit (where they took a third of all instructions).
 struct GnShape {
   int groups;         // of the slab
   int in_slab;        // first channel of this CTA, from the slab's first
   int channels;       // of this CTA
-  int cols, lanes;    // pieces of VEC channels in a row, rows per step
+  int cols, lanes;    // pieces of VEC channels in a row, rounded up to a power of two; rows per step
+  int real;           // pieces that there are: the threads of the others have no rows
   int col, lane;      // this thread's
   int rows;           // of this thread: lane, lane + lanes, ... of the CTA's
   int group;          // of the thread's first channel, within the slab
   bool any;           // whether the CTA has rows at all
   int r0;             // the CTA's first
   size_t inside;      // the thread's first element, from the unit's (first position, first channel of the slab)
-  bool even;          // the pieces of a row fill a warp evenly: cols is a power of two up to 32
+  bool even;          // a warp holds whole rows
 };
 template <int T, int VEC>
 __device__ __forceinline__ GnShape gn_shape(const GnTile& t, int groups, int rank) {
@@ -213,17 +276,19 @@ __device__ __forceinline__ GnShape gn_shape(const GnTile& t, int groups, int ran
   p.groups = groups;
   p.in_slab = (rank % t.csplit) * t.channels;
   p.channels = min(t.channels, groups * t.d.width - p.in_slab);
-  p.cols = p.channels / VEC;
-  p.lanes = T / p.cols;
-  p.col = threadIdx.x % p.cols;
-  p.lane = threadIdx.x / p.cols;
+  p.real = p.channels / VEC;
+  const int shift = p.real > 1 ? 32 - __clz(p.real - 1) : 0;
+  p.cols = 1 << shift;
+  p.lanes = T >> shift;
+  p.col = threadIdx.x & (p.cols - 1);
+  p.lane = threadIdx.x >> shift;
   const int r0 = min(t.d.S, (rank / t.csplit) * t.rows), r1 = min(t.d.S, r0 + t.rows);
   p.any = r0 < r1;
   p.r0 = r0;
-  p.rows = p.lane < p.lanes ? max(0, (r1 - r0 - p.lane + p.lanes - 1) / p.lanes) : 0;
+  p.rows = p.col < p.real ? max(0, (r1 - r0 - p.lane + p.lanes - 1) >> (31 - __clz(p.lanes))) : 0;
   p.group = (p.in_slab + p.col * VEC) / t.d.width;
   p.inside = (size_t)(r0 + p.lane) * t.d.C + p.in_slab + p.col * VEC;
-  p.even = p.cols <= 32 && (p.cols & (p.cols - 1)) == 0;
+  p.even = p.cols <= 32;
   return p;
 }
 
@@ -389,7 +454,7 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
   constexpr int T = kGnFwdThreads;
   constexpr int PAIRS = GROUPED ? 1 : VEC;  // GROUPED: the channels of a thread's piece are all of one group
   constexpr int PER = VEC / PAIRS;          // channels per pair of sums
-  __shared__ double2 sm_pair[T * PAIRS];
+  __shared__ double2 sm_pair[T * PAIRS];      // [row lane or warp][entry or group]
   __shared__ GnMail<double2> mail;
   __shared__ float2 sm_stat[kGnMaxGroups];
   extern __shared__ __align__(128) float slots[];
@@ -463,24 +528,33 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
       const double nm = (double)n * (double)mean;
       acc[q] = make_double2(nm, fma(nm, (double)mean, (double)dist));
     }
-    const bool shuffle = p.even && cq_even && cq <= p.cols;
-    if (shuffle) {
-      // lanes of a warp that hold one group: the other rows' (steps of cols), then the other pieces of its channels
+    // The pairs of all rows, per entry (a piece, or a channel of it): by shuffles where a warp holds whole rows.
+    const int entries = p.cols * PAIRS, parts = p.even ? T / 32 : p.lanes;  // of a row; rows of sums
+    const bool whole = p.even && cq_even && cq <= p.cols;  // a group is some lanes of a warp: its entries by shuffles too
+    if (p.even) {
 #pragma unroll
       for (int o = 16; o; o >>= 1) {
-        if (o >= p.cols || o < cq) {
-          acc[0].x += __shfl_xor_sync(~0u, acc[0].x, o);
-          acc[0].y += __shfl_xor_sync(~0u, acc[0].y, o);
+        if (o >= p.cols || (whole && o < cq)) {
+#pragma unroll
+          for (int q = 0; q < PAIRS; ++q) {
+            acc[q].x += __shfl_xor_sync(~0u, acc[q].x, o);
+            acc[q].y += __shfl_xor_sync(~0u, acc[q].y, o);
+          }
         }
       }
       const int lane = tid & 31;
-      if (lane < p.cols && (lane & (cq - 1)) == 0) sm_pair[warp * p.groups + p.group] = acc[0];
+      if (whole) {
+        if (lane < p.real && (lane & (cq - 1)) == 0) sm_pair[warp * p.groups + p.group] = acc[0];
+      } else if (lane < p.cols) {
+#pragma unroll
+        for (int q = 0; q < PAIRS; ++q) sm_pair[warp * entries + lane * PAIRS + q] = acc[q];
+      }
     } else {
 #pragma unroll
       for (int q = 0; q < PAIRS; ++q) sm_pair[tid * PAIRS + q] = acc[q];
     }
     __syncthreads();
-    if (shuffle) {
+    if (whole) {
       if (tid < p.groups) {
         double2 s = sm_pair[tid];
 #pragma unroll
@@ -488,15 +562,12 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
         gn_send(mail, turn, rank, ctas, tid, s);
       }
     } else {
-      // one warp per group of the slab: the pairs of its channels in this CTA, all rows
+      // one warp per group of the slab: its entries in this CTA
       for (int g = warp; g < p.groups; g += T / 32) {
         const int lo = max(g * width - p.in_slab, 0) / PER, hi = min((g + 1) * width - p.in_slab, p.channels) / PER;
         double2 s = make_double2(0.0, 0.0);
-        const int n = hi > lo ? hi - lo : 0, entries = p.channels / PER;
-        for (int i = tid & 31; i < n * p.lanes; i += 32) {
-          const double2 e = sm_pair[(i / n) * entries + lo + i % n];
-          s.x += e.x, s.y += e.y;
-        }
+        for (int q = 0; q < parts; ++q)
+          for (int e = lo + (tid & 31); e < hi; e += 32) s.x += sm_pair[q * entries + e].x, s.y += sm_pair[q * entries + e].y;
 #pragma unroll
         for (int o = 16; o; o >>= 1) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
         if ((tid & 31) == 0) gn_send(mail, turn, rank, ctas, g, s);
@@ -544,15 +615,15 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
   if (ctas > 1) cluster.sync();  // no CTA leaves while another may still send to it
 }
 
-// Backward.  The channel sums of each CTA go to `sums` [B * rsplit][C] (dz * h, dz) for gn_params_tile_kernel.
+// Backward.  The channel sums of each CTA go to `sums` [B * rsplit][C] (dz, dz * h) for gn_params_kernel.
 template <int ACT, int VEC, int VPT, bool GROUPED, bool TMA>
 __global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads : 1024 / kGnBwdThreads)
     gn_bwd_tile_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_x, const float* g, const float* x, const float* gamma, const float* beta, const float* mean,
                        const float* rstd, GnTile t, float* dx, float2* sums, uint32_t* status) {
   namespace cg = cooperative_groups;
   constexpr int T = kGnBwdThreads;
-  __shared__ float2 sm_part[T * VEC];  // [lane][channel]
-  __shared__ float2 sm_chan[T * VEC];  // [part][channel]
+  __shared__ float2 sm_part[T * VEC];  // [channel], weighted
+  __shared__ float2 sm_chan[T * VEC];  // [row lane or warp][channel]
   __shared__ GnMail<float2> mail;
   __shared__ float2 sm_coef[kGnMaxGroups];
   extern __shared__ __align__(128) float slots[];
@@ -640,8 +711,8 @@ __global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads :
         for (int k = 0; k < VEC; ++k) {
           const float m = mu[k % NG], r = rs[k % NG], h = __fmul_rn(__fsub_rn(vx[i].e[k], m), r);
           const float dz = act_bwd<ACT>(vg[i].e[k], vx[i].e[k], m, r, ga[k], be[k], h);
-          acc[k].x = fmaf(dz, h, acc[k].x);
-          acc[k].y += dz;
+          acc[k].x += dz;
+          acc[k].y = fmaf(dz, h, acc[k].y);
           vx[i].e[k] = h, vg[i].e[k] = dz;  // what dx is made of
         }
       }
@@ -658,33 +729,21 @@ __global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads :
       }
       if ((tid & 31) < p.cols) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) sm_chan[warp * p.channels + p.col * VEC + k] = acc[k];
+        for (int k = 0; k < VEC; ++k) sm_chan[(warp * p.cols + p.col) * VEC + k] = acc[k];
       }
-    } else if (p.lane < p.lanes) {
+    } else {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) sm_part[p.lane * p.channels + p.col * VEC + k] = acc[k];
+      for (int k = 0; k < VEC; ++k) sm_chan[tid * VEC + k] = acc[k];
     }
     __syncthreads();
-    int parts = T / 32;  // rows of sums per channel in sm_chan
-    if (!p.even) {
-      parts = max(1, min(T / p.channels, p.lanes));
-      for (int i = tid; i < parts * p.channels; i += T) {
-        float2 s = make_float2(0.f, 0.f);
-        for (int l = i / p.channels; l < p.lanes; l += parts) {
-          const float2 e = sm_part[l * p.channels + i % p.channels];
-          s.x += e.x, s.y += e.y;
-        }
-        sm_chan[i] = s;
-      }
-      __syncthreads();
-    }
+    const int parts = p.even ? T / 32 : p.lanes, padded = p.cols * VEC;  // rows of sums, and how far they are apart
     for (int c0 = warp * 32; c0 < p.channels; c0 += T) {  // whole warps
       const int ch = c0 + (tid & 31);
       float2 s = make_float2(0.f, 0.f);
       if (ch < p.channels) {
         s = sm_chan[ch];
         for (int q = 1; q < parts; ++q) {
-          const float2 e = sm_chan[q * p.channels + ch];
+          const float2 e = sm_chan[q * padded + ch];
           s.x += e.x, s.y += e.y;
         }
         if (sums) sums[((size_t)u.b * stretches + stretch) * t.d.C + slab_c + ch] = s;
@@ -735,7 +794,7 @@ __global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads :
         for (int i = 0; i < VPT; ++i, to += step) {
           if (i >= p.rows) break;
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) vx[i].e[k] = fmaf(ga[k], vg[i].e[k], fmaf(vx[i].e[k], cf[k % NG].x, cf[k % NG].y));
+          for (int k = 0; k < VEC; ++k) vx[i].e[k] = fmaf(ga[k], vg[i].e[k], fmaf(vx[i].e[k], cf[k % NG].y, cf[k % NG].x));
           gn_store<VEC>(to, vx[i]);
         }
       }
@@ -747,31 +806,6 @@ __global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads :
     if (gn_groups(t, u) != p.groups) p = gn_shape<T, VEC>(t, gn_groups(t, u), rank);
   }
   if (ctas > 1) cluster.sync();
-}
-
-// dgamma and dbeta from the channel sums: 8 channels and 32 stretches of rows per CTA, so that few loads of a thread
-// wait for one another (a few hundred rows as a rule: latency, not bytes).
-__global__ void __launch_bounds__(256) gn_params_tile_kernel(const float2* sums, int rows, int C, float* dgamma, float* dbeta) {
-  __shared__ double2 sm[8][8];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int cl = threadIdx.x & 7, c = blockIdx.x * 8 + cl, warp = threadIdx.x >> 5;
-  double2 s = make_double2(0.0, 0.0);
-  if (c < C) {
-#pragma unroll 8
-    for (int r = threadIdx.x >> 3; r < rows; r += 32) {
-      const float2 e = sums[(size_t)r * C + c];
-      s.x += (double)e.x, s.y += (double)e.y;
-    }
-  }
-#pragma unroll
-  for (int o = 8; o < 32; o <<= 1) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
-  if ((threadIdx.x & 31) < 8) sm[warp][cl] = s;
-  __syncthreads();
-  if (threadIdx.x >= 8 || c >= C) return;
-  for (int q = 1; q < 8; ++q) s.x += sm[q][cl].x, s.y += sm[q][cl].y;
-  if (dgamma) dgamma[c] = (float)s.x;
-  if (dbeta) dbeta[c] = (float)s.y;
 }
 
 // Launches as many clusters as the GPU holds at a time (each goes on to further units), at most one per unit.
@@ -790,8 +824,8 @@ cudaError_t cluster_launch(vtlb_ctx* ctx, std::atomic<int>* resident, void (*ker
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
+  cudaError_t e;
+  if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
   unsigned clusters = units;
   if (units > 8) {
     int fit = resident[cluster].load(std::memory_order_relaxed);
@@ -834,6 +868,65 @@ int check_dims(vtlb_ctx* ctx, const char* fn, int B, int S, int C, int groups, i
   return VTLB_OK;
 }
 
+GnGrid grid_of(const GnDims& d, int vec) {
+  GnGrid t{d, 0};
+  while (t.shift < 8 && (1 << t.shift) * vec < d.C && ((1 << t.shift) < 32 || d.S * (1 << t.shift) < kRows * 8)) ++t.shift;
+  return t;  // 32 pieces wide as a rule, wider where there are few rows
+}
+
+template <int ACT, int VEC>
+int gn_forward_general(vtlb_ctx* ctx, const float* x, GnDims d, const float* gamma, const float* beta, double eps, float* y,
+                       float* mean, float* rstd) {
+  const int chunks = (d.S + kRows - 1) / kRows;
+  const GnGrid t = grid_of(d, VEC);
+  const dim3 grid((d.C + (VEC << t.shift) - 1) / (VEC << t.shift), chunks, d.B);
+  vtlb_workspace ws(ctx);
+  void* partial = nullptr;
+  if (int rc = ws.get((size_t)d.B * chunks * d.C * sizeof(double2), &partial)) return rc;
+  const float* none = nullptr;
+  VTLB_CUDA(ctx, vtlb_launch_early(gn_sums_kernel<ACT, false, VEC>, grid, dim3(256), 0, ctx->stream, x, none, none, none, none,
+                                   none, t, (double2*)partial));
+  VTLB_LAUNCHED(ctx);
+  VTLB_CUDA(ctx, vtlb_launch_early(gn_groups_kernel<false>, dim3((unsigned)(((size_t)d.B * d.G + 7) / 8)), dim3(256), 0,
+                                   ctx->stream, (const double2*)partial, chunks, d, none, eps, mean, rstd, (float2*)nullptr));
+  VTLB_LAUNCHED(ctx);
+  VTLB_CUDA(ctx, vtlb_launch_early(gn_apply_kernel<ACT, false, VEC>, grid, dim3(256), 0, ctx->stream, x, none, gamma, beta,
+                                   (const float*)mean, (const float*)rstd, (const float2*)nullptr, t, y));
+  VTLB_LAUNCHED(ctx);
+  return VTLB_OK;
+}
+
+template <int ACT, int VEC>
+int gn_backward_general(vtlb_ctx* ctx, const float* g, const float* x, GnDims d, const float* gamma, const float* beta,
+                        const float* mean, const float* rstd, float* dx, float* dgamma, float* dbeta) {
+  const int chunks = (d.S + kRows - 1) / kRows;
+  const GnGrid t = grid_of(d, VEC);
+  const dim3 grid((d.C + (VEC << t.shift) - 1) / (VEC << t.shift), chunks, d.B);
+  const size_t sums = (size_t)d.B * chunks * d.C * sizeof(double2);
+  vtlb_workspace ws(ctx);
+  void* scratch = nullptr;
+  if (int rc = ws.get(sums + (size_t)d.B * d.G * sizeof(float2), &scratch)) return rc;
+  double2* partial = (double2*)scratch;
+  float2* coef = (float2*)((char*)scratch + sums);
+  VTLB_CUDA(ctx, vtlb_launch_early(gn_sums_kernel<ACT, true, VEC>, grid, dim3(256), 0, ctx->stream, x, g, gamma, beta, mean,
+                                   rstd, t, partial));
+  VTLB_LAUNCHED(ctx);
+  if (dgamma || dbeta) {
+    VTLB_CUDA(ctx, vtlb_launch_early(gn_params_kernel<double2>, dim3((d.C + 7) / 8), dim3(256), 0, ctx->stream,
+                                     (const double2*)partial, d.B * chunks, d.C, dgamma, dbeta));
+    VTLB_LAUNCHED(ctx);
+  }
+  if (!dx) return VTLB_OK;
+  VTLB_CUDA(ctx, vtlb_launch_early(gn_groups_kernel<true>, dim3((unsigned)(((size_t)d.B * d.G + 7) / 8)), dim3(256), 0,
+                                   ctx->stream, (const double2*)partial, chunks, d, gamma, 0.0, (float*)nullptr,
+                                   (float*)nullptr, coef));
+  VTLB_LAUNCHED(ctx);
+  VTLB_CUDA(ctx, vtlb_launch_early(gn_apply_kernel<ACT, true, VEC>, grid, dim3(256), 0, ctx->stream, x, g, gamma, beta, mean,
+                                   rstd, (const float2*)coef, t, dx));
+  VTLB_LAUNCHED(ctx);
+  return VTLB_OK;
+}
+
 template <int ACT>
 int gn_forward(vtlb_ctx* ctx, const float* x, GnDims d, const float* gamma, const float* beta, double eps, float* y,
                float* mean, float* rstd) {
@@ -864,19 +957,8 @@ int gn_forward(vtlb_ctx* ctx, const float* x, GnDims d, const float* gamma, cons
     VTLB_LAUNCHED(ctx);
     return VTLB_OK;
   }
-  const int chunks = (d.S + kRows - 1) / kRows;
-  vtlb_workspace ws(ctx);
-  void* partial = nullptr;
-  if (int rc = ws.get((size_t)d.B * chunks * d.C * sizeof(double2), &partial)) return rc;
-  gn_sums_kernel<ACT, false><<<dim3((d.C + 31) / 32, chunks, d.B), 256, 0, ctx->stream>>>(
-      x, nullptr, nullptr, nullptr, nullptr, nullptr, d, (double2*)partial);
-  VTLB_LAUNCHED(ctx);
-  gn_groups_kernel<false><<<(unsigned)(((size_t)d.B * d.G + 7) / 8), 256, 0, ctx->stream>>>(
-      (const double2*)partial, chunks, d, nullptr, eps, mean, rstd, nullptr);
-  VTLB_LAUNCHED(ctx);
-  gn_apply_kernel<ACT, false><<<ctx->sm_count * 8, 256, 0, ctx->stream>>>(x, nullptr, gamma, beta, mean, rstd, nullptr, d, y);
-  VTLB_LAUNCHED(ctx);
-  return VTLB_OK;
+  return plan.vec == 4 ? gn_forward_general<ACT, 4>(ctx, x, d, gamma, beta, eps, y, mean, rstd)
+                       : gn_forward_general<ACT, 1>(ctx, x, d, gamma, beta, eps, y, mean, rstd);
 }
 
 template <int ACT>
@@ -918,31 +1000,14 @@ int gn_backward(vtlb_ctx* ctx, const float* g, const float* x, GnDims d, const f
 #undef VTLB_GN_BWD
     VTLB_LAUNCHED(ctx);
     if (sums) {
-      VTLB_CUDA(ctx, vtlb_launch_early(gn_params_tile_kernel, dim3((d.C + 7) / 8), dim3(256), 0, ctx->stream,
+      VTLB_CUDA(ctx, vtlb_launch_early(gn_params_kernel<float2>, dim3((d.C + 7) / 8), dim3(256), 0, ctx->stream,
                                        (const float2*)sums, rows, d.C, dgamma, dbeta));
       VTLB_LAUNCHED(ctx);
     }
     return VTLB_OK;
   }
-  const int chunks = (d.S + kRows - 1) / kRows;
-  const size_t sums = (size_t)d.B * chunks * d.C * sizeof(double2);
-  if (int rc = ws.get(sums + (size_t)d.B * d.G * sizeof(float2), &scratch)) return rc;
-  double2* partial = (double2*)scratch;
-  float2* coef = (float2*)((char*)scratch + sums);
-  gn_sums_kernel<ACT, true><<<dim3((d.C + 31) / 32, chunks, d.B), 256, 0, ctx->stream>>>(x, g, gamma, beta, mean, rstd, d,
-                                                                                         partial);
-  VTLB_LAUNCHED(ctx);
-  if (dgamma || dbeta) {
-    gn_params_kernel<<<(d.C + 63) / 64, 64, 0, ctx->stream>>>(partial, d.B * chunks, d.C, dgamma, dbeta);
-    VTLB_LAUNCHED(ctx);
-  }
-  if (!dx) return VTLB_OK;
-  gn_groups_kernel<true><<<(unsigned)(((size_t)d.B * d.G + 7) / 8), 256, 0, ctx->stream>>>(partial, chunks, d, gamma, 0.0,
-                                                                                           nullptr, nullptr, coef);
-  VTLB_LAUNCHED(ctx);
-  gn_apply_kernel<ACT, true><<<ctx->sm_count * 8, 256, 0, ctx->stream>>>(x, g, gamma, beta, mean, rstd, coef, d, dx);
-  VTLB_LAUNCHED(ctx);
-  return VTLB_OK;
+  return plan.vec == 4 ? gn_backward_general<ACT, 4>(ctx, g, x, d, gamma, beta, mean, rstd, dx, dgamma, dbeta)
+                       : gn_backward_general<ACT, 1>(ctx, g, x, d, gamma, beta, mean, rstd, dx, dgamma, dbeta);
 }
 
 }  // namespace

@@ -19,25 +19,27 @@ struct GnPlan {
 
 constexpr int kGnFwdThreads = 512, kGnBwdThreads = 256, kGnMaxGroups = 32, kGnMaxCluster = 8;
 
-// The kernels have `middle` and `most` rows per thread to choose from, and one.
-inline GnPlan gn_plan(int B, int S, int C, int G, bool aligned, int threads, int middle, int most, int sm_count) {
+// The kernels have `middle` and `most` rows per thread to choose from, and one; a row's pieces take a power of two of the
+// threads.
+inline int gn_pow2(int n) {
+  int p = 1;
+  while (p < n) p *= 2;
+  return p;
+}
+
+// The plan with `groups` groups per slab.
+inline GnPlan gn_plan_slab(int B, int S, int C, int G, int vec, int groups, int threads, int middle, int most, int sm_count) {
   GnPlan p = {};
-  const int width = C / G;
-  p.vec = aligned && C % 4 == 0 ? 4 : 1;
-  // Slabs of 32 channels and more: 128-byte pieces of a row.
-  int unit = 1;  // groups whose channels are a multiple of vec
-  while (((long long)unit * width) % p.vec) ++unit;
-  const long long per_unit = (long long)unit * width;
-  p.groups = unit * (int)((32 + per_unit - 1) / per_unit);
-  if (p.groups > G) p.groups = G;
-  p.slabs = (G + p.groups - 1) / p.groups;
-  const int slab = p.groups * width, cols = slab / p.vec;
+  p.vec = vec;
+  p.groups = groups;
+  p.slabs = (G + groups - 1) / groups;
+  const int cols = groups * (C / G) / vec;
   p.csplit = 1;
   while ((cols + p.csplit - 1) / p.csplit > threads && p.csplit < kGnMaxCluster) p.csplit *= 2;
   const int cols_cta = (cols + p.csplit - 1) / p.csplit;
-  p.channels = cols_cta * p.vec;
-  if (cols_cta > threads || p.groups > kGnMaxGroups) return p;
-  const int lanes = threads / cols_cta;  // rows that a CTA takes in one step
+  p.channels = cols_cta * vec;
+  if (cols_cta > threads || groups > kGnMaxGroups) return p;
+  const int lanes = threads / gn_pow2(cols_cta);  // rows that a CTA takes in one step
   const auto fits = [&](int vpt, int rsplit) { return (long long)lanes * vpt * rsplit >= S; };
   const int max_r = kGnMaxCluster / p.csplit;
   p.rsplit = 1;
@@ -48,9 +50,28 @@ inline GnPlan gn_plan(int B, int S, int C, int G, bool aligned, int threads, int
   p.rows = (S + p.rsplit - 1) / p.rsplit;
   p.vpt = p.rows <= lanes ? 1 : p.rows <= lanes * middle ? middle : most;
   // TMA boxes are at most 256 by 256; rows of less than 64 bytes are not worth one.
-  p.tma = p.vec == 4 && p.channels >= 16 && p.channels <= 256;
+  p.tma = vec == 4 && p.channels >= 16 && p.channels <= 256;
   p.boxes = (p.rows + 255) / 256;
   p.box_rows = ((p.rows + p.boxes - 1) / p.boxes + 7) / 8 * 8;
   p.on_chip = true;
   return p;
+}
+
+inline GnPlan gn_plan(int B, int S, int C, int G, bool aligned, int threads, int middle, int most, int sm_count) {
+  const int width = C / G, vec = aligned && C % 4 == 0 ? 4 : 1;
+  int unit = 1;  // groups whose channels are a multiple of vec
+  while (((long long)unit * width) % vec) ++unit;
+  // Slabs of 32 channels and more (128-byte pieces of a row) up to 32 pieces a row, the one that wastes fewest threads;
+  // narrower ones for groups that do not fit otherwise.
+  GnPlan best = {};
+  double best_score = -1.0;
+  for (int groups = unit; groups == unit || (groups <= G && (long long)groups * width <= 32 * vec); groups += unit) {
+    const int k = groups < G ? groups : G;
+    if (k > kGnMaxGroups && k > unit) break;
+    const GnPlan p = gn_plan_slab(B, S, C, G, vec, k, threads, middle, most, sm_count);
+    const int cols = p.channels / vec, channels = k * width;
+    const double score = (p.on_chip ? 4.0 : 0.0) + (channels >= 32 || k == G ? 2.0 : channels / 32.0) + (double)cols / gn_pow2(cols);
+    if (score > best_score + 1e-9) best = p, best_score = score;
+  }
+  return best;
 }
