@@ -1,0 +1,169 @@
+"""Embedding, dropout and group norm captured into CUDA graphs, replayed on other streams beside one another, and called
+from two contexts: each keeps to its own workspace."""
+import numpy as np
+import pytest
+
+import token_ops_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def rt():
+    from cuda.bindings import runtime
+    return runtime
+
+
+def ck(result):
+    err, *rest = result
+    assert int(err) == 0, err
+    return rest[0] if rest else None
+
+
+class Work:
+    """One call of each operator with its own inputs and outputs."""
+
+    def __init__(self, dev, seed):
+        rng = np.random.default_rng(seed)
+        self.dev, self.n, self.V, self.D, self.B, self.S, self.C, self.G = dev, 20000, 300, 12, 3, 700, 64, 4
+        self.ids = (self.V * rng.random(self.n)**3).astype(np.int32)
+        self.W = rng.standard_normal((self.V, self.D)).astype(np.float32)
+        self.g = rng.standard_normal((self.n, self.D)).astype(np.float32)
+        self.x = rng.standard_normal((self.B, self.S, self.C)).astype(np.float32)
+        self.gx = rng.standard_normal(self.x.shape).astype(np.float32)
+        self.seed = seed
+        up = dev.to_device
+        self.d = {k: up(v) for k, v in dict(ids=self.ids, W=self.W, g=self.g, x=self.x, gx=self.gx).items()}
+        self.out = {k: dev.zeros(s) for k, s in dict(y=(self.n, self.D), dW=(self.V, self.D), z=self.x.shape,
+                                                     mean=(self.B, self.G), rstd=(self.B, self.G), dx=self.x.shape,
+                                                     dgamma=self.C, dbeta=self.C).items()}
+
+    def call(self):
+        dev, d, o = self.dev, self.d, self.out
+        dev.embedding_fwd_f32(d["W"], self.V, self.D, d["ids"], self.n, o["y"], scale=2.0, p=0.2, seed=self.seed, step=1,
+                              check=False)
+        dev.embedding_bwd_f32(d["g"], d["ids"], self.n, self.V, self.D, o["dW"], scale=2.0, p=0.2, seed=self.seed, step=1)
+        dev.groupnorm_fwd_f32(d["x"], self.B, self.S, self.C, self.G, None, None, 1e-5, dev.ACT_SILU, o["z"], o["mean"],
+                              o["rstd"])
+        dev.groupnorm_bwd_f32(d["gx"], d["x"], self.B, self.S, self.C, self.G, None, None, o["mean"], o["rstd"], dev.ACT_SILU,
+                              o["dx"], o["dgamma"], o["dbeta"])
+        dev.dropout_fwd_f32(o["z"], o["z"], self.x.size, 0.3, self.seed, 2)
+
+    def results(self):
+        return {k: b.numpy() for k, b in self.out.items()}
+
+    def clear(self):
+        for b in self.out.values():
+            self.dev.memset0(b, b.nbytes)
+        self.dev.sync()
+
+    def free(self):
+        for b in list(self.d.values()) + list(self.out.values()):
+            b.free()
+
+
+def same(a, b):
+    return all(np.array_equal(a[k].view(np.uint32), b[k].view(np.uint32)) for k in a)
+
+
+def capture(dev, work):
+    r = rt()
+    stream = dev.lib.vtlb_stream(dev.h)
+    ck(r.cudaStreamBeginCapture(stream, r.cudaStreamCaptureMode.cudaStreamCaptureModeThreadLocal))
+    try:
+        work.call()
+    finally:
+        graph = ck(r.cudaStreamEndCapture(stream))
+    return graph, ck(r.cudaGraphInstantiate(graph, 0))
+
+
+def test_two_graphs_and_calls_side_by_side(dev):
+    r = rt()
+    works = [Work(dev, s) for s in (1, 2, 3)]
+    for w in works:
+        w.call()
+    want = [w.results() for w in works]
+    w0 = works[0]
+    assert np.array_equal(want[0]["y"].view(np.uint32), ref.embedding_f32(w0.W, w0.ids, 2.0, 0.2, 1, 1).view(np.uint32))
+    dW, tol = ref.embedding_bwd(w0.g, w0.ids, w0.V, 2.0, 0.2, 1, 1)
+    assert (np.abs(want[0]["dW"] - dW) <= tol).all()
+    graphs = [capture(dev, w) for w in works[:2]]
+    # the context's scratch is replaced between capture and replay
+    dev.reserve_scratch(64 << 20)
+    streams = [ck(r.cudaStreamCreateWithFlags(1)) for _ in range(2)]
+    for w in works:
+        w.clear()
+    for _ in range(5):
+        for (_, ex), st in zip(graphs, streams):
+            ck(r.cudaGraphLaunch(ex, st))
+        works[2].call()
+    for st in streams:
+        ck(r.cudaStreamSynchronize(st))
+    dev.sync()
+    for w, v in zip(works, want):
+        assert same(w.results(), v)
+    # new inputs in the same buffers
+    rng = np.random.default_rng(9)
+    ids = rng.integers(-1, w0.V, w0.n).astype(np.int32)
+    dev.h2d_raw(w0.d["ids"], ids.ctypes.data, ids.nbytes)
+    dev.sync()
+    ck(r.cudaGraphLaunch(graphs[0][1], streams[0]))
+    ck(r.cudaStreamSynchronize(streams[0]))
+    assert np.array_equal(w0.results()["y"].view(np.uint32), ref.embedding_f32(w0.W, ids, 2.0, 0.2, 1, 1).view(np.uint32))
+    dW, tol = ref.embedding_bwd(w0.g, ids, w0.V, 2.0, 0.2, 1, 1)
+    assert (np.abs(w0.results()["dW"] - dW) <= tol).all()
+    for graph, ex in graphs:
+        ck(r.cudaGraphExecDestroy(ex))
+        ck(r.cudaGraphDestroy(graph))
+    for st in streams:
+        ck(r.cudaStreamDestroy(st))
+    for w in works:
+        w.free()
+
+
+def test_check_is_refused_under_capture_and_the_capture_goes_on(dev):
+    from vtl_b200.capi import ESTATE, VtlbError
+    r = rt()
+    w = Work(dev, 4)
+    w.call()
+    want = w.results()
+    stream = dev.lib.vtlb_stream(dev.h)
+    ck(r.cudaStreamBeginCapture(stream, r.cudaStreamCaptureMode.cudaStreamCaptureModeThreadLocal))
+    try:
+        with pytest.raises(VtlbError, match="capture") as e:
+            dev.embedding_fwd_f32(w.d["W"], w.V, w.D, w.d["ids"], w.n, w.out["y"], check=True)
+        w.call()
+    finally:
+        graph = ck(r.cudaStreamEndCapture(stream))
+    assert e.value.code == ESTATE
+    ex = ck(r.cudaGraphInstantiate(graph, 0))
+    w.clear()
+    ck(r.cudaGraphLaunch(ex, stream))
+    dev.sync()
+    assert same(w.results(), want)
+    ck(r.cudaGraphExecDestroy(ex))
+    ck(r.cudaGraphDestroy(graph))
+    w.free()
+
+
+def test_two_contexts_at_once(dev):
+    from vtl_b200 import capi
+    other = capi.Device(0)
+    a, b = Work(dev, 5), Work(other, 6)
+    a.call(); b.call()
+    want = a.results(), b.results()
+    for _ in range(10):
+        a.call(); b.call()
+    dev.sync(); other.sync()
+    assert same(a.results(), want[0]) and same(b.results(), want[1])
+    a.free(); b.free()
+    assert other.check_status() == 0
+    other.close()
+
+
+def test_launches_are_the_librarys_own(dev):
+    w = Work(dev, 7)
+    before = dev.launch_count()
+    w.call()
+    # lookup 1; sort, sums, join 3; group norm 1 and 2; dropout 1
+    assert dev.launch_count() - before == 8
+    w.free()

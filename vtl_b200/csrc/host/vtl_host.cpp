@@ -611,6 +611,10 @@ VarPtr Sequential::forward(const VarPtr& train) {
     } else if (relu_next && !std::strcmp(l->kind(), "conv2d")) {
       cur = static_cast<Conv2DLayer*>(l)->forward_with_relu(cur);
       ++i;
+    } else if (fuse_relu && i + 1 < layers.size() && !std::strcmp(l->kind(), "embedding") &&
+               !std::strcmp(layers[i + 1]->kind(), "dropout")) {
+      cur = static_cast<EmbeddingLayer*>(l)->forward_with_dropout(cur, *static_cast<DropoutLayer*>(layers[i + 1].get()));
+      ++i;
     } else {
       cur = l->forward(cur);
     }

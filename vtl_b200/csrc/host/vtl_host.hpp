@@ -327,6 +327,69 @@ struct BatchNorm1DLayer : Layer {
   std::vector<std::pair<std::string, int>> config() const override { return {{"num_features", num_features}}; }
 };
 
+// Dropout from the counter-based generator of include/vtlb.h: every training pass through the layer takes the next step
+// of its key; under no_grad the layer hands its input on.
+struct DropoutLayer : Layer {
+  struct Mask {
+    double p = 0.0;
+    uint64_t seed = 0, step = 0;
+  };
+  std::vector<int> shape;
+  double p;
+  uint64_t seed, step = 0;
+  DropoutLayer(Context* ctx, std::vector<int> shape, double p);
+  Mask next_mask(Context* ctx);
+  VarPtr forward(const VarPtr& input) override;
+  std::vector<int> output_shape() const override { return shape; }
+  const char* kind() const override { return "dropout"; }
+  const char* type_name() const override { return "DropoutLayer"; }
+  std::vector<std::pair<std::string, int>> config() const override { return {{"prob_millionths", (int)(p * 1e6 + 0.5)}}; }
+};
+
+// Table lookup: tokens [batch, ...] (whole numbers in an f32 tensor; anything else, as padding, gives a row of zeros)
+// -> [batch, ..., dim], scaled.  weights [vocabulary, dim] start from N(0, 1).
+struct EmbeddingLayer : Layer {
+  VarPtr weights;
+  std::vector<int> in_shape;
+  int vocabulary, dim;
+  float scale;
+  EmbeddingLayer(Context* ctx, std::vector<int> in_shape, int vocabulary, int dim, float scale);
+  VarPtr forward(const VarPtr& input) override;
+  // Lookup followed by dropout in one launch, forward and backward; the same bits as the two layers.
+  VarPtr forward_with_dropout(const VarPtr& input, DropoutLayer& d);
+  std::vector<VarPtr> variables() override { return {weights}; }
+  std::vector<int> output_shape() const override;
+  const char* kind() const override { return "embedding"; }
+  const char* type_name() const override { return "EmbeddingLayer"; }
+  std::vector<std::pair<std::string, int>> config() const override { return {{"vocabulary", vocabulary}, {"dim", dim}}; }
+
+ private:
+  VarPtr run(const VarPtr& input, const DropoutLayer::Mask& mask);
+};
+
+// Group norm over the positions of a sample and the channels of a group, channels last ([batch, ..., channels]), with
+// the activation behind it; gamma, beta [1, channels].
+struct GroupNormConfig {
+  double eps = 1e-5;
+  int activation = VTLB_ACT_NONE;
+};
+struct GroupNormLayer : Layer {
+  VarPtr gamma, beta;
+  std::vector<int> in_shape;
+  int channels, groups;
+  double eps;
+  int activation;
+  GroupNormLayer(Context* ctx, std::vector<int> in_shape, int groups, GroupNormConfig c);
+  VarPtr forward(const VarPtr& input) override;
+  std::vector<VarPtr> variables() override { return {gamma, beta}; }
+  std::vector<int> output_shape() const override { return in_shape; }
+  const char* kind() const override { return "groupnorm"; }
+  const char* type_name() const override { return "GroupNormLayer"; }
+  std::vector<std::pair<std::string, int>> config() const override {
+    return {{"num_groups", groups}, {"num_channels", channels}, {"activation", activation}};
+  }
+};
+
 // nn/types/loss.v:7-27, nn/loss/mse.v:30-41, nn/loss/softmax_cross_entropy.v
 struct Loss {
   virtual ~Loss() = default;
@@ -357,6 +420,9 @@ class Sequential {
   void avgpool2d(int kh, int kw, int ph, int pw, int sh, int sw);
   void global_avgpool2d();
   void batchnorm1d(int num_features, BatchNorm1DConfig c = {});
+  void embedding(int vocabulary, int dim, double scale = 1.0);
+  void dropout(double p);
+  void groupnorm(int groups, GroupNormConfig c = {});
   void mse_loss();
   void softmax_cross_entropy_loss();
   VarPtr forward(const VarPtr& train);                                  // sequential.v:204-215
@@ -370,7 +436,7 @@ class Sequential {
   void load_weights(const std::string& path, AdamOptimizer* opt = nullptr);
   std::vector<std::unique_ptr<Layer>> layers;
   std::unique_ptr<Loss> loss_fn;
-  bool fuse_relu = true;  // run Linear/Conv + ReLU pairs as one launch
+  bool fuse_relu = true;  // run Linear/Conv + ReLU and embedding + dropout pairs as one launch
 
  private:
   Context ctx_;

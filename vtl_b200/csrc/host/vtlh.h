@@ -54,6 +54,14 @@ int vtlh_model_softmax(vtlh_model* m);
 int vtlh_model_avgpool2d(vtlh_model* m, int kh, int kw, int ph, int pw, int sh, int sw);
 int vtlh_model_global_avgpool2d(vtlh_model* m);
 int vtlh_model_batchnorm1d(vtlh_model* m, int num_features, double eps, double momentum);
+/* embedding: tokens as whole numbers in an f32 tensor [batch, ...] (anything else is padding) -> [batch, ..., dim];
+ * dropout: active in train_step, not in forward; groupnorm: channels last, activation 0 none, 1 ReLU, 2 SiLU */
+int vtlh_model_embedding(vtlh_model* m, int vocabulary, int dim, double scale);
+int vtlh_model_dropout(vtlh_model* m, double p);
+int vtlh_model_groupnorm(vtlh_model* m, int groups, double eps, int activation);
+/* key and next step of the dropout_index-th dropout layer of the model */
+int vtlh_model_get_dropout_state(vtlh_model* m, int dropout_index, unsigned long long* seed, unsigned long long* step);
+int vtlh_model_set_dropout_state(vtlh_model* m, int dropout_index, unsigned long long seed, unsigned long long step);
 int vtlh_model_get_running_stat(vtlh_model* m, int bn_index, int which, float* host); /* 0 mean, 1 variance */
 int vtlh_model_get_sq_avg(vtlh_model* m, int i, float* host);
 

@@ -186,6 +186,35 @@ int vtlh_model_global_avgpool2d(vtlh_model* m) {
 int vtlh_model_batchnorm1d(vtlh_model* m, int num_features, double eps, double momentum) {
   return guard([&] { m->seq->batchnorm1d(num_features, BatchNorm1DConfig{eps, momentum}); });
 }
+int vtlh_model_embedding(vtlh_model* m, int vocabulary, int dim, double scale) {
+  return guard([&] { m->seq->embedding(vocabulary, dim, scale); });
+}
+int vtlh_model_dropout(vtlh_model* m, double p) {
+  return guard([&] { m->seq->dropout(p); });
+}
+int vtlh_model_groupnorm(vtlh_model* m, int groups, double eps, int activation) {
+  return guard([&] { m->seq->groupnorm(groups, GroupNormConfig{eps, activation}); });
+}
+static DropoutLayer& dropout_layer(vtlh_model* m, int index) {
+  int k = 0;
+  for (auto& l : m->seq->layers)
+    if (!std::strcmp(l->kind(), "dropout") && k++ == index) return *static_cast<DropoutLayer*>(l.get());
+  throw Error(VTLB_EINVAL, "no such dropout layer");
+}
+int vtlh_model_get_dropout_state(vtlh_model* m, int index, unsigned long long* seed, unsigned long long* step) {
+  return guard([&] {
+    const DropoutLayer& d = dropout_layer(m, index);
+    if (seed) *seed = d.seed;
+    if (step) *step = d.step;
+  });
+}
+int vtlh_model_set_dropout_state(vtlh_model* m, int index, unsigned long long seed, unsigned long long step) {
+  return guard([&] {
+    DropoutLayer& d = dropout_layer(m, index);
+    d.seed = seed;
+    d.step = step;
+  });
+}
 // running statistics of the i-th BatchNorm1D layer of the model (which = 0: mean, 1: variance)
 int vtlh_model_get_running_stat(vtlh_model* m, int bn_index, int which, float* host) {
   return guard([&] {

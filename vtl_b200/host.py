@@ -58,6 +58,9 @@ def load() -> C.CDLL:
             "vtlh_model_sgd": [vp, d], "vtlh_model_rmsprop": [vp, d, d, d, d],
             "vtlh_model_softmax": [vp], "vtlh_model_avgpool2d": [vp] + [i] * 6,
             "vtlh_model_global_avgpool2d": [vp], "vtlh_model_batchnorm1d": [vp, i, d, d],
+            "vtlh_model_embedding": [vp, i, i, d], "vtlh_model_dropout": [vp, d], "vtlh_model_groupnorm": [vp, i, d, i],
+            "vtlh_model_get_dropout_state": [vp, i, C.POINTER(C.c_ulonglong), C.POINTER(C.c_ulonglong)],
+            "vtlh_model_set_dropout_state": [vp, i, C.c_ulonglong, C.c_ulonglong],
             "vtlh_model_get_running_stat": [vp, i, i, vp], "vtlh_model_get_sq_avg": [vp, i, vp],
             "vtlh_model_save_checkpoint": [vp, C.c_char_p, i, d, i],
             "vtlh_model_load_weights": [vp, C.c_char_p, i],
@@ -205,6 +208,27 @@ class Model:
 
     def batchnorm1d(self, num_features, eps=1e-5, momentum=0.1):
         _ck(self.lib.vtlh_model_batchnorm1d(self.h, int(num_features), float(eps), float(momentum)))
+
+    def embedding(self, vocabulary, dim, scale=1.0):
+        """Tokens, as whole numbers in an f32 buffer [batch, ...], to scaled rows of a table [batch, ..., dim]."""
+        _ck(self.lib.vtlh_model_embedding(self.h, int(vocabulary), int(dim), float(scale)))
+
+    def dropout(self, p=0.5):
+        """Active in train_step, not in forward."""
+        _ck(self.lib.vtlh_model_dropout(self.h, float(p)))
+
+    def groupnorm(self, groups, eps=1e-5, activation="none"):
+        """Channels last; activation "none", "relu" or "silu"."""
+        _ck(self.lib.vtlh_model_groupnorm(self.h, int(groups), float(eps), {"none": 0, "relu": 1, "silu": 2}[activation]))
+
+    def dropout_state(self, dropout_index):
+        """(key, next step) of a dropout layer: with set_dropout_state, what it takes to repeat or resume its masks."""
+        seed, step = C.c_ulonglong(0), C.c_ulonglong(0)
+        _ck(self.lib.vtlh_model_get_dropout_state(self.h, int(dropout_index), C.byref(seed), C.byref(step)))
+        return seed.value, step.value
+
+    def set_dropout_state(self, dropout_index, seed, step):
+        _ck(self.lib.vtlh_model_set_dropout_state(self.h, int(dropout_index), int(seed), int(step)))
 
     def running_stat(self, bn_index, num_features, variance=False):
         out = np.empty(num_features, np.float32)
