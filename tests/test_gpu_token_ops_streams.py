@@ -164,6 +164,6 @@ def test_launches_are_the_librarys_own(dev):
     w = Work(dev, 7)
     before = dev.launch_count()
     w.call()
-    # lookup 1; sort, sums, join 3; group norm 1 and 2; dropout 1
+    # lookup 1; sort, sums and join 3; group norm 1 and 2; dropout 1
     assert dev.launch_count() - before == 8
     w.free()

@@ -808,6 +808,9 @@ __global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads :
   if (ctas > 1) cluster.sync();
 }
 
+// Dynamic shared memory that a launch may ask for without an attribute: 48 KB less the kernels' static arrays.
+constexpr size_t kGnPlainSmem = 4 << 10;
+
 // Launches as many clusters as the GPU holds at a time (each goes on to further units), at most one per unit.
 template <typename... KArgs, typename... Args>
 cudaError_t cluster_launch(vtlb_ctx* ctx, std::atomic<int>* resident, void (*kern)(KArgs...), int threads, unsigned units,
@@ -818,19 +821,27 @@ cudaError_t cluster_launch(vtlb_ctx* ctx, std::atomic<int>* resident, void (*ker
   cfg.dynamicSmemBytes = smem;
   cfg.stream = ctx->stream;
   cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   cudaError_t e;
-  if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
+  if (smem > kGnPlainSmem &&
+      (e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess)
+    return e;
   unsigned clusters = units;
   if (units > 8) {
     int fit = resident[cluster].load(std::memory_order_relaxed);
     if (!fit) {  // asked once per kernel and cluster size: the library runs on one kind of GPU
-      if ((e = cudaOccupancyMaxActiveClusters(&fit, kern, &cfg)) != cudaSuccess) return e;
+      if (cluster > 1) {
+        e = cudaOccupancyMaxActiveClusters(&fit, kern, &cfg);
+      } else {
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, threads, smem);
+        fit *= ctx->sm_count;
+      }
+      if (e != cudaSuccess) return e;
       if (fit < 1) fit = 1;
       resident[cluster].store(fit, std::memory_order_relaxed);
     }
