@@ -339,16 +339,10 @@ __device__ __forceinline__ void zero_absent(const EmbGrad& p, size_t row0, size_
 }
 
 constexpr int kTileMax = 64, kCtaPositions = 2048;  // positions per tile and per CTA
-// Up to this many positions, and up to a table of kOrderTable bytes, every CTA finds the order itself and the sort is no
-// launch of its own (256 positions into 12 MB: 12.0 us against 14.7; into 80 MB 29.2 against 26.5, as there the zeroes
-// hide the sort).
-constexpr int kOrderMax = 256;
-constexpr size_t kOrderTable = (size_t)32 << 20;
 template <bool VEC, bool DROP>
-__global__ void __launch_bounds__(256, 3) embedding_sums_kernel(EmbGrad p, vtlb_mask m, unsigned zero_ctas, int2* order_out) {
+__global__ void __launch_bounds__(256, 3) embedding_sums_kernel(EmbGrad p, vtlb_mask m, unsigned zero_ctas) {
   __shared__ int2 window[kCtaPositions + 2 * kTileMax + 2];  // the sorted positions of this CTA's tiles and a tile around them
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (order_out) asm volatile("griddepcontrol.wait;" ::: "memory");  // no sort in front of this launch
   if (blockIdx.x < zero_ctas) {
     // No wait for the sort: nothing of it is read here, and it started only when everything in front of it was done.
     const size_t each = ((size_t)p.V + zero_ctas - 1) / zero_ctas, row0 = blockIdx.x * each;
@@ -358,43 +352,8 @@ __global__ void __launch_bounds__(256, 3) embedding_sums_kernel(EmbGrad p, vtlb_
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const unsigned cta = blockIdx.x - zero_ctas;
   const int T = p.tile, t0 = (int)(cta / p.slabs) * p.per_cta, w0 = (t0 - 1) * T - 1;
-  const int span = (p.per_cta + 2) * T + 2;
-  if (order_out) {
-    __shared__ uint4 keys4[kOrderMax / 4];
-    uint32_t* keys = reinterpret_cast<uint32_t*>(keys4);
-    for (int i = threadIdx.x; i < span; i += blockDim.x) window[i] = make_int2(-1, 0);
-    for (int j = threadIdx.x; j < kOrderMax; j += blockDim.x) {
-      const int id = j < p.n ? __ldg(p.ids + j) : -1;
-      keys[j] = j >= p.n ? 0xffffffffu : id >= 0 && id < p.V ? (uint32_t)id : (uint32_t)p.V;
-    }
-    __syncthreads();
-    const int quads = (p.n + 3) / 4;
-    for (int j = threadIdx.x; j < p.n; j += blockDim.x) {
-      const uint32_t key = keys[j];
-      int rank = 0;
-      const int own = (j & ~31) / 4;  // the 32 positions that the warp's own are among: eight quads
-#pragma unroll 8
-      for (int i = 0; i < own; ++i) {
-        const uint4 k = keys4[i];
-        rank += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key);
-      }
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const uint32_t k = keys[own * 4 + i];
-        rank += k < key || (k == key && own * 4 + i < j);
-      }
-#pragma unroll 8
-      for (int i = own + 8; i < quads; ++i) {
-        const uint4 k = keys4[i];
-        rank += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key);
-      }
-      if (rank >= w0 && rank - w0 < span) window[rank - w0] = make_int2((int)key, j);
-      if (cta == 0) order_out[rank] = make_int2((int)key, j);  // for the join
-    }
-  } else {
-    for (int i = threadIdx.x; i < span; i += blockDim.x)
-      window[i] = w0 + i >= 0 && w0 + i < p.n ? __ldg(p.sorted + w0 + i) : make_int2(-1, 0);
-  }
+  for (int i = threadIdx.x; i < (p.per_cta + 2) * T + 2; i += blockDim.x)
+    window[i] = w0 + i >= 0 && w0 + i < p.n ? __ldg(p.sorted + w0 + i) : make_int2(-1, 0);
   __syncthreads();
   const int unit = VEC ? threadIdx.x : threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = unit / p.slab, at = (int)(cta % p.slabs) * p.slab + unit % p.slab;
@@ -600,11 +559,8 @@ int embedding_bwd_batch(vtlb_ctx* ctx, vtlb_workspace& ws, const float* g, const
   p.sorted = sorted;
   p.partial = (float*)((char*)scr + list);
 
-  const bool order = n <= kOrderMax && (size_t)V * D * 4 <= kOrderTable;
-  if (!order) {
-    VTLB_CUDA(ctx, sort_positions(ctx, ids, n, V, sorted));
-    VTLB_LAUNCHED(ctx);
-  }
+  VTLB_CUDA(ctx, sort_positions(ctx, ids, n, V, sorted));
+  VTLB_LAUNCHED(ctx);
 
   const unsigned sum_ctas = (unsigned)((p.tiles + p.per_cta - 1) / p.per_cta) * p.slabs;
   // Each zeroing CTA reads all ids, so they are no more than write four times what all of them read, but two per SM
@@ -616,8 +572,7 @@ int embedding_bwd_batch(vtlb_ctx* ctx, vtlb_workspace& ws, const float* g, const
   const unsigned zero_ctas = accumulate ? 0u : (unsigned)(want < (size_t)V ? want : (size_t)V);
   auto sums = vec ? (m.any ? embedding_sums_kernel<true, true> : embedding_sums_kernel<true, false>)
                   : (m.any ? embedding_sums_kernel<false, true> : embedding_sums_kernel<false, false>);
-  VTLB_CUDA(ctx, vtlb_launch_early(sums, dim3(sum_ctas + zero_ctas), dim3(threads), 0, ctx->stream, p, m, zero_ctas,
-                                   order ? sorted : (int2*)nullptr));
+  VTLB_CUDA(ctx, vtlb_launch_early(sums, dim3(sum_ctas + zero_ctas), dim3(threads), 0, ctx->stream, p, m, zero_ctas));
   VTLB_LAUNCHED(ctx);
   if (p.tiles > 2) {
     auto join = vec ? embedding_join_kernel<true> : embedding_join_kernel<false>;
