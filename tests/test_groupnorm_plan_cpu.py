@@ -52,7 +52,9 @@ int main() {
       if (p.tma) {
         CHECK(p.channels <= 256 && p.channels * 4 % 16 == 0 && p.box_rows <= 256 && p.box_rows % 8 == 0);
         CHECK(p.boxes * p.box_rows >= p.rows);
-        CHECK((long long)p.boxes * p.box_rows * p.channels * 4 * (bwd ? 2 : 1) <= 180 * 1024);
+        CHECK((long long)p.boxes * p.box_rows * p.channels * 4 * (bwd ? 2 : 1) <= kGnMaxSmem);
+      } else {
+        CHECK((long long)threads * p.vpt * p.vec * 4 * (bwd ? 2 : 1) <= kGnMaxSmem);
       }
     }
   std::printf("%ld plans, %ld on chip\n", plans, on_chip);

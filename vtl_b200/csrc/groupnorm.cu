@@ -17,49 +17,6 @@ struct GnDims {
   int B, S, C, G, width;  // width = C / G
 };
 
-// 1 / (1 + exp(-z)) in four instructions; expf and IEEE division take some twenty, more than the rest of the forward
-// kernel per element.  In half steps (2^-24, relative): the product z * log2(e) is rounded, which weighs |z| in the
-// power, the approximate power and reciprocal are good to 2 ulp and 1 ulp: |z| + 4 + 1 + 2 together, less for z > 0.
-// Below z = -87.3, where the power passes 2^126, the result is 0 (the logistic function is under 1.2e-38 there).
-__device__ __forceinline__ float logistic(float z) {
-  float e, s;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + e));
-  return s;
-}
-
-template <int ACT>
-__device__ __forceinline__ float act(float z) {
-  if (ACT == VTLB_ACT_RELU) return z < 0.0f ? 0.0f : z;
-  if (ACT == VTLB_ACT_SILU) return z * logistic(z);
-  return z;
-}
-
-// g * act'(z).  ReLU passes the gradient at exactly zero (nn/internal/activation.v:78-87).  z close to zero is
-// evaluated again in f64: rounding must not decide which side it is on.
-template <int ACT>
-__device__ __forceinline__ float act_bwd(float g, float x, float mean, float rstd, float gamma, float beta, float h) {
-  if (ACT == VTLB_ACT_NONE) return g;
-  const float a = __fmul_rn(gamma, h), z = __fadd_rn(a, beta);
-  if (ACT == VTLB_ACT_RELU) {
-    if (fabsf(z) <= 1e-6f * (fabsf(a) + fabsf(beta))) {
-      const double zd = ((double)x - (double)mean) * (double)rstd * (double)gamma + (double)beta;
-      return zd < 0.0 ? 0.0f : g;
-    }
-    return z < 0.0f ? 0.0f : g;
-  }
-  const float s = logistic(z);
-  return g * fmaf(s, fmaf(-z, s, z), s);  // s + s * (z - z * s)
-}
-
-// 1 / sqrt(v), v >= 0, rounded from a value good to 2^-40: an approximate root and one Newton step in f64, a tenth of the
-// time of f64 division and root, which every CTA would sit through between two barriers.
-__device__ __forceinline__ float inv_sqrt(double v) {
-  if (!(v > 1e-30 && v < 1e30)) return (float)(1.0 / sqrt(v));
-  const double r = (double)rsqrtf((float)v);
-  return (float)(r * fma(-0.5 * v * r, r, 1.5));
-}
-
 template <int VEC>
 struct GnVec {
   float e[VEC];
@@ -81,6 +38,129 @@ __device__ __forceinline__ void gn_store(float* p, const GnVec<VEC>& v) {
     *reinterpret_cast<float4*>(p) = make_float4(v.e[0], v.e[1], v.e[2], v.e[3]);
   else
     *p = v.e[0];
+}
+
+// Two f32 operations in one instruction (each rounded as the scalar one is): the kernels below are bound by what the
+// schedulers issue before they are bound by HBM.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+template <int VEC>
+__device__ __forceinline__ GnVec<VEC> gn_splat(float x) {
+  GnVec<VEC> r;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) r.e[k] = x;
+  return r;
+}
+#define VTLB_GN_VEC_OP(NAME, PARAMS, PAIR, SINGLE)                                                                        \
+  template <int VEC>                                                                                                      \
+  __device__ __forceinline__ GnVec<VEC> NAME PARAMS {                                                                     \
+    GnVec<VEC> r;                                                                                                         \
+    if constexpr (VEC == 4) {                                                                                             \
+      _Pragma("unroll") for (int k = 0; k < 4; k += 2) {                                                                  \
+        const float2 t = unpack2(PAIR);                                                                                   \
+        r.e[k] = t.x, r.e[k + 1] = t.y;                                                                                   \
+      }                                                                                                                   \
+    } else {                                                                                                              \
+      const int k = 0;                                                                                                    \
+      r.e[0] = SINGLE;                                                                                                    \
+    }                                                                                                                     \
+    return r;                                                                                                             \
+  }
+#define VTLB_GN_PAIR(v) pack2(v.e[k], v.e[k + 1])
+VTLB_GN_VEC_OP(vadd, (const GnVec<VEC>& a, const GnVec<VEC>& b), add2(VTLB_GN_PAIR(a), VTLB_GN_PAIR(b)),
+               __fadd_rn(a.e[k], b.e[k]))
+VTLB_GN_VEC_OP(vmul, (const GnVec<VEC>& a, const GnVec<VEC>& b), mul2(VTLB_GN_PAIR(a), VTLB_GN_PAIR(b)),
+               __fmul_rn(a.e[k], b.e[k]))
+VTLB_GN_VEC_OP(vfma, (const GnVec<VEC>& a, const GnVec<VEC>& b, const GnVec<VEC>& c),
+               fma2(VTLB_GN_PAIR(a), VTLB_GN_PAIR(b), VTLB_GN_PAIR(c)), fmaf(a.e[k], b.e[k], c.e[k]))
+#undef VTLB_GN_PAIR
+#undef VTLB_GN_VEC_OP
+template <int VEC>
+__device__ __forceinline__ GnVec<VEC> vneg(const GnVec<VEC>& a) {
+  GnVec<VEC> r;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) r.e[k] = -a.e[k];
+  return r;
+}
+
+// 1 / (1 + exp(-z)) in four instructions; expf and IEEE division take some twenty, more than the rest of the forward
+// kernel per element.  In half steps (2^-24, relative): the product z * log2(e) is rounded, which weighs |z| in the
+// power, the approximate power and reciprocal are good to 2 ulp and 1 ulp: |z| + 4 + 1 + 2 together, less for z > 0.
+// Below z = -87.3, where the power passes 2^126, the result is 0 (the logistic function is under 1.2e-38 there).
+template <int VEC>
+__device__ __forceinline__ GnVec<VEC> vlogistic(const GnVec<VEC>& z) {
+  GnVec<VEC> t = vmul(z, gn_splat<VEC>(-1.4426950408889634f));
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t.e[k]) : "f"(t.e[k]));
+  t = vadd(t, gn_splat<VEC>(1.0f));
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t.e[k]) : "f"(t.e[k]));
+  return t;
+}
+
+template <int ACT, int VEC>
+__device__ __forceinline__ GnVec<VEC> act(GnVec<VEC> z) {
+  if (ACT == VTLB_ACT_RELU) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) z.e[k] = z.e[k] < 0.0f ? 0.0f : z.e[k];
+  }
+  return ACT == VTLB_ACT_SILU ? vmul(z, vlogistic(z)) : z;
+}
+
+// g * act'(z), z = gamma * h + beta.  ReLU passes the gradient at exactly zero (nn/internal/activation.v:78-87); z close to
+// zero is evaluated again in f64: rounding must not decide which side it is on.
+template <int ACT, int VEC>
+__device__ __forceinline__ GnVec<VEC> act_bwd(GnVec<VEC> g, const GnVec<VEC>& x, const GnVec<VEC>& mean, const GnVec<VEC>& rstd,
+                                              const GnVec<VEC>& gamma, const GnVec<VEC>& beta, const GnVec<VEC>& h) {
+  if (ACT == VTLB_ACT_RELU) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const float a = __fmul_rn(gamma.e[k], h.e[k]), z = __fadd_rn(a, beta.e[k]);
+      if (fabsf(z) <= 1e-6f * (fabsf(a) + fabsf(beta.e[k]))) {
+        const double zd = ((double)x.e[k] - (double)mean.e[k]) * (double)rstd.e[k] * (double)gamma.e[k] + (double)beta.e[k];
+        g.e[k] = zd < 0.0 ? 0.0f : g.e[k];
+      } else {
+        g.e[k] = z < 0.0f ? 0.0f : g.e[k];
+      }
+    }
+    return g;
+  }
+  if (ACT == VTLB_ACT_SILU) {
+    const GnVec<VEC> z = vfma(gamma, h, beta), s = vlogistic(z);
+    return vmul(g, vfma(s, vfma(vneg(z), s, z), s));  // s + s * (z - z * s)
+  }
+  return g;
+}
+
+// 1 / sqrt(v), v >= 0, rounded from a value good to 2^-40: an approximate root and one Newton step in f64, a tenth of the
+// time of f64 division and root, which every CTA would sit through between two barriers.
+__device__ __forceinline__ float inv_sqrt(double v) {
+  if (!(v > 1e-30 && v < 1e30)) return (float)(1.0 / sqrt(v));
+  const double r = (double)rsqrtf((float)v);
+  return (float)(r * fma(-0.5 * v * r, r, 1.5));
 }
 
 // ---------------------------------------------------------------- groups of any size
@@ -106,29 +186,31 @@ __global__ void __launch_bounds__(256) gn_sums_kernel(const float* x, const floa
   const int r1 = min(d.S, (chunk + 1) * kRows);
   double2 acc[VEC] = {};
   if (c < d.C) {
-    float mu[VEC], rs[VEC], ga[VEC], be[VEC];
+    GnVec<VEC> mu = {}, rs = {}, ga = {}, be = {};
     if (BWD) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         const size_t st = (size_t)b * d.G + (c + k) / d.width;
-        mu[k] = mean[st], rs[k] = rstd[st];
-        ga[k] = gamma ? gamma[c + k] : 1.0f, be[k] = beta ? beta[c + k] : 0.0f;
+        mu.e[k] = mean[st], rs.e[k] = rstd[st];
+        ga.e[k] = gamma ? gamma[c + k] : 1.0f, be.e[k] = beta ? beta[c + k] : 0.0f;
       }
     }
+    const GnVec<VEC> minus = vneg(mu);
     const size_t base = (size_t)b * d.S * d.C + c;
 #pragma unroll 4
     for (int r = chunk * kRows + lane; r < r1; r += lanes) {
       const GnVec<VEC> v = gn_load<VEC>(x + base + (size_t)r * d.C);
-      GnVec<VEC> w = {};
-      if (BWD) w = gn_load<VEC>(g + base + (size_t)r * d.C);
+      if (BWD) {
+        const GnVec<VEC> h = vmul(vadd(v, minus), rs);
+        const GnVec<VEC> dz = act_bwd<ACT>(gn_load<VEC>(g + base + (size_t)r * d.C), v, mu, rs, ga, be, h);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        if (BWD) {
-          const float h = __fmul_rn(__fsub_rn(v.e[k], mu[k]), rs[k]);
-          const float dz = act_bwd<ACT>(w.e[k], v.e[k], mu[k], rs[k], ga[k], be[k], h);
-          acc[k].x += (double)dz;
-          acc[k].y = fma((double)dz, (double)h, acc[k].y);
-        } else {
+        for (int k = 0; k < VEC; ++k) {
+          acc[k].x += (double)dz.e[k];
+          acc[k].y = fma((double)dz.e[k], (double)h.e[k], acc[k].y);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
           acc[k].x += (double)v.e[k];
           acc[k].y = fma((double)v.e[k], (double)v.e[k], acc[k].y);
         }
@@ -213,32 +295,26 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const float* x, const flo
   const int c = (blockIdx.x * cols + col) * VEC, chunk = blockIdx.y, b = blockIdx.z;
   const int r1 = min(d.S, (chunk + 1) * kRows);
   if (c >= d.C) return;
-  float mu[VEC], rs[VEC], ga[VEC], be[VEC];
-  float2 cf[VEC];
+  GnVec<VEC> mu, rs, ga, be, c1 = {}, c2 = {};
 #pragma unroll
   for (int k = 0; k < VEC; ++k) {
     const size_t st = (size_t)b * d.G + (c + k) / d.width;
-    mu[k] = mean[st], rs[k] = rstd[st];
-    ga[k] = gamma ? gamma[c + k] : 1.0f, be[k] = beta ? beta[c + k] : 0.0f;
-    if (BWD) cf[k] = coef[st];
+    mu.e[k] = mean[st], rs.e[k] = rstd[st];
+    ga.e[k] = gamma ? gamma[c + k] : 1.0f, be.e[k] = beta ? beta[c + k] : 0.0f;
+    if (BWD) c1.e[k] = -rs.e[k] * coef[st].x, c2.e[k] = -rs.e[k] * coef[st].y;
   }
+  const GnVec<VEC> minus = vneg(mu), a = vmul(ga, rs);
   const size_t base = (size_t)b * d.S * d.C + c;
 #pragma unroll 4
   for (int r = chunk * kRows + lane; r < r1; r += lanes) {
     const size_t i = base + (size_t)r * d.C;
-    GnVec<VEC> v = gn_load<VEC>(x + i), w = {};
-    if (BWD) w = gn_load<VEC>(g + i);
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      const float h = __fmul_rn(__fsub_rn(v.e[k], mu[k]), rs[k]);
-      if (BWD) {
-        const float dz = act_bwd<ACT>(w.e[k], v.e[k], mu[k], rs[k], ga[k], be[k], h);
-        v.e[k] = rs[k] * (ga[k] * dz - cf[k].x - h * cf[k].y);
-      } else {
-        v.e[k] = act<ACT>(fmaf(ga[k], h, be[k]));
-      }
+    const GnVec<VEC> v = gn_load<VEC>(x + i), dist = vadd(v, minus);
+    if (BWD) {
+      const GnVec<VEC> h = vmul(dist, rs);
+      gn_store<VEC>(out + i, vfma(a, act_bwd<ACT>(gn_load<VEC>(g + i), v, mu, rs, ga, be, h), vfma(h, c2, c1)));
+    } else {
+      gn_store<VEC>(out + i, act<ACT>(vfma(dist, a, be)));
     }
-    gn_store<VEC>(out + i, v);
   }
 }
 
@@ -510,21 +586,35 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
 #pragma unroll
     for (int q = 0; q < PAIRS; ++q) {
       const float n = (float)(p.rows * PER);
-      float sum = 0.0f, dist = 0.0f;
+      float sum = 0.0f, dist = 0.0f, mean;
+      if constexpr (PAIRS == 1) {
+        GnVec<VEC> part = gn_splat<VEC>(0.0f);
 #pragma unroll
-      for (int i = 0; i < VPT; ++i)
+        for (int i = 0; i < VPT; ++i) part = vadd(part, v[i]);
 #pragma unroll
-        for (int k = 0; k < PER; ++k) sum += v[i].e[q * PER + k];
-      const float mean = p.rows ? __fdividef(sum, n) : 0.0f;  // any value near the mean serves
+        for (int k = 0; k < VEC; ++k) sum += part.e[k];
+        mean = p.rows ? __fdividef(sum, n) : 0.0f;  // any value near the mean serves
+        const GnVec<VEC> minus = gn_splat<VEC>(-mean);
+        part = gn_splat<VEC>(0.0f);
 #pragma unroll
-      for (int i = 0; i < VPT; ++i)
-        if (i < p.rows) {
+        for (int i = 0; i < VPT; ++i)
+          if (i < p.rows) {
+            const GnVec<VEC> e = vadd(v[i], minus);
+            part = vfma(e, e, part);
+          }
 #pragma unroll
-          for (int k = 0; k < PER; ++k) {
-            const float e = v[i].e[q * PER + k] - mean;
+        for (int k = 0; k < VEC; ++k) dist += part.e[k];
+      } else {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) sum += v[i].e[q];
+        mean = p.rows ? __fdividef(sum, n) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+          if (i < p.rows) {
+            const float e = v[i].e[q] - mean;
             dist = fmaf(e, e, dist);
           }
-        }
+      }
       const double nm = (double)n * (double)mean;
       acc[q] = make_double2(nm, fma(nm, (double)mean, (double)dist));
     }
@@ -590,22 +680,20 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
     __syncthreads();
     if (p.rows) {
       const int c = (int)u.slab * t.groups * width + p.in_slab + p.col * VEC;
-      float mu[VEC], a[VEC], be[VEC];
+      GnVec<VEC> minus, a, be;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         const float2 st = sm_stat[GROUPED ? p.group : (p.in_slab + p.col * VEC + k) / width];
-        mu[k] = st.x;
-        a[k] = gamma ? st.y * __ldg(gamma + c + k) : st.y;
-        be[k] = beta ? __ldg(beta + c + k) : 0.0f;
+        minus.e[k] = -st.x;
+        a.e[k] = gamma ? st.y * __ldg(gamma + c + k) : st.y;
+        be.e[k] = beta ? __ldg(beta + c + k) : 0.0f;
       }
       float* to = y + gn_base(t, u) + p.inside;
       const size_t step = (size_t)p.lanes * t.d.C;
 #pragma unroll
       for (int i = 0; i < VPT; ++i, to += step) {
         if (i >= p.rows) break;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) v[i].e[k] = act<ACT>(fmaf(__fsub_rn(v[i].e[k], mu[k]), a[k], be[k]));
-        gn_store<VEC>(to, v[i]);
+        gn_store<VEC>(to, act<ACT>(vfma(vadd(v[i], minus), a, be)));
       }
     }
     if (next.unit >= t.units) break;
@@ -673,17 +761,16 @@ __global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads :
     const GnUnit next = gn_next(t, u, stride);
     const int slab_c = (int)u.slab * t.groups * width + p.in_slab;  // first channel of this CTA
     const float own_gamma = gamma && tid < p.channels ? __ldg(gamma + slab_c + tid) : 1.0f;  // of channel tid, for the sums
-    float rs[NG], ga[VEC];
-    float2 acc[VEC] = {};
+    GnVec<VEC> rs = {}, ga = {}, sum1 = gn_splat<VEC>(0.0f), sum2 = sum1;  // of dz and of dz * h
     {
-      float mu[NG], be[VEC];
+      GnVec<VEC> mu = {}, be = {};
       if (p.rows) {
 #pragma unroll
-        for (int k = 0; k < NG; ++k) mu[k] = mu_next[k], rs[k] = rs_next[k];
+        for (int k = 0; k < VEC; ++k) mu.e[k] = mu_next[k % NG], rs.e[k] = rs_next[k % NG];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-          ga[k] = gamma ? __ldg(gamma + slab_c + p.col * VEC + k) : 1.0f;
-          be[k] = beta ? __ldg(beta + slab_c + p.col * VEC + k) : 0.0f;
+          ga.e[k] = gamma ? __ldg(gamma + slab_c + p.col * VEC + k) : 1.0f;
+          be.e[k] = beta ? __ldg(beta + slab_c + p.col * VEC + k) : 0.0f;
         }
       }
       uint32_t after = 0;
@@ -704,19 +791,20 @@ __global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads :
         else
           fetch(next, gn_shape<T, VEC>(t, gn_groups(t, next), rank), after);
       }
+      const GnVec<VEC> minus = vneg(mu);
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         if (i >= p.rows) break;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          const float m = mu[k % NG], r = rs[k % NG], h = __fmul_rn(__fsub_rn(vx[i].e[k], m), r);
-          const float dz = act_bwd<ACT>(vg[i].e[k], vx[i].e[k], m, r, ga[k], be[k], h);
-          acc[k].x += dz;
-          acc[k].y = fmaf(dz, h, acc[k].y);
-          vx[i].e[k] = h, vg[i].e[k] = dz;  // what dx is made of
-        }
+        const GnVec<VEC> h = vmul(vadd(vx[i], minus), rs);
+        vg[i] = act_bwd<ACT>(vg[i], vx[i], mu, rs, ga, be, h);  // dz
+        vx[i] = h;
+        sum1 = vadd(sum1, vg[i]);
+        sum2 = vfma(vg[i], h, sum2);
       }
     }
+    float2 acc[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] = make_float2(sum1.e[k], sum2.e[k]);
     if (p.even) {
 #pragma unroll
       for (int o = 16; o; o >>= 1) {
@@ -780,22 +868,19 @@ __global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads :
       }
       __syncthreads();
       if (p.rows) {
-        float2 cf[NG];  // minus rstd times the two means
+        GnVec<VEC> c1, c2;  // minus rstd times the two means
 #pragma unroll
-        for (int k = 0; k < NG; ++k) {
+        for (int k = 0; k < VEC; ++k) {
           const float2 m = sm_coef[GROUPED ? p.group : (p.in_slab + p.col * VEC + k) / width];
-          cf[k] = make_float2(-rs[k] * m.x, -rs[k] * m.y);
+          c1.e[k] = -rs.e[k] * m.x, c2.e[k] = -rs.e[k] * m.y;
         }
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) ga[k] *= rs[k % NG];
+        ga = vmul(ga, rs);
         float* to = dx + gn_base(t, u) + p.inside;
         const size_t step = (size_t)p.lanes * t.d.C;
 #pragma unroll
         for (int i = 0; i < VPT; ++i, to += step) {
           if (i >= p.rows) break;
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) vx[i].e[k] = fmaf(ga[k], vg[i].e[k], fmaf(vx[i].e[k], cf[k % NG].y, cf[k % NG].x));
-          gn_store<VEC>(to, vx[i]);
+          gn_store<VEC>(to, vfma(ga, vg[i], vfma(vx[i], c2, c1)));
         }
       }
     } else {
@@ -808,12 +893,17 @@ __global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads :
   if (ctas > 1) cluster.sync();
 }
 
-// Dynamic shared memory that a launch may ask for without an attribute: 48 KB less the kernels' static arrays.
-constexpr size_t kGnPlainSmem = 4 << 10;
+// What is known of one kernel: how many clusters of each size the GPU holds at a time (asked once: the library runs on one
+// kind of GPU), and per device whether it has been allowed the most shared memory that any plan asks for.
+struct GnKernelInfo {
+  static constexpr int kDevices = 16;
+  std::atomic<int> resident[kGnMaxCluster + 1];
+  std::atomic<bool> allowed[kDevices];
+};
 
 // Launches as many clusters as the GPU holds at a time (each goes on to further units), at most one per unit.
 template <typename... KArgs, typename... Args>
-cudaError_t cluster_launch(vtlb_ctx* ctx, std::atomic<int>* resident, void (*kern)(KArgs...), int threads, unsigned units,
+cudaError_t cluster_launch(vtlb_ctx* ctx, GnKernelInfo& info, void (*kern)(KArgs...), int threads, unsigned units,
                            int cluster, size_t smem, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cluster);
@@ -828,13 +918,15 @@ cudaError_t cluster_launch(vtlb_ctx* ctx, std::atomic<int>* resident, void (*ker
   cfg.attrs = at;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
   cudaError_t e;
-  if (smem > kGnPlainSmem &&
-      (e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess)
-    return e;
+  std::atomic<bool>* allowed = ctx->device < GnKernelInfo::kDevices ? &info.allowed[ctx->device] : nullptr;
+  if (!allowed || !allowed->load(std::memory_order_relaxed)) {
+    if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kGnMaxSmem)) != cudaSuccess) return e;
+    if (allowed) allowed->store(true, std::memory_order_relaxed);
+  }
   unsigned clusters = units;
   if (units > 8) {
-    int fit = resident[cluster].load(std::memory_order_relaxed);
-    if (!fit) {  // asked once per kernel and cluster size: the library runs on one kind of GPU
+    int fit = info.resident[cluster].load(std::memory_order_relaxed);
+    if (!fit) {
       if (cluster > 1) {
         e = cudaOccupancyMaxActiveClusters(&fit, kern, &cfg);
       } else {
@@ -843,7 +935,7 @@ cudaError_t cluster_launch(vtlb_ctx* ctx, std::atomic<int>* resident, void (*ker
       }
       if (e != cudaSuccess) return e;
       if (fit < 1) fit = 1;
-      resident[cluster].store(fit, std::memory_order_relaxed);
+      info.resident[cluster].store(fit, std::memory_order_relaxed);
     }
     // as few as finish in the same number of rounds: a cluster that finds no room yet would run behind all others
     const unsigned rounds = (units + fit - 1) / fit;
@@ -854,15 +946,15 @@ cudaError_t cluster_launch(vtlb_ctx* ctx, std::atomic<int>* resident, void (*ker
 }
 template <int ACT, int VEC, int VPT, bool GROUPED, bool TMA, typename... Args>
 cudaError_t fwd_tile(vtlb_ctx* ctx, const GnTile& t, int cluster, Args... args) {
-  static std::atomic<int> resident[kGnMaxCluster + 1];
+  static GnKernelInfo info;
   const size_t smem = TMA ? (size_t)t.boxes * t.box_rows * t.channels * 4 : (size_t)kGnFwdThreads * VPT * VEC * 4;
-  return cluster_launch(ctx, resident, gn_fwd_tile_kernel<ACT, VEC, VPT, GROUPED, TMA>, kGnFwdThreads, t.units, cluster, smem, args...);
+  return cluster_launch(ctx, info, gn_fwd_tile_kernel<ACT, VEC, VPT, GROUPED, TMA>, kGnFwdThreads, t.units, cluster, smem, args...);
 }
 template <int ACT, int VEC, int VPT, bool GROUPED, bool TMA, typename... Args>
 cudaError_t bwd_tile(vtlb_ctx* ctx, const GnTile& t, int cluster, Args... args) {
-  static std::atomic<int> resident[kGnMaxCluster + 1];
+  static GnKernelInfo info;
   const size_t smem = TMA ? (size_t)t.boxes * t.box_rows * t.channels * 8 : (size_t)kGnBwdThreads * VPT * VEC * 8;
-  return cluster_launch(ctx, resident, gn_bwd_tile_kernel<ACT, VEC, VPT, GROUPED, TMA>, kGnBwdThreads, t.units, cluster, smem, args...);
+  return cluster_launch(ctx, info, gn_bwd_tile_kernel<ACT, VEC, VPT, GROUPED, TMA>, kGnBwdThreads, t.units, cluster, smem, args...);
 }
 
 GnTile tile_of(const GnDims& d, const GnPlan& p) { return GnTile{d, p.groups, p.slabs, p.csplit, p.channels, p.rows, (unsigned)d.B * (unsigned)p.slabs, 0u,

@@ -18,6 +18,7 @@ struct GnPlan {
 };
 
 constexpr int kGnFwdThreads = 512, kGnBwdThreads = 256, kGnMaxGroups = 32, kGnMaxCluster = 8;
+constexpr int kGnMaxSmem = 150 << 10;  // for the pieces; with the kernels' static arrays within 227 KB
 
 // The kernels have `middle` and `most` rows per thread to choose from, and one; a row's pieces take a power of two of the
 // threads.

@@ -74,9 +74,11 @@ int encode_tmap_3d_u8(vtlb_ctx* ctx, CUtensorMap* out, const void* base, uint64_
 // boxes out of a plain row-major shared-memory tile.
 int encode_tmap_3d_f32_plain(vtlb_ctx* ctx, CUtensorMap* out, const void* base, uint64_t inner, uint64_t rows,
                              uint64_t planes, uint32_t box_inner, uint32_t box_rows) {
-  CUtensorMap probe;
-  int rc = encode_tmap_2d(ctx, &probe, true, base, inner, rows, inner * 4, 32, 1);
-  if (rc) return rc;  // resolves the driver entry point and checks alignment
+  if (!g_encode || !vtlb_aligned16(base) || (inner & 3u)) {
+    CUtensorMap probe;
+    int rc = encode_tmap_2d(ctx, &probe, true, base, inner, rows, inner * 4, 32, 1);
+    if (rc) return rc;  // resolves the driver entry point and checks alignment
+  }
   cuuint64_t dims[3] = {inner, rows, planes};
   cuuint64_t strides[2] = {inner * 4, inner * rows * 4};
   cuuint32_t box[3] = {box_inner, box_rows, 1};
