@@ -180,6 +180,26 @@ def test_relu_passes_its_gradient_by_the_sign_in_64_bits(dev):
         b.free()
 
 
+@pytest.mark.parametrize("B,S,C,G", [(2, 40, 16, 4), (1, 30, 33, 3), (1, 20000, 8, 1)])
+def test_silu_of_large_values(dev, B, S, C, G):
+    """z to a few hundred on both sides: 0 and z, slopes 0 and 1, no infinities."""
+    rng = np.random.default_rng(11)
+    x, g = rng.standard_normal((B, S, C)).astype(np.float32), rng.standard_normal((B, S, C)).astype(np.float32)
+    gamma = np.full(C, 100, np.float32)
+    dx_, dg, dga = dev.to_device(x), dev.to_device(g), dev.to_device(gamma)
+    y, mean, rstd, dx, dgamma, dbeta = (dev.zeros(s) for s in (x.shape, (B, G), (B, G), x.shape, C, C))
+    dev.groupnorm_fwd_f32(dx_, B, S, C, G, dga, None, 1e-5, ref.SILU, y, mean, rstd)
+    want = ref.groupnorm(x, G, gamma, None, 1e-5, ref.SILU)
+    # (below z = -87.3 the logistic function is held at 2^-126)
+    assert (np.abs(y.numpy() - want[0]) <= forward_bounds(x, G, gamma, None, 1e-5, ref.SILU, *want)[0] + 1e-35).all()
+    dev.groupnorm_bwd_f32(dg, dx_, B, S, C, G, dga, None, mean, rstd, ref.SILU, dx, dgamma, dbeta)
+    r = ref.groupnorm_bwd(g, x, G, gamma, None, mean.numpy(), rstd.numpy(), ref.SILU)
+    for out, name, t in zip((dx, dgamma, dbeta), ("dx", "dgamma", "dbeta"), backward_bounds(r, g, gamma, ref.SILU, S)):
+        assert (np.abs(out.numpy() - r[name]) <= t + 1e-33).all(), name
+    for b in (dx_, dg, dga, y, mean, rstd, dx, dgamma, dbeta):
+        b.free()
+
+
 @pytest.mark.parametrize("C,G", [(64, 8), (33, 3)])
 def test_pointers_off_the_16_byte_grid(dev, C, G):
     rng = np.random.default_rng(9)

@@ -19,6 +19,7 @@
 
 // Bits of the device status word (vtlb_check_status).
 #define VTLB_ST_GEMM_TIMEOUT 0x1u  // a pipeline wait inside a tcgen05 GEMM ran out
+#define VTLB_ST_NORM_TIMEOUT 0x2u  // a wait inside group norm did
 
 struct vtlb_ctx {
   int device = 0;

@@ -177,6 +177,8 @@ VTLB_API int vtlb_check_status(vtlb_ctx* ctx, uint32_t* status) {
     return vtlb_fail(ctx, VTLB_ETIMEOUT,
                      "a tcgen05 GEMM pipeline wait ran out (status 0x%x); its output is invalid",
                      st);
+  if (st & VTLB_ST_NORM_TIMEOUT)
+    return vtlb_fail(ctx, VTLB_ETIMEOUT, "a wait inside group norm ran out (status 0x%x); its output is invalid", st);
   return VTLB_OK;
 }
 

@@ -106,19 +106,20 @@ __device__ __forceinline__ GnVec<VEC> vneg(const GnVec<VEC>& a) {
   return r;
 }
 
-// 1 / (1 + exp(-z)) in four instructions; expf and IEEE division take some twenty, more than the rest of the forward
-// kernel per element.  In half steps (2^-24, relative): the product z * log2(e) is rounded, which weighs |z| in the
-// power, the approximate power and reciprocal are good to 2 ulp and 1 ulp: |z| + 4 + 1 + 2 together, less for z > 0.
-// Below z = -87.3, where the power passes 2^126, the result is 0 (the logistic function is under 1.2e-38 there).
+// e = exp(-z) and s = 1 / (1 + e); expf and IEEE division take some twenty instructions, more than the rest of the forward
+// kernel per element.  e is held at 2^126 at most, so that e * s stays a number: below z = -87.3 s is 1.2e-38.
+// In half steps (2^-24, relative): the product z * log2(e) is rounded, which weighs |z| in the power; the approximate
+// power is good to 2 ulp, the sum to half an ulp, the approximate reciprocal to 1 ulp: |z| + 4 + 1 + 2 for s, less for
+// z > 0.  (A power on the FMA pipe for one element of four and one reciprocal for two were tried: no gain, the kernels
+// wait for HBM.)
 template <int VEC>
-__device__ __forceinline__ GnVec<VEC> vlogistic(const GnVec<VEC>& z) {
-  GnVec<VEC> t = vmul(z, gn_splat<VEC>(-1.4426950408889634f));
+__device__ __forceinline__ void vlogistic(const GnVec<VEC>& z, GnVec<VEC>& e, GnVec<VEC>& s) {
+  e = vmul(z, gn_splat<VEC>(-1.4426950408889634f));
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t.e[k]) : "f"(t.e[k]));
-  t = vadd(t, gn_splat<VEC>(1.0f));
+  for (int k = 0; k < VEC; ++k) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.e[k]) : "f"(fminf(e.e[k], 126.0f)));
+  s = vadd(e, gn_splat<VEC>(1.0f));
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t.e[k]) : "f"(t.e[k]));
-  return t;
+  for (int k = 0; k < VEC; ++k) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.e[k]) : "f"(s.e[k]));
 }
 
 template <int ACT, int VEC>
@@ -127,7 +128,12 @@ __device__ __forceinline__ GnVec<VEC> act(GnVec<VEC> z) {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) z.e[k] = z.e[k] < 0.0f ? 0.0f : z.e[k];
   }
-  return ACT == VTLB_ACT_SILU ? vmul(z, vlogistic(z)) : z;
+  if (ACT == VTLB_ACT_SILU) {
+    GnVec<VEC> e, s;
+    vlogistic(z, e, s);
+    return vmul(z, s);
+  }
+  return z;
 }
 
 // g * act'(z), z = gamma * h + beta.  ReLU passes the gradient at exactly zero (nn/internal/activation.v:78-87); z close to
@@ -149,8 +155,10 @@ __device__ __forceinline__ GnVec<VEC> act_bwd(GnVec<VEC> g, const GnVec<VEC>& x,
     return g;
   }
   if (ACT == VTLB_ACT_SILU) {
-    const GnVec<VEC> z = vfma(gamma, h, beta), s = vlogistic(z);
-    return vmul(g, vfma(s, vfma(vneg(z), s, z), s));  // s + s * (z - z * s)
+    const GnVec<VEC> z = vfma(gamma, h, beta);
+    GnVec<VEC> e, s;
+    vlogistic(z, e, s);
+    return vmul(g, vfma(s, vmul(z, vmul(e, s)), s));  // s + s * z * (1 - s), and 1 - s = e * s without cancellation
   }
   return g;
 }
@@ -441,7 +449,7 @@ __device__ __forceinline__ void gn_receive(GnMail<T>& m, int turn, unsigned roun
   if (threadIdx.x == 0) ptx::mbar_arrive_expect_tx(bar, (uint32_t)(ctas * groups * sizeof(T)));
   __syncwarp();
   if (!ptx::mbar_wait_bounded(bar, (round >> 1) & 1, &m.abort, 2000000000ull) && (threadIdx.x & 31) == 0)
-    atomicOr(status, VTLB_ST_GEMM_TIMEOUT);
+    atomicOr(status, VTLB_ST_NORM_TIMEOUT);
   __syncwarp();  // lanes leave the wait one by one
 }
 
@@ -449,8 +457,19 @@ __device__ __forceinline__ void gn_receive(GnMail<T>& m, int turn, unsigned roun
 template <typename T>
 __device__ __forceinline__ void gn_wait_data(GnMail<T>& m, unsigned round, uint32_t* status) {
   if (!ptx::mbar_wait_bounded(ptx::smem_u32(&m.data), round & 1, &m.abort, 2000000000ull) && threadIdx.x == 0)
-    atomicOr(status, VTLB_ST_GEMM_TIMEOUT);
+    atomicOr(status, VTLB_ST_NORM_TIMEOUT);
   __syncwarp();  // lanes leave the wait one by one, and a warp that is not whole counts as a whole one at a barrier
+}
+
+// Every copy has been waited for, unless a wait ran out: then the one under way gets another second before the CTA and its
+// shared memory go.
+template <typename T>
+__device__ __forceinline__ void gn_last_copies(GnMail<T>& m) {
+  if (!*(volatile uint32_t*)&m.abort || threadIdx.x) return;
+  for (uint32_t parity = 0; parity < 2; ++parity) {
+    uint32_t none = 0;
+    ptx::mbar_wait_bounded(ptx::smem_u32(&m.data), parity, &none, 1000000000ull);
+  }
 }
 
 // Each thread has slots of its own in shared memory, [i][thread], and reads back what it fetched itself.  A slot is
@@ -565,7 +584,7 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
       if (p.any) gn_wait_data(mail, round, status);
       gn_take_box(v, slots, t, p);
       gn_slots_read();
-      if (tid == 0 && p.any && next.unit < t.units) {
+      if (tid == 0 && p.any && next.unit < t.units && !mail.abort) {
         ptx::mbar_arrive_expect_tx(bar, box_bytes);
         gn_fetch_box(slots, &map, t, next, p, bar);  // (in_slab and r0 are those of every slab)
       }
@@ -700,6 +719,7 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
     u = next;
     if (gn_groups(t, u) != p.groups) p = gn_shape<T, VEC>(t, gn_groups(t, u), rank);
   }
+  if (TMA && p.any) gn_last_copies(mail);
   if (ctas > 1) cluster.sync();  // no CTA leaves while another may still send to it
 }
 
@@ -734,7 +754,7 @@ __global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads :
   float mu_next[NG], rs_next[NG];
   const auto fetch = [&](const GnUnit& w, const GnShape& q, uint32_t after) {
     if constexpr (TMA) {
-      if (tid == 0 && q.any) {
+      if (tid == 0 && q.any && !mail.abort) {
         ptx::mbar_arrive_expect_tx(bar, 2 * box_bytes);
         gn_fetch_box(slots, &map_x, t, w, q, bar);
         gn_fetch_box(slots_g, &map_g, t, w, q, bar);
@@ -890,6 +910,7 @@ __global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads :
     u = next;
     if (gn_groups(t, u) != p.groups) p = gn_shape<T, VEC>(t, gn_groups(t, u), rank);
   }
+  if (TMA && p.any) gn_last_copies(mail);
   if (ctas > 1) cluster.sync();
 }
 
