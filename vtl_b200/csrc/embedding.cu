@@ -338,7 +338,7 @@ __device__ __forceinline__ void zero_absent(const EmbGrad& p, size_t row0, size_
   }
 }
 
-constexpr int kTileMax = 64, kCtaPositions = 2048;  // positions per tile and per CTA
+constexpr int kTileMax = 64, kCtaPositions = 1024;  // positions per tile and per CTA
 template <bool VEC, bool DROP>
 __global__ void __launch_bounds__(256, 3) embedding_sums_kernel(EmbGrad p, vtlb_mask m, unsigned zero_ctas) {
   __shared__ int2 window[kCtaPositions + 2 * kTileMax + 2];  // the sorted positions of this CTA's tiles and a tile around them
@@ -550,7 +550,7 @@ int embedding_bwd_batch(vtlb_ctx* ctx, vtlb_workspace& ws, const float* g, const
   const int threads = vec ? (p.slab * p.per_cta + 31) / 32 * 32 : p.slab * p.per_cta * 32;
   // Tiles of 4 to 64 positions: long enough that few runs are cut, short enough for eight to sixteen CTAs per SM.
   p.tile = 4;
-  while (p.tile < kTileMax && p.tile * p.per_cta < kCtaPositions && (long long)n * p.slabs > (long long)p.tile * p.per_cta * 16 * ctx->sm_count) p.tile *= 2;
+  while (p.tile < kTileMax && p.tile * 2 * p.per_cta <= kCtaPositions && (long long)n * p.slabs > (long long)p.tile * p.per_cta * 16 * ctx->sm_count) p.tile *= 2;
   p.tiles = (n + p.tile - 1) / p.tile;
   const size_t list = vtlb_round_up((size_t)n * sizeof(int2), 256);
   void* scr = nullptr;
