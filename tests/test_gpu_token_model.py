@@ -202,6 +202,16 @@ def test_builder_refusals(sess):
         m.groupnorm(2, eps=-1.0)
     with pytest.raises(VtlbError, match="positive"):
         m.embedding(0, 8)
+    m.groupnorm(2)
+    d = sess.dev.zeros(64)
+    with pytest.raises(VtlbError, match="batch"):
+        m.forward(d, (0, 3, 4, 4), d)
+    with pytest.raises(VtlbError, match="channels"):
+        m.forward(d, (1, 3, 4, 5), d)
+    d.free()
+    m.close()
+    m = host.Model(sess)
+    m.input([3, 4, 4])
     m.conv2d(3, 4, (3, 3), padding=(1, 1))
     with pytest.raises(VtlbError, match="convolutions"):
         m.groupnorm(2)

@@ -149,7 +149,7 @@ VarPtr GroupNormLayer::forward(const VarPtr& input) {
   Context* ctx = input->context;
   Session* s = ctx->device_session;
   const auto& xs = input->value.shape();
-  if (xs.size() < 2 || xs.back() != channels)
+  if (xs.size() < 2 || xs[0] <= 0 || xs.back() != channels)
     throw Error(VTLB_EINVAL, "GroupNormLayer.forward: input must be [batch, ..., channels]");
   const int B = xs[0], S = (int)(input->value.size() / B / channels);
   Tensor y = Tensor::empty(s, xs), mean = Tensor::empty(s, {B, groups}), rstd = Tensor::empty(s, {B, groups});
