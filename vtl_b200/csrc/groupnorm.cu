@@ -172,14 +172,30 @@ __device__ __forceinline__ float inv_sqrt(double v) {
 }
 
 // ---------------------------------------------------------------- groups of any size
-// Two passes over x (and g): sums per channel and chunk of kRows positions, then the result.  CTAs take 256 threads as
-// `cols` pieces of VEC channels by 256 / cols rows.
-constexpr int kRows = 256;
+// Two passes over x (and g): sums per channel and chunk of positions, then the result.  CTAs take 256 threads as
+// `cols` pieces of VEC channels by 256 / cols rows.  Sums are f64: sum and sum of squares forward, dz and dz * h backward.
+// Bound by HBM, 12 bytes per element forward, 20 backward, less what of x and g still lies in L2 for the second pass.
+// Ten samples of 20000 positions by one group of 64 channels: 35 us forward, 64 us backward, 4.4 and 4 TB/s of those bytes.
+// Sixty of 4000 by two groups of 31 (rows on no 16-byte boundary, one channel a load): 48 and 86 us, 3.7 and 3.5 TB/s.
+constexpr int kRows = 256;  // positions per chunk, fewer where there would be too few CTAs
 
 struct GnGrid {
   GnDims d;
   int shift;  // log2 of the pieces per CTA
+  int rows;   // positions per chunk
 };
+
+// Rows that a thread asks for before it uses the first one.  (The result may lie where x or g does, so the compiler would
+// not move a load in front of a store: 2.4 TB/s.)
+template <int VEC>
+constexpr int gn_ahead = VEC == 4 ? 4 : 8;
+template <int VEC>
+__device__ __forceinline__ void gn_rows(GnVec<VEC> (&v)[gn_ahead<VEC>], const float* from, int r, int r1, int lanes, int C) {
+#pragma unroll
+  for (int i = 0; i < gn_ahead<VEC>; ++i) {
+    if (r + i * lanes < r1) v[i] = gn_load<VEC>(from + (size_t)(r + i * lanes) * C);
+  }
+}
 
 template <int ACT, bool BWD, int VEC>
 __global__ void __launch_bounds__(256) gn_sums_kernel(const float* x, const float* g, const float* gamma,
@@ -191,7 +207,7 @@ __global__ void __launch_bounds__(256) gn_sums_kernel(const float* x, const floa
   const GnDims d = t.d;
   const int cols = 1 << t.shift, lanes = 256 >> t.shift, col = threadIdx.x & (cols - 1), lane = threadIdx.x >> t.shift;
   const int c = (blockIdx.x * cols + col) * VEC, chunk = blockIdx.y, b = blockIdx.z;
-  const int r1 = min(d.S, (chunk + 1) * kRows);
+  const int r1 = min(d.S, (chunk + 1) * t.rows);
   double2 acc[VEC] = {};
   if (c < d.C) {
     GnVec<VEC> mu = {}, rs = {}, ga = {}, be = {};
@@ -205,22 +221,28 @@ __global__ void __launch_bounds__(256) gn_sums_kernel(const float* x, const floa
     }
     const GnVec<VEC> minus = vneg(mu);
     const size_t base = (size_t)b * d.S * d.C + c;
-#pragma unroll 4
-    for (int r = chunk * kRows + lane; r < r1; r += lanes) {
-      const GnVec<VEC> v = gn_load<VEC>(x + base + (size_t)r * d.C);
-      if (BWD) {
-        const GnVec<VEC> h = vmul(vadd(v, minus), rs);
-        const GnVec<VEC> dz = act_bwd<ACT>(gn_load<VEC>(g + base + (size_t)r * d.C), v, mu, rs, ga, be, h);
+    for (int r = chunk * t.rows + lane; r < r1; r += gn_ahead<VEC> * lanes) {
+      GnVec<VEC> vx[gn_ahead<VEC>], vg[gn_ahead<VEC>];
+      gn_rows<VEC>(vx, x + base, r, r1, lanes, d.C);
+      if (BWD) gn_rows<VEC>(vg, g + base, r, r1, lanes, d.C);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          acc[k].x += (double)dz.e[k];
-          acc[k].y = fma((double)dz.e[k], (double)h.e[k], acc[k].y);
-        }
-      } else {
+      for (int i = 0; i < gn_ahead<VEC>; ++i) {
+        if (r + i * lanes >= r1) break;
+        const GnVec<VEC> v = vx[i];
+        if (BWD) {
+          const GnVec<VEC> h = vmul(vadd(v, minus), rs);
+          const GnVec<VEC> dz = act_bwd<ACT>(vg[i], v, mu, rs, ga, be, h);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          acc[k].x += (double)v.e[k];
-          acc[k].y = fma((double)v.e[k], (double)v.e[k], acc[k].y);
+          for (int k = 0; k < VEC; ++k) {
+            acc[k].x += (double)dz.e[k];
+            acc[k].y = fma((double)dz.e[k], (double)h.e[k], acc[k].y);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            acc[k].x += (double)v.e[k];
+            acc[k].y = fma((double)v.e[k], (double)v.e[k], acc[k].y);
+          }
         }
       }
     }
@@ -237,25 +259,38 @@ __global__ void __launch_bounds__(256) gn_sums_kernel(const float* x, const floa
   }
 }
 
-// One warp per (sample, group): the sums over chunks and channels, in a fixed order.
+// One CTA per (sample, group), T threads: the sums over chunks and channels, in a fixed order.  (With a warp for each, which
+// also divided to find its channels, 79 chunks of 64 channels took 40 us, longer than both passes over x.)
 template <bool BWD>
 __global__ void __launch_bounds__(256) gn_groups_kernel(const double2* partial, int chunks, GnDims d, const float* gamma,
                                                         double eps, float* mean, float* rstd, float2* coef) {
+  __shared__ double2 sm[8];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const size_t k = (blockIdx.x * (size_t)blockDim.x + threadIdx.x) >> 5;
-  if (k >= (size_t)d.B * d.G) return;
+  const unsigned k = blockIdx.x, T = blockDim.x;
   const int b = (int)(k / d.G), grp = (int)(k % d.G);
+  const int down = T / d.width, along = T % d.width;  // from one entry of a thread to its next
+  int row = threadIdx.x / d.width, col = threadIdx.x % d.width;
   double s0 = 0.0, s1 = 0.0;
-  for (int i = lane; i < chunks * d.width; i += 32) {
-    const int c = grp * d.width + i % d.width;
-    const double2 p = partial[((size_t)b * chunks + i / d.width) * d.C + c];
-    const double w = BWD && gamma ? (double)gamma[c] : 1.0;
-    s0 += w * p.x, s1 += w * p.y;
+  while (row < chunks) {
+    double2 p[8];
+    double w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = grp * d.width + col;
+      p[i] = row < chunks ? partial[((size_t)b * chunks + row) * d.C + c] : make_double2(0.0, 0.0);
+      w[i] = row >= chunks ? 0.0 : BWD && gamma ? (double)gamma[c] : 1.0;
+      row += down, col += along;
+      if (col >= d.width) col -= d.width, ++row;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s0 = fma(w[i], p[i].x, s0), s1 = fma(w[i], p[i].y, s1);
   }
   for (int o = 16; o; o >>= 1) s0 += __shfl_xor_sync(~0u, s0, o), s1 += __shfl_xor_sync(~0u, s1, o);
-  if (lane) return;
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = make_double2(s0, s1);
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (unsigned q = 1; q < T / 32; ++q) s0 += sm[q].x, s1 += sm[q].y;
   const double n = (double)d.S * d.width;
   if (BWD) {
     coef[k] = make_float2((float)(s0 / n), (float)(s1 / n));
@@ -301,7 +336,7 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const float* x, const flo
   const GnDims d = t.d;
   const int cols = 1 << t.shift, lanes = 256 >> t.shift, col = threadIdx.x & (cols - 1), lane = threadIdx.x >> t.shift;
   const int c = (blockIdx.x * cols + col) * VEC, chunk = blockIdx.y, b = blockIdx.z;
-  const int r1 = min(d.S, (chunk + 1) * kRows);
+  const int r1 = min(d.S, (chunk + 1) * t.rows);
   if (c >= d.C) return;
   GnVec<VEC> mu, rs, ga, be, c1 = {}, c2 = {};
 #pragma unroll
@@ -313,15 +348,21 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const float* x, const flo
   }
   const GnVec<VEC> minus = vneg(mu), a = vmul(ga, rs);
   const size_t base = (size_t)b * d.S * d.C + c;
-#pragma unroll 4
-  for (int r = chunk * kRows + lane; r < r1; r += lanes) {
-    const size_t i = base + (size_t)r * d.C;
-    const GnVec<VEC> v = gn_load<VEC>(x + i), dist = vadd(v, minus);
-    if (BWD) {
-      const GnVec<VEC> h = vmul(dist, rs);
-      gn_store<VEC>(out + i, vfma(a, act_bwd<ACT>(gn_load<VEC>(g + i), v, mu, rs, ga, be, h), vfma(h, c2, c1)));
-    } else {
-      gn_store<VEC>(out + i, act<ACT>(vfma(dist, a, be)));
+  for (int r = chunk * t.rows + lane; r < r1; r += gn_ahead<VEC> * lanes) {
+    GnVec<VEC> vx[gn_ahead<VEC>], vg[gn_ahead<VEC>];
+    gn_rows<VEC>(vx, x + base, r, r1, lanes, d.C);
+    if (BWD) gn_rows<VEC>(vg, g + base, r, r1, lanes, d.C);
+#pragma unroll
+    for (int i = 0; i < gn_ahead<VEC>; ++i) {
+      if (r + i * lanes >= r1) break;
+      const GnVec<VEC> dist = vadd(vx[i], minus);
+      float* to = out + base + (size_t)(r + i * lanes) * d.C;
+      if (BWD) {
+        const GnVec<VEC> h = vmul(dist, rs);
+        gn_store<VEC>(to, vfma(a, act_bwd<ACT>(vg[i], vx[i], mu, rs, ga, be, h), vfma(h, c2, c1)));
+      } else {
+        gn_store<VEC>(to, act<ACT>(vfma(dist, a, be)));
+      }
     }
   }
 }
@@ -992,17 +1033,22 @@ int check_dims(vtlb_ctx* ctx, const char* fn, int B, int S, int C, int groups, i
   return VTLB_OK;
 }
 
-GnGrid grid_of(const GnDims& d, int vec) {
-  GnGrid t{d, 0};
+GnGrid grid_of(const GnDims& d, int vec, int sm_count) {
+  GnGrid t{d, 0, kRows};
   while (t.shift < 8 && (1 << t.shift) * vec < d.C && ((1 << t.shift) < 32 || d.S * (1 << t.shift) < kRows * 8)) ++t.shift;
-  return t;  // 32 pieces wide as a rule, wider where there are few rows
+  // 32 pieces wide as a rule, wider where there are few rows; four rows a thread at least.
+  const long long across = (long long)d.B * ((d.C + (vec << t.shift) - 1) / (vec << t.shift));
+  while (t.rows > 4 * (256 >> t.shift) && t.rows > 32 && across * ((d.S + t.rows - 1) / t.rows) < 2LL * sm_count) t.rows /= 2;
+  return t;
 }
+
+int group_threads(const GnDims& d, int chunks) { return (long long)chunks * d.width > 256 ? 256 : 32; }
 
 template <int ACT, int VEC>
 int gn_forward_general(vtlb_ctx* ctx, const float* x, GnDims d, const float* gamma, const float* beta, double eps, float* y,
                        float* mean, float* rstd) {
-  const int chunks = (d.S + kRows - 1) / kRows;
-  const GnGrid t = grid_of(d, VEC);
+  const GnGrid t = grid_of(d, VEC, ctx->sm_count);
+  const int chunks = (d.S + t.rows - 1) / t.rows;
   const dim3 grid((d.C + (VEC << t.shift) - 1) / (VEC << t.shift), chunks, d.B);
   vtlb_workspace ws(ctx);
   void* partial = nullptr;
@@ -1011,7 +1057,7 @@ int gn_forward_general(vtlb_ctx* ctx, const float* x, GnDims d, const float* gam
   VTLB_CUDA(ctx, vtlb_launch_early(gn_sums_kernel<ACT, false, VEC>, grid, dim3(256), 0, ctx->stream, x, none, none, none, none,
                                    none, t, (double2*)partial));
   VTLB_LAUNCHED(ctx);
-  VTLB_CUDA(ctx, vtlb_launch_early(gn_groups_kernel<false>, dim3((unsigned)(((size_t)d.B * d.G + 7) / 8)), dim3(256), 0,
+  VTLB_CUDA(ctx, vtlb_launch_early(gn_groups_kernel<false>, dim3((unsigned)d.B * d.G), dim3(group_threads(d, chunks)), 0,
                                    ctx->stream, (const double2*)partial, chunks, d, none, eps, mean, rstd, (float2*)nullptr));
   VTLB_LAUNCHED(ctx);
   VTLB_CUDA(ctx, vtlb_launch_early(gn_apply_kernel<ACT, false, VEC>, grid, dim3(256), 0, ctx->stream, x, none, gamma, beta,
@@ -1023,8 +1069,8 @@ int gn_forward_general(vtlb_ctx* ctx, const float* x, GnDims d, const float* gam
 template <int ACT, int VEC>
 int gn_backward_general(vtlb_ctx* ctx, const float* g, const float* x, GnDims d, const float* gamma, const float* beta,
                         const float* mean, const float* rstd, float* dx, float* dgamma, float* dbeta) {
-  const int chunks = (d.S + kRows - 1) / kRows;
-  const GnGrid t = grid_of(d, VEC);
+  const GnGrid t = grid_of(d, VEC, ctx->sm_count);
+  const int chunks = (d.S + t.rows - 1) / t.rows;
   const dim3 grid((d.C + (VEC << t.shift) - 1) / (VEC << t.shift), chunks, d.B);
   const size_t sums = (size_t)d.B * chunks * d.C * sizeof(double2);
   vtlb_workspace ws(ctx);
@@ -1041,7 +1087,7 @@ int gn_backward_general(vtlb_ctx* ctx, const float* g, const float* x, GnDims d,
     VTLB_LAUNCHED(ctx);
   }
   if (!dx) return VTLB_OK;
-  VTLB_CUDA(ctx, vtlb_launch_early(gn_groups_kernel<true>, dim3((unsigned)(((size_t)d.B * d.G + 7) / 8)), dim3(256), 0,
+  VTLB_CUDA(ctx, vtlb_launch_early(gn_groups_kernel<true>, dim3((unsigned)d.B * d.G), dim3(group_threads(d, chunks)), 0,
                                    ctx->stream, (const double2*)partial, chunks, d, gamma, 0.0, (float*)nullptr,
                                    (float*)nullptr, coef));
   VTLB_LAUNCHED(ctx);

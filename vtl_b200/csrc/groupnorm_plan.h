@@ -50,8 +50,10 @@ inline GnPlan gn_plan_slab(int B, int S, int C, int G, int vec, int groups, int 
   while (p.rsplit < max_r && !fits(1, p.rsplit) && (long long)B * p.slabs * p.csplit * p.rsplit * 2 <= sm_count) p.rsplit *= 2;
   p.rows = (S + p.rsplit - 1) / p.rsplit;
   p.vpt = p.rows <= lanes ? 1 : p.rows <= lanes * middle ? middle : most;
-  // TMA boxes are at most 256 by 256; rows of less than 64 bytes are not worth one.
-  p.tma = vec == 4 && p.channels >= 16 && p.channels <= 256;
+  // TMA boxes are at most 256 by 256; rows of less than 64 bytes are not worth one.  Nor is a map, half a microsecond of the
+  // host's time, for a few pieces of one step (8 x 8 positions of 128 channels: 7.1 us a call with one, 6.6 us without).
+  const bool few = p.vpt == 1 && (long long)B * p.slabs * p.csplit * p.rsplit <= 2LL * sm_count;
+  p.tma = vec == 4 && p.channels >= 16 && p.channels <= 256 && !few;
   p.boxes = (p.rows + 255) / 256;
   p.box_rows = ((p.rows + p.boxes - 1) / p.boxes + 7) / 8 * 8;
   p.on_chip = true;
