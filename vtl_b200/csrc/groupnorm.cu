@@ -963,10 +963,11 @@ struct GnKernelInfo {
   std::atomic<bool> allowed[kDevices];
 };
 
-// Launches as many clusters as the GPU holds at a time (each goes on to further units), at most one per unit.
+// Launches as many clusters as the GPU holds at a time (each goes on to further units), at most one per unit.  `usual` is
+// the shared memory that threads full of rows take, for which the clusters are counted whatever this call's rows.
 template <typename... KArgs, typename... Args>
 cudaError_t cluster_launch(vtlb_ctx* ctx, GnKernelInfo& info, void (*kern)(KArgs...), int threads, unsigned units,
-                           int cluster, size_t smem, Args&&... args) {
+                           int cluster, size_t smem, size_t usual, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cluster);
   cfg.blockDim = dim3(threads);
@@ -990,9 +991,11 @@ cudaError_t cluster_launch(vtlb_ctx* ctx, GnKernelInfo& info, void (*kern)(KArgs
     int fit = info.resident[cluster].load(std::memory_order_relaxed);
     if (!fit) {
       if (cluster > 1) {
+        cfg.dynamicSmemBytes = usual;
         e = cudaOccupancyMaxActiveClusters(&fit, kern, &cfg);
+        cfg.dynamicSmemBytes = smem;
       } else {
-        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, threads, smem);
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, threads, usual);
         fit *= ctx->sm_count;
       }
       if (e != cudaSuccess) return e;
@@ -1009,14 +1012,14 @@ cudaError_t cluster_launch(vtlb_ctx* ctx, GnKernelInfo& info, void (*kern)(KArgs
 template <int ACT, int VEC, int VPT, bool GROUPED, bool TMA, typename... Args>
 cudaError_t fwd_tile(vtlb_ctx* ctx, const GnTile& t, int cluster, Args... args) {
   static GnKernelInfo info;
-  const size_t smem = TMA ? (size_t)t.boxes * t.box_rows * t.channels * 4 : (size_t)kGnFwdThreads * VPT * VEC * 4;
-  return cluster_launch(ctx, info, gn_fwd_tile_kernel<ACT, VEC, VPT, GROUPED, TMA>, kGnFwdThreads, t.units, cluster, smem, args...);
+  const size_t usual = (size_t)kGnFwdThreads * VPT * VEC * 4, smem = TMA ? (size_t)t.boxes * t.box_rows * t.channels * 4 : usual;
+  return cluster_launch(ctx, info, gn_fwd_tile_kernel<ACT, VEC, VPT, GROUPED, TMA>, kGnFwdThreads, t.units, cluster, smem, usual, args...);
 }
 template <int ACT, int VEC, int VPT, bool GROUPED, bool TMA, typename... Args>
 cudaError_t bwd_tile(vtlb_ctx* ctx, const GnTile& t, int cluster, Args... args) {
   static GnKernelInfo info;
-  const size_t smem = TMA ? (size_t)t.boxes * t.box_rows * t.channels * 8 : (size_t)kGnBwdThreads * VPT * VEC * 8;
-  return cluster_launch(ctx, info, gn_bwd_tile_kernel<ACT, VEC, VPT, GROUPED, TMA>, kGnBwdThreads, t.units, cluster, smem, args...);
+  const size_t usual = (size_t)kGnBwdThreads * VPT * VEC * 8, smem = TMA ? (size_t)t.boxes * t.box_rows * t.channels * 8 : usual;
+  return cluster_launch(ctx, info, gn_bwd_tile_kernel<ACT, VEC, VPT, GROUPED, TMA>, kGnBwdThreads, t.units, cluster, smem, usual, args...);
 }
 
 GnTile tile_of(const GnDims& d, const GnPlan& p) { return GnTile{d, p.groups, p.slabs, p.csplit, p.channels, p.rows, (unsigned)d.B * (unsigned)p.slabs, 0u,
