@@ -28,7 +28,7 @@ def tokens(rng, n, V, how):
     return ids
 
 
-SHAPES = [(1, 1, 1), (1, 8, 5), (3, 4, 2), (8, 256, 100), (33, 7, 3), (257, 130, 1000), (999, 2047, 61), (1024, 64, 17),
+SHAPES = [(1, 1, 1), (1, 8, 5), (3, 4, 2), (8, 256, 100), (33, 7, 3), (257, 130, 1000), (512, 96, 40), (513, 97, 40), (600, 640, 7), (999, 2047, 61), (1024, 64, 17),
           (4097, 12, 5000), (8192, 20, 70000), (20011, 5, 300)]
 HOW = ["uniform", "skewed", "one", "distinct", "padded"]
 
@@ -93,8 +93,9 @@ def test_gradient_of_one_position_is_one_product(dev):
         b.free()
 
 
-def test_infinities_and_nan_stay_in_their_rows(dev):
-    n, D, V = 40, 9, 6
+@pytest.mark.parametrize("n", [40, 700])
+def test_infinities_and_nan_stay_in_their_rows(dev, n):
+    D, V = 9, 6
     rng = np.random.default_rng(9)
     ids = rng.integers(0, V, n).astype(np.int32)
     ids[5], ids[6], ids[7] = 1, 2, -1
@@ -116,9 +117,10 @@ def test_infinities_and_nan_stay_in_their_rows(dev):
 
 @pytest.mark.parametrize("off", [1, 2, 3])
 @pytest.mark.parametrize("D", [64, 21])
-def test_pointers_off_the_16_byte_grid(dev, off, D):
+@pytest.mark.parametrize("n", [130, 900])
+def test_pointers_off_the_16_byte_grid(dev, off, D, n):
     rng = np.random.default_rng(off)
-    n, V = 130, 40
+    V = 40
     W, g, ids = rng.standard_normal(V * D + 4).astype(np.float32), rng.standard_normal(n * D + 4).astype(np.float32), \
         rng.integers(-1, V, n + 4).astype(np.int32)
     dW_, dg, dids = dev.to_device(W), dev.to_device(g), dev.to_device(ids)

@@ -69,7 +69,8 @@ __global__ void __launch_bounds__(256) embedding_fwd_kernel(const float* __restr
 
 // ---------------------------------------------------------------- gradient
 // The positions are sorted by token (stable: those of a token stay in order), then read in that order, so that a sum is
-// a run of consecutive rows and no two threads add to one place: no atomics, the same bits every time.  Three launches:
+// a run of consecutive rows and no two threads add to one place: no atomics, the same bits every time.  Three launches, or
+// one where there are few positions (embedding_few_kernel):
 //   sort   pairs (token, position); tokens outside [0, V) take the key V and end up behind all others
 //   sums   the sorted positions in tiles of equal length whatever the tokens are.  A run that ends within a tile's
 //          length of the tile it starts in is summed there as a whole; a longer one leaves a partial row per tile.
@@ -338,6 +339,115 @@ __device__ __forceinline__ void zero_absent(const EmbGrad& p, size_t row0, size_
   }
 }
 
+// Few positions in one launch, without a sort: a warp finds the positions of the token of position j by comparing with all,
+// and where j is the first of them it sums 128 columns of their rows (eight rows at a time, in order).  More than kFewAlone
+// rows are summed by all warps of the CTA, an eighth each.  Rows of absent tokens are zeroed by further CTAs.  Bound by
+// latency: the host's launch, the ids, a row of g.
+// 256 positions x 600, 5000 tokens: 5.1 us, 10.4 by way of the sort; 1024 x 600: 9.0 and 13.0; 512 x 4096: 23.0 and 27.8;
+// 2048 x 512: 30.0 and 27.1, all of them one token 18.6 and 28.1; 2048 x 1023: 36 and 22 (each CTA compares the positions
+// for itself, so many CTAs do so many times).  With a mask, whose blocks leave room for four rows at a time, half as many:
+// 2048 x 255: 16.8 and 18.2; 1024 x 1023: 21.1 and 17.9.
+constexpr int kFewAlways = 512, kFewMax = 2048, kFewElements = 1 << 20, kFewAlone = 16;
+template <bool VEC, bool DROP>
+__global__ void __launch_bounds__(256, 4) embedding_few_kernel(EmbGrad p, vtlb_mask m, unsigned zero_ctas) {
+  __shared__ int ids[kFewMax];
+  __shared__ uint16_t list[8][kFewMax];  // the positions of each warp's token
+  __shared__ int count[8];
+  __shared__ float4 part[8][32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (blockIdx.x < zero_ctas) {
+    const size_t each = ((size_t)p.V + zero_ctas - 1) / zero_ctas, row0 = blockIdx.x * each;
+    zero_absent(p, row0, row0 + each < (size_t)p.V ? row0 + each : (size_t)p.V);
+    return;
+  }
+  const unsigned cta = blockIdx.x - zero_ctas;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, words = (p.n + 31) / 32;
+  // (positions far from one another: tokens met often have their first positions together, at the start)
+  const int apart = (p.n + 7) / 8, j0 = (int)(cta / p.slabs), j = j0 + warp * apart;
+  const size_t total = (size_t)p.n * p.D;
+  const bool aligned = ((uintptr_t)p.g & 15) == 0;
+  for (int i = threadIdx.x; i < words * 32; i += 256) {
+    const int id = i < p.n ? __ldg(p.ids + i) : -1;
+    ids[i] = id < p.V ? id : -1;
+  }
+  __syncthreads();
+  const int id = j < p.n ? ids[j] : -1;
+  if (id >= 0) {
+    bool first = true;
+    for (int i = lane; i < (j & ~31); i += 32) first = first && ids[i] != id;
+    first = __all_sync(0xffffffffu, first && ((j & ~31) + lane >= j || ids[(j & ~31) + lane] != id));
+    int found = 0;
+    if (first)
+      for (int i = j / 32; i < words; ++i) {
+        const bool hit = ids[i * 32 + lane] == id;
+        const uint32_t hits = __ballot_sync(0xffffffffu, hit);
+        if (hit) list[warp][found + __popc(hits & ((1u << lane) - 1u))] = (uint16_t)(i * 32 + lane);
+        found += __popc(hits);
+      }
+    if (lane == 0) count[warp] = found;
+  } else if (lane == 0) {
+    count[warp] = 0;
+  }
+  __syncwarp();
+  const auto sum = [&](const uint16_t* rows, int k0, int k1, int c, bool own) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int U = DROP ? 4 : 8;
+    for (int k = k0; k < k1; k += U) {
+      float4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k + u < k1) {
+          const size_t row = (size_t)rows[k + u] * p.D;
+          if (VEC) {
+            if (own) v[u] = __ldg(reinterpret_cast<const float4*>(p.g + row) + c);
+          } else if (4 * c - (int)(row & 3) < p.D) {
+            v[u] = block_load(p.g, (row & ~(size_t)3) + 4 * (size_t)c, total, aligned);
+          }
+        }
+      }
+      if (DROP || !VEC) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const size_t e = (p.first_pos + rows[min(k + u, k1 - 1)]) * (size_t)p.D;
+          if (DROP) v[u] = vtlb_drop4(m, e / 4 + c, v[u]);
+          if (!VEC) v[u] = shift_down(v[u], (int)(e & 3));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (k + u < k1) add4(acc, v[u]);
+    }
+    return acc;
+  };
+  constexpr int kWide = VEC ? 32 : 31;
+  const int c0 = (int)(cta % p.slabs) * p.slab * kWide, c1 = min(p.cols, c0 + p.slab * kWide);
+  const int rows = count[warp];
+  if (rows && rows <= kFewAlone)
+    for (int c = c0 + lane; c - lane < c1; c += kWide) {
+      const bool own = c < p.cols && lane < kWide;
+      const float4 acc = sum(list[warp], 0, rows, c, own);
+      if (own) row_store<VEC>(p.dW + (size_t)id * p.D, c, p.D, mul4(acc, p.scale), p.accumulate);
+    }
+  __syncthreads();
+  for (int w = 0; w < 8; ++w) {
+    const int all = count[w], share = (all + 7) / 8;
+    if (all <= kFewAlone) continue;
+    for (int c = c0 + lane; c - lane < c1; c += kWide) {
+      const bool own = c < p.cols && lane < kWide;
+      part[warp][lane] = sum(list[w], warp * share, min(all, (warp + 1) * share), c, own);
+      __syncthreads();
+      if (warp == 0 && own) {
+        float4 acc = part[0][lane];
+        for (int q = 1; q * share < all; ++q) add4(acc, part[q][lane]);
+        row_store<VEC>(p.dW + (size_t)ids[j0 + w * apart] * p.D, c, p.D, mul4(acc, p.scale), p.accumulate);
+      }
+      __syncthreads();
+    }
+  }
+}
+
 constexpr int kTileMax = 64, kCtaPositions = 1024;  // positions per tile and per CTA
 template <bool VEC, bool DROP>
 __global__ void __launch_bounds__(256, 3) embedding_sums_kernel(EmbGrad p, vtlb_mask m, unsigned zero_ctas) {
@@ -543,6 +653,25 @@ int embedding_bwd_batch(vtlb_ctx* ctx, vtlb_workspace& ws, const float* g, const
   p.g = g, p.ids = ids, p.dW = dW, p.first_pos = first_pos, p.n = n, p.V = V, p.D = D, p.scale = scale, p.accumulate = accumulate;
   p.cols = (D + 3) / 4;
   const bool vec = D % 4 == 0 && vtlb_aligned16(g) && vtlb_aligned16(dW);
+  // Each zeroing CTA reads all ids, so they are no more than write four times what all of them read, but two per SM
+  // where there are 32 KB to write for each.
+  const size_t table = (size_t)V * D * 4;
+  size_t want = table / ((size_t)n * 16), least = (size_t)2 * ctx->sm_count;
+  want = want < least ? least : want;
+  if (want > table / 32768 + 1) want = table / 32768 + 1;
+  const unsigned zero_ctas = accumulate ? 0u : (unsigned)(want < (size_t)V ? want : (size_t)V);
+  if (n <= kFewAlways >> m.any || (n <= kFewMax && (long long)n * D <= kFewElements >> m.any)) {
+    // Pieces of 128 columns to a CTA: as many as leave eight CTAs per SM, for each finds its positions for itself.
+    const int pieces = vec ? (p.cols + 31) / 32 : (p.cols + 30) / 31;
+    p.slab = 1;
+    while (p.slab < pieces && (long long)((n + 7) / 8) * pieces > (long long)p.slab * 8 * ctx->sm_count) p.slab *= 2;
+    p.slabs = (pieces + p.slab - 1) / p.slab;
+    auto few = vec ? (m.any ? embedding_few_kernel<true, true> : embedding_few_kernel<true, false>)
+                   : (m.any ? embedding_few_kernel<false, true> : embedding_few_kernel<false, false>);
+    VTLB_CUDA(ctx, vtlb_launch_early(few, dim3((unsigned)((n + 7) / 8) * p.slabs + zero_ctas), dim3(256), 0, ctx->stream, p, m, zero_ctas));
+    VTLB_LAUNCHED(ctx);
+    return VTLB_OK;
+  }
   const int units = vec ? p.cols : (p.cols + 30) / 31, most = vec ? 256 : 8;  // threads, or warps, per row and per CTA
   p.slabs = (units + most - 1) / most;
   p.slab = (units + p.slabs - 1) / p.slabs;
@@ -563,13 +692,6 @@ int embedding_bwd_batch(vtlb_ctx* ctx, vtlb_workspace& ws, const float* g, const
   VTLB_LAUNCHED(ctx);
 
   const unsigned sum_ctas = (unsigned)((p.tiles + p.per_cta - 1) / p.per_cta) * p.slabs;
-  // Each zeroing CTA reads all ids, so they are no more than write four times what all of them read, but two per SM
-  // where there are 32 KB to write for each.
-  const size_t table = (size_t)V * D * 4;
-  size_t want = table / ((size_t)n * 16), least = (size_t)2 * ctx->sm_count;
-  want = want < least ? least : want;
-  if (want > table / 32768 + 1) want = table / 32768 + 1;
-  const unsigned zero_ctas = accumulate ? 0u : (unsigned)(want < (size_t)V ? want : (size_t)V);
   auto sums = vec ? (m.any ? embedding_sums_kernel<true, true> : embedding_sums_kernel<true, false>)
                   : (m.any ? embedding_sums_kernel<false, true> : embedding_sums_kernel<false, false>);
   VTLB_CUDA(ctx, vtlb_launch_early(sums, dim3(sum_ctas + zero_ctas), dim3(threads), 0, ctx->stream, p, m, zero_ctas));
