@@ -75,6 +75,7 @@ inline GnPlan gn_plan(int B, int S, int C, int G, bool aligned, int threads, int
     const int cols = p.channels / vec, channels = k * width;
     const double score = (p.on_chip ? 4.0 : 0.0) + (channels >= 32 || k == G ? 2.0 : channels / 32.0) + (double)cols / gn_pow2(cols);
     if (score > best_score + 1e-9) best = p, best_score = score;
+    if (score >= 7.0) break;  // there is no better one
   }
   return best;
 }
