@@ -412,7 +412,8 @@ int vtlb_batchnorm1d_bwd_f32(vtlb_ctx* ctx, const void* d_g, const void* d_x, in
  * whatever x_i holds; r_i is word i % 4 of the Philox4x32-10 block with key `seed` and counter (i / 4, step), each 64
  * bits, low words first.  The mask is a function of (seed, step, i) alone and is not stored: the backward pass is given
  * the seed and step of the forward pass and draws it again.  Every pass wants a step of its own, a captured call
- * included: a replay repeats the mask it was captured with.  0 <= p <= 1; d_y may be d_x (not overlap it in part). */
+ * included: a replay repeats the mask it was captured with.  0 <= p <= 1; n <= 2^41; d_y may be d_x (not overlap it in
+ * part). */
 int vtlb_dropout_fwd_f32(vtlb_ctx* ctx, const void* d_x, void* d_y, size_t n, double p, uint64_t seed, uint64_t step);
 int vtlb_dropout_bwd_f32(vtlb_ctx* ctx, const void* d_g, void* d_dx, size_t n, double p, uint64_t seed, uint64_t step);
 /* Embedding: Y[j, :] = scale * W[ids[j], :] for j < n, W[V, D].  An id outside [0, V) (padding, by convention -1) is
@@ -427,7 +428,8 @@ int vtlb_embedding_fwd_f32(vtlb_ctx* ctx, const void* d_W, int V, int D, const v
                            double p, uint64_t seed, uint64_t step, void* d_Y, int check);
 int vtlb_embedding_bwd_f32(vtlb_ctx* ctx, const void* d_G, const void* d_ids_i32, size_t n, int V, int D, float scale,
                            double p, uint64_t seed, uint64_t step, void* d_dW, int accumulate);
-/* ids[i] = src[i] where that is a whole number in [0, 2^31), else -1: tokens that arrive in an f32 tensor. */
+/* ids[i] = src[i] where that is a whole number in [0, 2^31), else -1: tokens that arrive in an f32 tensor.  d_ids may be
+ * d_src (not overlap it in part). */
 int vtlb_ids_from_f32(vtlb_ctx* ctx, const void* d_src, size_t n, void* d_ids_i32);
 /* Group norm with an activation, channels last: x[B, S, C] (S = positions of a feature map or a sequence, 1 for plain
  * features), the C channels in `groups` equal groups.  Per sample and group: h = (x - mean) * rstd with
@@ -436,7 +438,9 @@ int vtlb_ids_from_f32(vtlb_ctx* ctx, const void* d_src, size_t n, void* d_ids_i3
  * the statistics; the backward pass reads them, and x, and recomputes z.  d_y may be d_x where x is not needed again.
  * Backward, dz = g * act'(z): dgamma[c] = sum dz * h, dbeta[c] = sum dz over samples and positions,
  * dx = rstd * (gamma dz - mean(gamma dz) - h * mean(gamma dz h)), the means over the group; any output may be NULL,
- * d_dx may be d_g or d_x. */
+ * d_dx may be d_g or d_x.  Other buffers may not overlap.  B * S and B * groups go to 2^31 - 1, S to 65535 * 256.  The
+ * backward pass takes up to 8 C (min(S, 8) B) bytes of workspace for the sums of dgamma and dbeta (groups too large for
+ * the chip: 16 C B per 32 to 256 positions). */
 #define VTLB_ACT_NONE 0
 #define VTLB_ACT_RELU 1
 #define VTLB_ACT_SILU 2

@@ -232,4 +232,9 @@ def test_ids_from_f32(dev):
     a, b = dev.to_device(src), dev.zeros(src.size, np.int32)
     dev.ids_from_f32(a, src.size, b)
     assert b.numpy().tolist() == want
+    from vtl_b200.capi import VtlbError
+    with pytest.raises(VtlbError, match="overlap"):
+        dev.ids_from_f32(a, src.size - 1, a.ptr + 4)
+    dev.ids_from_f32(a, src.size, a)  # in place
+    assert a.numpy().view(np.int32).tolist() == want
     a.free(); b.free()

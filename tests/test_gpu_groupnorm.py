@@ -248,6 +248,9 @@ def test_refusals(dev):
             dev.groupnorm_bwd_f32(d, d, B, S, C, G, None, None, d, d, 0, o)
     with pytest.raises(VtlbError, match="unknown activation"):
         dev.groupnorm_fwd_f32(d, 1, 4, 4, 2, None, None, 1e-5, 3, o, o, o)
+    for B, S, C, G in ((1 << 30, 1, 4, 4), (1 << 16, 1 << 15, 1, 1), (1, 65535 * 256 + 1, 4, 1)):
+        with pytest.raises(VtlbError, match="go to"):
+            dev.groupnorm_fwd_f32(d, B, S, C, G, None, None, 1e-5, 0, o, o, o)
     for eps in (-1e-5, float("nan")):
         with pytest.raises(VtlbError, match="eps"):
             dev.groupnorm_fwd_f32(d, 1, 4, 4, 2, None, None, eps, 0, o, o, o)
@@ -261,3 +264,48 @@ def test_refusals(dev):
         dev.groupnorm_bwd_f32(d, o, 1, 4, 4, 2, None, None, o, o, 0, d.ptr + 32)
     assert (d.numpy() == 1).all()
     d.free(); o.free()
+
+
+@pytest.mark.parametrize("B,S,C,G", [(70001, 1, 32, 1), (66000, 2, 6, 3), (70000, 1, 40, 40)])
+def test_many_samples(dev, B, S, C, G):
+    rng = np.random.default_rng(12)
+    x, g = rng.standard_normal((B, S, C)).astype(np.float32), rng.standard_normal((B, S, C)).astype(np.float32)
+    dx_, dg = dev.to_device(x), dev.to_device(g)
+    y, mean, rstd, dx, dgamma, dbeta = (dev.zeros(s) for s in (x.shape, (B, G), (B, G), x.shape, C, C))
+    dev.groupnorm_fwd_f32(dx_, B, S, C, G, None, None, 0.1, ref.SILU, y, mean, rstd)
+    want = ref.groupnorm(x, G, None, None, 0.1, ref.SILU)
+    for out, w, t in zip((y, mean, rstd), want, forward_bounds(x, G, None, None, 0.1, ref.SILU, *want)):
+        assert (np.abs(out.numpy() - w) <= t).all()
+    dev.groupnorm_bwd_f32(dg, dx_, B, S, C, G, None, None, mean, rstd, ref.SILU, dx, dgamma, dbeta)
+    r = ref.groupnorm_bwd(g, x, G, None, None, mean.numpy(), rstd.numpy(), ref.SILU)
+    for out, name, t in zip((dx, dgamma, dbeta), ("dx", "dgamma", "dbeta"), backward_bounds(r, g, None, ref.SILU, S)):
+        assert (np.abs(out.numpy() - r[name]) <= t).all(), name
+    for b in (dx_, dg, y, mean, rstd, dx, dgamma, dbeta):
+        b.free()
+
+
+def test_many_samples_whose_groups_are_read_twice(dev):
+    """More samples than a grid has rows: the last ones get what they get in a call of their own."""
+    B, S, C, last = 65600, 257, 33, 70
+    n = S * C
+    x, g, dx = (dev.empty(B * n) for _ in range(3))
+    dev.init_normal_f32(x, B * n, 0.5, 2.0, 1)
+    dev.init_normal_f32(g, B * n, 0.0, 1.0, 2)
+    mean, rstd, part = dev.empty(B), dev.empty(B), dev.empty(last * n)
+    dev.init_normal_f32(mean, B, 0.5, 0.1, 3)
+    dev.init_uniform_f32(rstd, B, 0.4, 0.6, 4)
+    dev.groupnorm_bwd_f32(g, x, B, S, C, 1, None, None, mean, rstd, ref.SILU, dx)
+    at, st = 4 * (B - last) * n, 4 * (B - last)
+    dev.groupnorm_bwd_f32(g.ptr + at, x.ptr + at, last, S, C, 1, None, None, mean.ptr + st, rstd.ptr + st, ref.SILU, part)
+    got = np.empty(last * n, np.float32)
+    dev.d2h_raw(got.ctypes.data, dx.ptr + at, got.nbytes)
+    # dx is of the order of 1; its two means differ by the order of their sums (64 bits) and one rounding
+    assert np.abs(got - part.numpy()).max() <= 2.0**-20
+    xs, gs = np.empty((1, S, C), np.float32), np.empty((1, S, C), np.float32)
+    dev.d2h_raw(xs.ctypes.data, x.ptr + 4 * (B - 1) * n, xs.nbytes)
+    dev.d2h_raw(gs.ctypes.data, g.ptr + 4 * (B - 1) * n, gs.nbytes)
+    r = ref.groupnorm_bwd(gs, xs, 1, None, None, mean.numpy()[-1:, None], rstd.numpy()[-1:, None], ref.SILU)
+    t = backward_bounds(r, gs, None, ref.SILU, S)[0]
+    assert (np.abs(got[-n:].reshape(1, S, C) - r["dx"]) <= t).all()
+    for b in (x, g, dx, mean, rstd, part):
+        b.free()

@@ -1,5 +1,9 @@
 """Embedding, dropout and group norm captured into CUDA graphs, replayed on other streams beside one another, and called
 from two contexts: each keeps to its own workspace."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -143,6 +147,37 @@ def test_check_is_refused_under_capture_and_the_capture_goes_on(dev):
     ck(r.cudaGraphExecDestroy(ex))
     ck(r.cudaGraphDestroy(graph))
     w.free()
+
+
+FIRST_CALLS = """
+import sys
+sys.path[:0] = [{tests!r}, {root!r}]
+import numpy as np
+import test_gpu_token_ops_streams as t
+from vtl_b200 import capi
+dev = capi.Device(0)
+w = t.Work(dev, 8)
+dev.sync()
+graph, ex = t.capture(dev, w)
+w.clear()
+for _ in range(2):
+    t.ck(t.rt().cudaGraphLaunch(ex, dev.lib.vtlb_stream(dev.h)))
+dev.sync()
+replayed = w.results()
+w.clear()
+w.call()
+assert t.same(w.results(), replayed)
+assert any(v.any() for v in replayed.values())
+print("the same")
+"""
+
+
+def test_first_calls_of_a_process_under_capture():
+    """Kernels that are not loaded yet, attributes that are not set yet: a capture may be what meets them first."""
+    tests = os.path.dirname(os.path.abspath(__file__))
+    code = FIRST_CALLS.format(tests=tests, root=os.path.dirname(tests))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "the same" in r.stdout, r.stderr[-2000:]
 
 
 def test_two_contexts_at_once(dev):

@@ -201,6 +201,14 @@ class vtlb_workspace {
   size_t own_bytes_ = 0;
 };
 
+inline bool vtlb_early_on() {
+  static const bool on = [] {
+    const char* e = getenv("VTLB_EARLY_LAUNCH");
+    return !e || atoi(e) != 0;
+  }();
+  return on;
+}
+
 // Launch with programmatic stream serialisation: the kernel's CTAs may become resident while
 // the kernel in front of it in the stream is still finishing, which hides the launch latency
 // of short dependent kernels.  Only for kernels that execute griddepcontrol.wait before their
@@ -209,11 +217,6 @@ class vtlb_workspace {
 template <typename... KArgs, typename... Args>
 static inline cudaError_t vtlb_launch_early(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
                                             cudaStream_t stream, Args&&... args) {
-  static int on = -1;
-  if (on < 0) {
-    const char* e = getenv("VTLB_EARLY_LAUNCH");
-    on = e ? atoi(e) != 0 : 1;
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -223,7 +226,7 @@ static inline cudaError_t vtlb_launch_early(void (*kern)(KArgs...), dim3 grid, d
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = on ? 1 : 0;
+  cfg.numAttrs = vtlb_early_on() ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kern, static_cast<Args&&>(args)...);
 }
 

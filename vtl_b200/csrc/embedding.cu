@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(EmbGrad p, int spli
   }
 }
 
-__global__ void __launch_bounds__(256) ids_from_f32_kernel(const float* __restrict__ src, size_t n, int32_t* __restrict__ ids) {
+__global__ void __launch_bounds__(256) ids_from_f32_kernel(const float* src, size_t n, int32_t* ids) {
   for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
     const float v = src[i];
     ids[i] = v >= 0.0f && v < 2147483648.0f && v == truncf(v) ? (int32_t)v : -1;
@@ -626,7 +626,7 @@ cudaError_t sort_launch(vtlb_ctx* ctx, int ctas, const int32_t* ids, int n, int 
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = vtlb_early_on() ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, ids, n, V, passes, bits, sorted);
 }
 
@@ -779,6 +779,8 @@ VTLB_API int vtlb_ids_from_f32(vtlb_ctx* ctx, const void* d_src, size_t n, void*
   VTLB_ENTER(ctx);
   if (n == 0) return VTLB_OK;
   if (!d_src || !d_ids_i32) return vtlb_fail(ctx, VTLB_EINVAL, "vtlb_ids_from_f32: null pointer");
+  if (d_src != d_ids_i32 && vtlb_overlap(d_src, n, d_ids_i32, n))
+    return vtlb_fail(ctx, VTLB_EINVAL, "vtlb_ids_from_f32: source and ids overlap in part");
   ids_from_f32_kernel<<<grid_for(ctx, n), 256, 0, ctx->stream>>>((const float*)d_src, n, (int32_t*)d_ids_i32);
   VTLB_LAUNCHED(ctx);
   return VTLB_OK;

@@ -4,6 +4,8 @@
 // Backward, with dz = g * act'(z) and n = S * C/groups:
 //   dgamma_c = sum over samples and positions of dz * h,   dbeta_c = sum of dz,
 //   dx = rstd * (gamma_c * dz - (sum gamma dz) / n - h * (sum gamma dz h) / n), the sums over the group.
+#include <climits>
+
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -183,6 +185,7 @@ struct GnGrid {
   GnDims d;
   int shift;  // log2 of the pieces per CTA
   int rows;   // positions per chunk
+  int across;  // CTAs side by side
 };
 
 // Rows that a thread asks for before it uses the first one.  (The result may lie where x or g does, so the compiler would
@@ -206,7 +209,7 @@ __global__ void __launch_bounds__(256) gn_sums_kernel(const float* x, const floa
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const GnDims d = t.d;
   const int cols = 1 << t.shift, lanes = 256 >> t.shift, col = threadIdx.x & (cols - 1), lane = threadIdx.x >> t.shift;
-  const int c = (blockIdx.x * cols + col) * VEC, chunk = blockIdx.y, b = blockIdx.z;
+  const int b = (int)(blockIdx.x / t.across), c0 = (int)(blockIdx.x % t.across) * cols * VEC, c = c0 + col * VEC, chunk = blockIdx.y;
   const int r1 = min(d.S, (chunk + 1) * t.rows);
   double2 acc[VEC] = {};
   if (c < d.C) {
@@ -251,7 +254,7 @@ __global__ void __launch_bounds__(256) gn_sums_kernel(const float* x, const floa
   for (int k = 0; k < VEC; ++k) sm[threadIdx.x * VEC + k] = acc[k];
   __syncthreads();
   for (int i = threadIdx.x; i < cols * VEC; i += 256) {
-    const int ch = blockIdx.x * cols * VEC + i;
+    const int ch = c0 + i;
     if (ch >= d.C) break;
     double2 s = sm[i];
     for (int l = 1; l < lanes; ++l) s.x += sm[l * cols * VEC + i].x, s.y += sm[l * cols * VEC + i].y;
@@ -335,7 +338,7 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const float* x, const flo
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const GnDims d = t.d;
   const int cols = 1 << t.shift, lanes = 256 >> t.shift, col = threadIdx.x & (cols - 1), lane = threadIdx.x >> t.shift;
-  const int c = (blockIdx.x * cols + col) * VEC, chunk = blockIdx.y, b = blockIdx.z;
+  const int b = (int)(blockIdx.x / t.across), c0 = (int)(blockIdx.x % t.across) * cols * VEC, c = c0 + col * VEC, chunk = blockIdx.y;
   const int r1 = min(d.S, (chunk + 1) * t.rows);
   if (c >= d.C) return;
   GnVec<VEC> mu, rs, ga, be, c1 = {}, c2 = {};
@@ -974,12 +977,16 @@ cudaError_t cluster_launch(vtlb_ctx* ctx, GnKernelInfo& info, void (*kern)(KArgs
   cfg.dynamicSmemBytes = smem;
   cfg.stream = ctx->stream;
   cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = cluster, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
+  if (vtlb_early_on()) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    auto& dim = at[cfg.numAttrs++].val.clusterDim;
+    dim.x = cluster, dim.y = 1, dim.z = 1;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
   cudaError_t e;
   std::atomic<bool>* allowed = ctx->device < GnKernelInfo::kDevices ? &info.allowed[ctx->device] : nullptr;
   if (!allowed || !allowed->load(std::memory_order_relaxed)) {
@@ -1030,18 +1037,20 @@ int check_dims(vtlb_ctx* ctx, const char* fn, int B, int S, int C, int groups, i
     return vtlb_fail(ctx, VTLB_EINVAL, "%s: bad shape B=%d S=%d C=%d groups=%d", fn, B, S, C, groups);
   if (act_kind != VTLB_ACT_NONE && act_kind != VTLB_ACT_RELU && act_kind != VTLB_ACT_SILU)
     return vtlb_fail(ctx, VTLB_EINVAL, "%s: unknown activation %d", fn, act_kind);
-  if (B > 65535 || S > 65535 * kRows)
-    return vtlb_fail(ctx, VTLB_EINVAL, "%s: B=%d S=%d is beyond 65535 samples of %d positions", fn, B, S, 65535 * kRows);
+  // (CTAs, units and rows of sums are counted in 31 bits; a sample's chunks are a grid's second dimension)
+  if ((long long)B * groups > INT_MAX || (long long)B * S > INT_MAX || S > 65535 * kRows)
+    return vtlb_fail(ctx, VTLB_EINVAL, "%s: B=%d S=%d groups=%d: B * S and B * groups go to 2^31 - 1, S to %d", fn, B, S, groups, 65535 * kRows);
   *d = GnDims{B, S, C, groups, C / groups};
   return VTLB_OK;
 }
 
 GnGrid grid_of(const GnDims& d, int vec, int sm_count) {
-  GnGrid t{d, 0, kRows};
+  GnGrid t{d, 0, kRows, 1};
   while (t.shift < 8 && (1 << t.shift) * vec < d.C && ((1 << t.shift) < 32 || d.S * (1 << t.shift) < kRows * 8)) ++t.shift;
   // 32 pieces wide as a rule, wider where there are few rows; four rows a thread at least.
-  const long long across = (long long)d.B * ((d.C + (vec << t.shift) - 1) / (vec << t.shift));
-  while (t.rows > 4 * (256 >> t.shift) && t.rows > 32 && across * ((d.S + t.rows - 1) / t.rows) < 2LL * sm_count) t.rows /= 2;
+  t.across = (d.C + (vec << t.shift) - 1) / (vec << t.shift);
+  const long long ctas = (long long)d.B * t.across;
+  while (t.rows > 4 * (256 >> t.shift) && t.rows > 32 && ctas * ((d.S + t.rows - 1) / t.rows) < 2LL * sm_count) t.rows /= 2;
   return t;
 }
 
@@ -1052,7 +1061,7 @@ int gn_forward_general(vtlb_ctx* ctx, const float* x, GnDims d, const float* gam
                        float* mean, float* rstd) {
   const GnGrid t = grid_of(d, VEC, ctx->sm_count);
   const int chunks = (d.S + t.rows - 1) / t.rows;
-  const dim3 grid((d.C + (VEC << t.shift) - 1) / (VEC << t.shift), chunks, d.B);
+  const dim3 grid((unsigned)d.B * t.across, chunks);
   vtlb_workspace ws(ctx);
   void* partial = nullptr;
   if (int rc = ws.get((size_t)d.B * chunks * d.C * sizeof(double2), &partial)) return rc;
@@ -1074,7 +1083,7 @@ int gn_backward_general(vtlb_ctx* ctx, const float* g, const float* x, GnDims d,
                         const float* mean, const float* rstd, float* dx, float* dgamma, float* dbeta) {
   const GnGrid t = grid_of(d, VEC, ctx->sm_count);
   const int chunks = (d.S + t.rows - 1) / t.rows;
-  const dim3 grid((d.C + (VEC << t.shift) - 1) / (VEC << t.shift), chunks, d.B);
+  const dim3 grid((unsigned)d.B * t.across, chunks);
   const size_t sums = (size_t)d.B * chunks * d.C * sizeof(double2);
   vtlb_workspace ws(ctx);
   void* scratch = nullptr;
