@@ -449,8 +449,9 @@ __global__ void __launch_bounds__(256, 4) embedding_few_kernel(EmbGrad p, vtlb_m
 }
 
 constexpr int kTileMax = 64, kCtaPositions = 1024;  // positions per tile and per CTA
+// (Four CTAs per SM without a mask: 16384 x 4096 186 us in all, 189 with three; with one three: 251 and 255.)
 template <bool VEC, bool DROP>
-__global__ void __launch_bounds__(256, 3) embedding_sums_kernel(EmbGrad p, vtlb_mask m, unsigned zero_ctas) {
+__global__ void __launch_bounds__(256, DROP ? 3 : 4) embedding_sums_kernel(EmbGrad p, vtlb_mask m, unsigned zero_ctas) {
   __shared__ int2 window[kCtaPositions + 2 * kTileMax + 2];  // the sorted positions of this CTA's tiles and a tile around them
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x < zero_ctas) {
