@@ -9,7 +9,9 @@ namespace {
 
 // Four consecutive elements of y per step, U steps at a time: bound by HBM (a row of W in, a row of y out), so what counts is
 // that every thread has U loads in flight.  VEC: D is a multiple of four and both arrays are 16-byte aligned, so that
-// the four lie in one row.
+// the four lie in one row.  16384 rows of 4096 out of 50000: 63 us, 5.9 TB/s, 90 % of a plain copy's rate (a simple
+// kernel with one load in flight: 170 us).  999 rows of 2047 with dropout: 6.3 us, of which the mask's ten dependent rounds and
+// the loads of ids and rows behind one another leave little to gain.  Eight rows of 4096: 4.5 us, the host's call.
 template <bool VEC, bool DROP, int U>
 __global__ void __launch_bounds__(256) embedding_fwd_kernel(const float* __restrict__ W, int V, uint32_t D,
                                                             const int32_t* __restrict__ ids, size_t total, float scale,
@@ -77,7 +79,10 @@ __global__ void __launch_bounds__(256) embedding_fwd_kernel(const float* __restr
 //          Rows of tokens that do not occur are zeroed by further CTAs of this launch, which need nothing of the sort and
 //          start while it runs
 //   join   the partial rows of each long run, in order
-// Bound by HBM: the rows of g that count are read once and dW is written once.
+// Bound by HBM: the rows of g that count are read once and dW is written once.  16384 x 4096 into 50000 rows: 186 us,
+// 5.8 TB/s, 89 % of a plain copy's rate.  8191 x 1023 with a mask into 3001 rows: 41 us against 5.7 of bytes; there it is
+// the sort (10 us, partly beside the zeroing), two rounds of loads and masks per tile with 20 warps on an SM (some 25), and
+// the join (7) behind one another.
 
 // Sort of up to kRankMax positions: a warp finds the ranks of four of them by comparing with all.  n^2 comparisons, two
 // instructions each, spread over the whole GPU, against two or three passes of a few microseconds each on one cluster.
@@ -131,7 +136,10 @@ size_t sort_smem(int items) {
 }
 
 // Radix sort of more positions, least significant digit first, in the shared memory of one thread-block cluster: CTA r
-// holds elements [r, r + 1) * 1024 * ITEMS of the current order, a warp 32 * ITEMS consecutive ones of them.
+// holds elements [r, r + 1) * 1024 * ITEMS of the current order, a warp 32 * ITEMS consecutive ones of them.  A pass ranks
+// a warp's elements by matching digits, adds up the warps' and CTAs' counts and sends each element to its place in some
+// CTA's shared memory; the keys have as many passes of up to nine bits as V needs.  Bound by the latency of the barriers
+// in the cluster: 16 us for 16384 positions of 16 bits, during which the zeroing writes 100 MB.
 template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(const int32_t* __restrict__ ids, int n, int V, int passes,
                                                                   int bits, int2* __restrict__ sorted) {
@@ -545,7 +553,8 @@ __global__ void __launch_bounds__(256, DROP ? 3 : 4) embedding_sums_kernel(EmbGr
 
 // Where a long run starts in tile t, its partial rows (slot 1 of tile t, slot 0 of the following ones) are added up: eight
 // stretches of them at a time, and the stretches in order.  A CTA looks after eight tiles (most start no long run, and
-// a CTA per tile costs more than the sums) and one of `split` shares of the columns.
+// a CTA per tile costs more than the sums) and one of `split` shares of the columns.  Bound by the latency of its few
+// loads behind one another: 7 us behind 8191 x 1023.
 constexpr int kJoinTiles = 8;
 template <bool VEC>
 __global__ void __launch_bounds__(256) embedding_join_kernel(EmbGrad p, int split) {
