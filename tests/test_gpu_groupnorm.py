@@ -54,7 +54,8 @@ def backward_bounds(r, g, gamma, kind, S):
 SHAPES = [(1, 1, 1, 1), (2, 1, 8, 2), (1, 2, 4, 4), (3, 5, 6, 3), (2, 64, 128, 32), (1, 1000, 33, 11), (3, 323, 330, 30),
           (4, 1024, 256, 32), (1, 4097, 40, 5), (2, 7, 4096, 1), (65, 3, 20, 4), (1, 20001, 8, 2), (5, 1, 1000, 1),
           (2, 130, 36, 3), (300, 17, 64, 64), (1, 300, 1028, 2), (2, 2048, 24, 24), (1, 9000, 72, 1), (3, 33, 130, 13),
-          (2, 515, 96, 3), (1, 1, 20000, 1), (1, 5, 40000, 2)]
+          (2, 515, 96, 3), (1, 1, 20000, 1), (1, 5, 40000, 2), (37, 1, 4096, 1), (9, 1, 16384, 2), (3, 1, 8196, 1), (50, 1, 130, 10),
+          (1000, 1, 640, 5), (33, 1, 2047, 1), (200, 1, 300, 1), (7, 1, 513, 1), (65, 1, 96, 32), (20000, 1, 600, 1)]
 
 
 @pytest.mark.parametrize("B,S,C,G", SHAPES)

@@ -173,6 +173,176 @@ __device__ __forceinline__ float inv_sqrt(double v) {
   return (float)(r * fma(-0.5 * v * r, r, 1.5));
 }
 
+// ---------------------------------------------------------------- one position per sample
+// Plain features and tokens (a layer norm, where there is one group): a group is one row of `width` values next to one
+// another.  L threads hold it, PER pieces of VEC each, and a CTA of 256 holds 256 / L rows, so that no thread idles and
+// no cluster is kept for a kilobyte.  Bound by HBM, 8 bytes per element forward, 12 backward: 10000 rows of 4096 52 us, 6.4 TB/s, and
+// 101 us, 4.9 TB/s (by the clusters below, which pay for an exchange per row, 248 and 531); 500000 of 64 40 and 84 us (2707
+// and 4730); 65536 of 32 groups of 32 with SiLU 127 and 216 us.
+constexpr int kGnRowThreads = 256;
+template <int L>
+__device__ __forceinline__ float2 gn_row_sum(float2 v, float2* sm, int turn) {  // over the L threads of a row
+#pragma unroll
+  for (int o = (L < 32 ? L : 32) / 2; o; o >>= 1) v.x += __shfl_xor_sync(~0u, v.x, o), v.y += __shfl_xor_sync(~0u, v.y, o);
+  if constexpr (L > 32) {
+    float2* box = sm + turn * (kGnRowThreads / 32);  // (two in turn: the next but one sum is written behind a barrier)
+    if ((threadIdx.x & 31) == 0) box[threadIdx.x >> 5] = v;
+    __syncthreads();
+    box += threadIdx.x / L * (L / 32);
+    v = box[0];
+#pragma unroll
+    for (int q = 1; q < L / 32; ++q) v.x += box[q].x, v.y += box[q].y;
+  }
+  return v;
+}
+
+template <int ACT, int VEC, int L, int PER>
+__global__ void __launch_bounds__(kGnRowThreads) gn_rows_fwd_kernel(const float* x, const float* gamma, const float* beta, GnDims d,
+                                                                    float eps, float* y, float* mean_out, float* rstd_out) {
+  __shared__ float2 sm[2 * kGnRowThreads / 32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int t = threadIdx.x % L, W = d.width;
+  const size_t row = blockIdx.x * (size_t)(kGnRowThreads / L) + threadIdx.x / L;
+  const bool in = row < (size_t)d.B * d.G;
+  const float* from = x + row * W;
+  GnVec<VEC> v[PER];
+  GnVec<VEC> s1 = gn_splat<VEC>(0.0f), s2 = s1;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = (i * L + t) * VEC;
+    v[i] = in && e < W ? gn_load<VEC>(from + e) : gn_splat<VEC>(0.0f);
+    s1 = vadd(s1, v[i]);
+  }
+  float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) s.x += s1.e[k];
+  const float part = 1.0f / (float)W;
+  const float m0 = gn_row_sum<L>(s, sm, 0).x * part;  // the mean but for its rounding; then the distances from it
+  const GnVec<VEC> minus0 = gn_splat<VEC>(-m0);
+  s1 = gn_splat<VEC>(0.0f);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if ((i * L + t) * VEC >= W) break;
+    const GnVec<VEC> a = vadd(v[i], minus0);
+    s1 = vadd(s1, a);
+    s2 = vfma(a, a, s2);
+  }
+  s = make_float2(0.0f, 0.0f);
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) s.x += s1.e[k], s.y += s2.e[k];
+  s = gn_row_sum<L>(s, sm, 1);
+  const float off = s.x * part, var = fmaf(s.y, part, -off * off);
+  const float mu = m0 + off, rs = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);
+  if (!in) return;
+  if (t == 0) mean_out[row] = mu, rstd_out[row] = rs;
+  const GnVec<VEC> minus = gn_splat<VEC>(-mu), scale = gn_splat<VEC>(rs);
+  const int c0 = (int)(row % d.G) * W;
+  float* to = y + row * W;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = (i * L + t) * VEC;
+    if (e >= W) break;
+    const GnVec<VEC> ga = gamma ? gn_load<VEC>(gamma + c0 + e) : gn_splat<VEC>(1.0f);
+    const GnVec<VEC> be = beta ? gn_load<VEC>(beta + c0 + e) : gn_splat<VEC>(0.0f);
+    gn_store<VEC>(to + e, act<ACT>(vfma(vmul(vadd(v[i], minus), scale), ga, be)));
+  }
+}
+
+// A CTA takes `each` rows of one group per place for a row, and leaves one row of sums for dgamma and dbeta (at most 64 rows
+// are added in f32, the places and, in gn_params_kernel, the CTAs in f64).
+template <int ACT, int VEC, int L, int PER>
+__global__ void __launch_bounds__(kGnRowThreads, PER > 4 ? 1 : 2)
+    gn_rows_bwd_kernel(const float* g, const float* x, const float* gamma, const float* beta, const float* mean, const float* rstd,
+                       GnDims d, int each, float* dx, float2* sums) {
+  constexpr int R = kGnRowThreads / L;
+  __shared__ float2 sm[2 * kGnRowThreads / 32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int t = threadIdx.x % L, place = threadIdx.x / L, W = d.width;
+  const int group = (int)(blockIdx.x % d.G), chunk = (int)(blockIdx.x / d.G), c0 = group * W;
+  const float part = 1.0f / (float)W;
+  GnVec<VEC> sum1[PER], sum2[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sum1[i] = sum2[i] = gn_splat<VEC>(0.0f);
+  const long long first = (long long)chunk * each * R, end = min((long long)d.B, first + (long long)each * R);
+  constexpr bool AHEAD = PER <= 4;  // the next row is fetched while this one is worked on, where the registers allow
+  GnVec<VEC> vx[PER], vg[PER], nx[PER], ng[PER];
+  float mu_next = 0.0f, rs_next = 0.0f;
+  const auto fetch = [&](GnVec<VEC>(&vx)[PER], GnVec<VEC>(&vg)[PER], long long b) {
+    const size_t row = (size_t)b * d.G + group;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = (i * L + t) * VEC;
+      vx[i] = vg[i] = gn_splat<VEC>(0.0f);
+      if (b < end && e < W) vx[i] = gn_load<VEC>(x + row * W + e), vg[i] = gn_load<VEC>(g + row * W + e);
+    }
+    if (b < end) mu_next = mean[row], rs_next = rstd[row];
+  };
+  fetch(nx, ng, first + place);
+  for (long long b0 = first, k = 0; b0 < end; b0 += R, ++k) {
+    const bool in = b0 + place < end;
+    const size_t row = (size_t)(b0 + place) * d.G + group;
+    const GnVec<VEC> mu = gn_splat<VEC>(mu_next), rs = gn_splat<VEC>(rs_next), minus = vneg(mu);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) vx[i] = nx[i], vg[i] = ng[i];
+    if (AHEAD) fetch(nx, ng, b0 + R + place);
+    GnVec<VEC> s1 = gn_splat<VEC>(0.0f), s2 = s1;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = (i * L + t) * VEC;
+      if (!in || e >= W) break;
+      const GnVec<VEC> ga = gamma ? gn_load<VEC>(gamma + c0 + e) : gn_splat<VEC>(1.0f);
+      const GnVec<VEC> be = beta ? gn_load<VEC>(beta + c0 + e) : gn_splat<VEC>(0.0f);
+      const GnVec<VEC> h = vmul(vadd(vx[i], minus), rs), dz = act_bwd<ACT>(vg[i], vx[i], mu, rs, ga, be, h);
+      sum1[i] = vadd(sum1[i], dz);
+      sum2[i] = vfma(dz, h, sum2[i]);
+      vx[i] = h;
+      vg[i] = vmul(dz, ga);
+      s1 = vadd(s1, vg[i]);
+      s2 = vfma(vg[i], h, s2);
+    }
+    if (dx) {
+      float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) s.x += s1.e[q], s.y += s2.e[q];
+      s = gn_row_sum<L>(s, sm, (int)k & 1);
+      const GnVec<VEC> m1 = gn_splat<VEC>(-s.x * part), m2 = gn_splat<VEC>(-s.y * part);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int e = (i * L + t) * VEC;
+        if (!in || e >= W) break;
+        gn_store<VEC>(dx + row * W + e, vmul(rs, vadd(vg[i], vfma(vx[i], m2, m1))));
+      }
+    }
+    if (!AHEAD) fetch(nx, ng, b0 + R + place);
+  }
+  if (!sums) return;
+  float2* out = sums + (size_t)chunk * d.C + c0;
+  if constexpr (R > 1) {
+    constexpr int kRow = L * PER * VEC;
+    __shared__ float2 box[R * kRow];
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) box[place * kRow + (i * L + t) * VEC + q] = make_float2(sum1[i].e[q], sum2[i].e[q]);
+    __syncthreads();
+    for (int e = threadIdx.x; e < W; e += kGnRowThreads) {
+      double2 s = make_double2(0.0, 0.0);
+      for (int q = 0; q < R; ++q) s.x += (double)box[q * kRow + e].x, s.y += (double)box[q * kRow + e].y;
+      out[e] = make_float2((float)s.x, (float)s.y);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = (i * L + t) * VEC;
+      if (e >= W) break;
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) out[e + q] = make_float2(sum1[i].e[q], sum2[i].e[q]);
+    }
+  }
+}
+
 // ---------------------------------------------------------------- groups of any size
 // Two passes over x (and g): sums per channel and chunk of positions, then the result.  CTAs take 256 threads as
 // `cols` pieces of VEC channels by 256 / cols rows.  Sums are f64: sum and sum of squares forward, dz and dz * h backward.
@@ -1115,9 +1285,74 @@ int gn_backward_general(vtlb_ctx* ctx, const float* g, const float* x, GnDims d,
   return VTLB_OK;
 }
 
+// Threads per row and pieces per thread, the fewest that hold it (pieces of four values, or one); false: too long a row.
+bool gn_row_shape(int width, int vec, bool bwd, int* threads, int* per) {
+  const int shapes[2][7][2] = {{{8, 2}, {8, 8}, {32, 4}, {32, 8}, {256, 2}, {256, 4}, {256, 8}},
+                               {{8, 2}, {32, 2}, {64, 2}, {128, 2}, {256, 2}, {256, 4}, {256, 8}}};
+  for (const auto& s : shapes[bwd])
+    if (width <= s[0] * s[1] * vec) {
+      *threads = s[0], *per = s[1];
+      return true;
+    }
+  return false;
+}
+
+template <int ACT, int VEC>
+int gn_forward_rows(vtlb_ctx* ctx, int threads, int per, const float* x, GnDims d, const float* gamma, const float* beta,
+                    double eps, float* y, float* mean, float* rstd) {
+  auto kern = threads == 8 ? (per == 2 ? gn_rows_fwd_kernel<ACT, VEC, 8, 2> : gn_rows_fwd_kernel<ACT, VEC, 8, 8>)
+              : threads == 32 ? (per == 4 ? gn_rows_fwd_kernel<ACT, VEC, 32, 4> : gn_rows_fwd_kernel<ACT, VEC, 32, 8>)
+              : per == 2      ? gn_rows_fwd_kernel<ACT, VEC, 256, 2>
+              : per == 4      ? gn_rows_fwd_kernel<ACT, VEC, 256, 4>
+                              : gn_rows_fwd_kernel<ACT, VEC, 256, 8>;
+  const int places = kGnRowThreads / threads;
+  const size_t ctas = ((size_t)d.B * d.G + places - 1) / places;
+  VTLB_CUDA(ctx, vtlb_launch_early(kern, dim3((unsigned)ctas), dim3(kGnRowThreads), 0, ctx->stream, x, gamma, beta, d, (float)eps, y, mean, rstd));
+  VTLB_LAUNCHED(ctx);
+  return VTLB_OK;
+}
+
+template <int ACT, int VEC>
+int gn_backward_rows(vtlb_ctx* ctx, int threads, int per, const float* g, const float* x, GnDims d, const float* gamma,
+                     const float* beta, const float* mean, const float* rstd, float* dx, float* dgamma, float* dbeta) {
+  auto kern = threads == 8 ? gn_rows_bwd_kernel<ACT, VEC, 8, 2>
+              : threads == 32  ? gn_rows_bwd_kernel<ACT, VEC, 32, 2>
+              : threads == 64  ? gn_rows_bwd_kernel<ACT, VEC, 64, 2>
+              : threads == 128 ? gn_rows_bwd_kernel<ACT, VEC, 128, 2>
+              : per == 2       ? gn_rows_bwd_kernel<ACT, VEC, 256, 2>
+              : per == 4       ? gn_rows_bwd_kernel<ACT, VEC, 256, 4>
+                               : gn_rows_bwd_kernel<ACT, VEC, 256, 8>;
+  // Up to 64 rows to a place, but eight CTAs per SM first; four, where that takes fewer than sixteen rows each, whose
+  // sums are a twelfth of the bytes (10000 x 4096: 101 us with sixteen, 110 with eight).
+  const int places = kGnRowThreads / threads;
+  const long long steps = ((long long)d.B + places - 1) / places;
+  const long long fill = steps * d.G / ((long long)ctx->sm_count * 4);  // rows to a place with four CTAs per SM
+  const long long each = fill < 1 ? 1 : fill <= 16 ? fill : fill <= 32 ? 16 : fill <= 128 ? fill / 2 : 64;
+  const long long chunks = (steps + each - 1) / each;
+  vtlb_workspace ws(ctx);
+  void* sums = nullptr;
+  if (dgamma || dbeta)
+    if (int rc = ws.get((size_t)chunks * d.C * sizeof(float2), &sums)) return rc;
+  VTLB_CUDA(ctx, vtlb_launch_early(kern, dim3((unsigned)(chunks * d.G)), dim3(kGnRowThreads), 0, ctx->stream, g, x, gamma, beta, mean,
+                                   rstd, d, (int)each, dx, (float2*)sums));
+  VTLB_LAUNCHED(ctx);
+  if (!sums) return VTLB_OK;
+  VTLB_CUDA(ctx, vtlb_launch_early(gn_params_kernel<float2>, dim3((d.C + 7) / 8), dim3(256), 0, ctx->stream, (const float2*)sums,
+                                   (int)chunks, d.C, dgamma, dbeta));
+  VTLB_LAUNCHED(ctx);
+  return VTLB_OK;
+}
+
 template <int ACT>
 int gn_forward(vtlb_ctx* ctx, const float* x, GnDims d, const float* gamma, const float* beta, double eps, float* y,
                float* mean, float* rstd) {
+  if (d.S == 1) {
+    const bool vec = d.width % 4 == 0 && vtlb_aligned16(x) && vtlb_aligned16(y) && vtlb_aligned16(gamma) && vtlb_aligned16(beta);
+    int threads, per;
+    if (gn_row_shape(d.width, vec ? 4 : 1, false, &threads, &per))
+      return vec ? gn_forward_rows<ACT, 4>(ctx, threads, per, x, d, gamma, beta, eps, y, mean, rstd)
+                 : gn_forward_rows<ACT, 1>(ctx, threads, per, x, d, gamma, beta, eps, y, mean, rstd);
+  }
   const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, vtlb_aligned16(x) && vtlb_aligned16(y), kGnFwdThreads, 4, 16, ctx->sm_count);
   if (plan.on_chip) {
     const GnTile t = tile_of(d, plan);
@@ -1153,6 +1388,13 @@ template <int ACT>
 int gn_backward(vtlb_ctx* ctx, const float* g, const float* x, GnDims d, const float* gamma, const float* beta,
                 const float* mean, const float* rstd, float* dx, float* dgamma, float* dbeta) {
   const bool aligned = vtlb_aligned16(x) && vtlb_aligned16(g) && vtlb_aligned16(dx);
+  if (d.S == 1) {
+    const bool vec = d.width % 4 == 0 && aligned && vtlb_aligned16(gamma) && vtlb_aligned16(beta);
+    int threads, per;
+    if (gn_row_shape(d.width, vec ? 4 : 1, true, &threads, &per))
+      return vec ? gn_backward_rows<ACT, 4>(ctx, threads, per, g, x, d, gamma, beta, mean, rstd, dx, dgamma, dbeta)
+                 : gn_backward_rows<ACT, 1>(ctx, threads, per, g, x, d, gamma, beta, mean, rstd, dx, dgamma, dbeta);
+  }
   const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, aligned, kGnBwdThreads, 4, 8, ctx->sm_count);
   vtlb_workspace ws(ctx);
   void* scratch = nullptr;
