@@ -202,7 +202,11 @@ def test_builder_refusals(sess):
         m.groupnorm(2, eps=-1.0)
     with pytest.raises(VtlbError, match="positive"):
         m.embedding(0, 8)
+    with pytest.raises(VtlbError, match="2\\^24"):
+        m.embedding((1 << 24) + 2, 1)
     m.groupnorm(2)
+    with pytest.raises(VtlbError, match="follows the input"):
+        m.embedding(5, 8)
     d = sess.dev.zeros(64)
     with pytest.raises(VtlbError, match="batch"):
         m.forward(d, (0, 3, 4, 4), d)

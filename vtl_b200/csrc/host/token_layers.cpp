@@ -74,6 +74,7 @@ struct GroupNormGate : Gate {
 EmbeddingLayer::EmbeddingLayer(Context* ctx, std::vector<int> in, int vocabulary_, int dim_, float scale_)
     : in_shape(std::move(in)), vocabulary(vocabulary_), dim(dim_), scale(scale_) {
   if (vocabulary <= 0 || dim <= 0) throw Error(VTLB_EINVAL, "EmbeddingLayer: vocabulary and dimension must be positive");
+  if (vocabulary > (1 << 24) + 1) throw Error(VTLB_EINVAL, "EmbeddingLayer: tokens arrive as f32, which holds whole numbers to 2^24");
   Session* s = ctx->device_session;
   Tensor w = Tensor::empty(s, {vocabulary, dim});
   s->check(vtlb_init_normal_f32(s->ctx, w.data(), w.size(), 0.0, 1.0, s->next_init_seed()));
@@ -169,6 +170,8 @@ VarPtr GroupNormLayer::forward(const VarPtr& input) {
 
 // ---------------------------------------------------------------- Sequential builders
 void Sequential::embedding(int vocabulary, int dim, double scale) {
+  for (const auto& l : layers)  // no gradient goes through tokens
+    if (std::strcmp(l->kind(), "input")) throw Error(VTLB_EINVAL, "Sequential.embedding: takes tokens, so it follows the input");
   layers.push_back(std::make_unique<EmbeddingLayer>(&ctx_, cur_shape(), vocabulary, dim, (float)scale));
 }
 void Sequential::dropout(double p) { layers.push_back(std::make_unique<DropoutLayer>(&ctx_, cur_shape(), p)); }
