@@ -891,12 +891,18 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
         gn_send(mail, turn, rank, ctas, tid, s);
       }
     } else {
-      // one warp per group of the slab: its entries in this CTA
+      // A thread per entry adds up the rows of sums; then one warp per group of the slab, its entries in this CTA.
+      for (int e = tid; parts > 1 && e < entries; e += T) {
+        double2 s = sm_pair[e];
+#pragma unroll 5
+        for (int q = 1; q < parts; ++q) s.x += sm_pair[q * entries + e].x, s.y += sm_pair[q * entries + e].y;
+        sm_pair[e] = s;
+      }
+      if (parts > 1) __syncthreads();
       for (int g = warp; g < p.groups; g += T / 32) {
         const int lo = max(g * width - p.in_slab, 0) / PER, hi = min((g + 1) * width - p.in_slab, p.channels) / PER;
         double2 s = make_double2(0.0, 0.0);
-        for (int q = 0; q < parts; ++q)
-          for (int e = lo + (tid & 31); e < hi; e += 32) s.x += sm_pair[q * entries + e].x, s.y += sm_pair[q * entries + e].y;
+        for (int e = lo + (tid & 31); e < hi; e += 32) s.x += sm_pair[e].x, s.y += sm_pair[e].y;
 #pragma unroll
         for (int o = 16; o; o >>= 1) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
         if ((tid & 31) == 0) gn_send(mail, turn, rank, ctas, g, s);

@@ -44,10 +44,10 @@ inline GnPlan gn_plan_slab(int B, int S, int C, int G, int vec, int groups, int 
   const auto fits = [&](int vpt, int rsplit) { return (long long)lanes * vpt * rsplit >= S; };
   const int max_r = kGnMaxCluster / p.csplit;
   p.rsplit = 1;
-  while (p.rsplit < max_r && !fits(most, p.rsplit)) p.rsplit *= 2;
+  while (p.rsplit < max_r && !fits(most, p.rsplit)) ++p.rsplit;
   if (!fits(most, p.rsplit)) return p;
   // Too few CTAs for the SMs: shorter stretches.
-  while (p.rsplit < max_r && !fits(1, p.rsplit) && (long long)B * p.slabs * p.csplit * p.rsplit * 2 <= sm_count) p.rsplit *= 2;
+  while (p.rsplit * 2 <= max_r && !fits(1, p.rsplit) && (long long)B * p.slabs * p.csplit * p.rsplit * 2 <= sm_count) p.rsplit *= 2;
   p.rows = (S + p.rsplit - 1) / p.rsplit;
   p.vpt = p.rows <= lanes ? 1 : p.rows <= lanes * middle ? middle : most;
   // TMA boxes are at most 256 by 256; rows of less than 64 bytes are not worth one.  Nor is a map, half a microsecond of the
