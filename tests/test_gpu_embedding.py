@@ -28,7 +28,7 @@ def tokens(rng, n, V, how):
     return ids
 
 
-SHAPES = [(1, 1, 1), (1, 8, 5), (3, 4, 2), (8, 256, 100), (33, 7, 3), (257, 130, 1000), (512, 96, 40), (513, 97, 40), (600, 640, 7), (999, 2047, 61), (1024, 64, 17),
+SHAPES = [(1, 1, 1), (1, 8, 5), (3, 4, 2), (8, 256, 100), (33, 7, 3), (257, 130, 1000), (512, 96, 40), (513, 97, 40), (600, 640, 7), (150, 1027, 9), (999, 2047, 61), (1024, 64, 17),
           (4097, 12, 5000), (8192, 20, 70000), (20011, 5, 300)]
 HOW = ["uniform", "skewed", "one", "distinct", "padded"]
 

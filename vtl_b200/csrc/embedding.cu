@@ -10,12 +10,12 @@ namespace {
 // Four consecutive elements of y per step, U steps at a time: bound by HBM (a row of W in, a row of y out), so what counts is
 // that every thread has U loads in flight.  VEC: D is a multiple of four and both arrays are 16-byte aligned, so that
 // the four lie in one row.  16384 rows of 4096 out of 50000: 63 us, 5.9 TB/s, 90 % of a plain copy's rate (a simple
-// kernel with one load in flight: 170 us).  999 rows of 2047 with dropout: 6.3 us, of which the mask's ten dependent rounds and
+// kernel with one load in flight: 170 us).  999 rows of 2047 with dropout: 6.2 us, of which the mask's ten dependent rounds and
 // the loads of ids and rows behind one another leave little to gain.  Eight rows of 4096: 4.5 us, the host's call.
 template <bool VEC, bool DROP, int U>
 __global__ void __launch_bounds__(256) embedding_fwd_kernel(const float* __restrict__ W, int V, uint32_t D,
                                                             const int32_t* __restrict__ ids, size_t total, float scale,
-                                                            float* __restrict__ y, int y_aligned, vtlb_mask m,
+                                                            float* __restrict__ y, bool blocks_of_w, bool y_aligned, vtlb_mask m,
                                                             uint32_t* bad) {
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the kernel in front is done from here on
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -38,6 +38,16 @@ __global__ void __launch_bounds__(256) embedding_fwd_kernel(const float* __restr
     if (VEC) {
       const float4 f = in ? __ldg(reinterpret_cast<const float4*>(W + (size_t)id * D + col)) : make_float4(0, 0, 0, 0);
       v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
+    } else if (blocks_of_w && in && col + 4 <= D && ((size_t)id * D + col) / 4 * 4 + 8 <= (size_t)V * D) {
+      // all of one row: the two aligned blocks that hold them (a neighbour's, too, so that HBM sees each once)
+      const size_t at = (size_t)id * D + col;
+      const uint32_t o = (uint32_t)at & 3;
+      const float4* blocks = reinterpret_cast<const float4*>(W) + at / 4;
+      const float4 a = __ldg(blocks), b = o ? __ldg(blocks + 1) : a;
+      v[u][0] = o == 0 ? a.x : o == 1 ? a.y : o == 2 ? a.z : a.w;
+      v[u][1] = o == 0 ? a.y : o == 1 ? a.z : o == 2 ? a.w : b.x;
+      v[u][2] = o == 0 ? a.z : o == 1 ? a.w : o == 2 ? b.x : b.y;
+      v[u][3] = o == 0 ? a.w : o == 1 ? b.x : o == 2 ? b.y : b.z;
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -741,6 +751,9 @@ VTLB_API int vtlb_embedding_fwd_f32(vtlb_ctx* ctx, const void* d_W, int V, int D
   }
   const vtlb_mask m = vtlb_make_mask(p, seed, step);
   const bool y_aligned = vtlb_aligned16(d_Y), vec = D % 4 == 0 && vtlb_aligned16(d_W) && y_aligned;
+  // Rows of odd widths in aligned blocks where few warps meet the end of a row (16384 x 4095: 96 -> 90 us, with a mask 139 ->
+  // 122; but 16384 x 181: 6.6 -> 7.2).
+  const bool blocks_of_w = vtlb_aligned16(d_W) && D >= 512;
   // Four loads in flight per thread where that still leaves eight CTAs for every SM (999 x 2047: one 6.8 us, four 9.3;
   // 3000 x 2047: one 16.1, four 15.3).
   const int U = total >= (size_t)ctx->sm_count * 8 * 256 * 4 * 4 ? 4 : 1;
@@ -751,7 +764,7 @@ VTLB_API int vtlb_embedding_fwd_f32(vtlb_ctx* ctx, const void* d_W, int V, int D
   const size_t ctas = (total + 1024 * U - 1) / (1024 * U);
   if (ctas > 0x7fffffffu) return vtlb_fail(ctx, VTLB_EINVAL, "vtlb_embedding_fwd_f32: n * D is beyond 2^43 elements");
   VTLB_CUDA(ctx, vtlb_launch_early(kern, dim3((unsigned)ctas), dim3(256), 0, ctx->stream, (const float*)d_W, V, (uint32_t)D,
-                                   (const int32_t*)d_ids_i32, total, scale, (float*)d_Y, (int)y_aligned, m, bad));
+                                   (const int32_t*)d_ids_i32, total, scale, (float*)d_Y, blocks_of_w, y_aligned, m, bad));
   VTLB_LAUNCHED(ctx);
   if (check) {
     uint32_t flag = 0;
