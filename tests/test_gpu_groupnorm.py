@@ -226,6 +226,23 @@ def test_pointers_off_the_16_byte_grid(dev, C, G):
         b.free()
 
 
+@pytest.mark.parametrize("B,S,C,G", [(3, 1, 64, 2), (2, 5, 8, 1)])
+def test_eps_below_the_smallest_f32(dev, B, S, C, G):
+    """rstd = 1 / sqrt(eps) of constant groups, where eps itself is no f32.  With several positions the variance comes from
+    sums in 64 bits, of which it loses some 2^-53 of the mean square, 9: more than this eps, so there only the bound that
+    counts it (512 * D53 * mean^2 in forward_bounds) can hold."""
+    h = np.full((B, S, C), 3, np.float32)
+    x = dev.to_device(h)
+    y, mean, rstd = dev.zeros((B, S, C)), dev.zeros((B, G)), dev.zeros((B, G))
+    dev.groupnorm_fwd_f32(x, B, S, C, G, None, None, 1e-60, ref.NONE, y, mean, rstd)
+    assert (y.numpy() == 0).all() and (mean.numpy() == 3).all()
+    want = ref.groupnorm(h, G, None, None, 1e-60, ref.NONE)
+    t = 1e30 * 2 * U if S == 1 else forward_bounds(h, G, None, None, 1e-60, ref.NONE, *want)[2]
+    assert (np.abs(rstd.numpy().astype(np.float64) - 1e30) <= t).all()
+    for b in (x, y, mean, rstd):
+        b.free()
+
+
 def test_layer_norm_is_one_group_of_one_position(dev):
     rng = np.random.default_rng(10)
     x = rng.standard_normal((70, 1, 256)).astype(np.float32)
