@@ -109,7 +109,8 @@ __device__ __forceinline__ GnVec<VEC> vneg(const GnVec<VEC>& a) {
 }
 
 // e = exp(-z) and s = 1 / (1 + e); expf and IEEE division take some twenty instructions, more than the rest of the forward
-// kernel per element.  e is held at 2^126 at most, so that e * s stays a number: below z = -87.3 s is 1.2e-38.
+// kernel per element.  e is held at 2^127 at most, whose reciprocal, a subnormal, is flushed to zero: for z below -87.3 s
+// and e * s are zero, as they are but for 1e-38, whatever multiple of z they are multiplied by.
 // In half steps (2^-24, relative): the product z * log2(e) is rounded, which weighs |z| in the power; the approximate
 // power is good to 2 ulp, the sum to half an ulp, the approximate reciprocal to 1 ulp: |z| + 4 + 1 + 2 for s, less for
 // z > 0.  (A power on the FMA pipe for one element of four and one reciprocal for two were tried: no gain, the kernels
@@ -118,7 +119,7 @@ template <int VEC>
 __device__ __forceinline__ void vlogistic(const GnVec<VEC>& z, GnVec<VEC>& e, GnVec<VEC>& s) {
   e = vmul(z, gn_splat<VEC>(-1.4426950408889634f));
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.e[k]) : "f"(fminf(e.e[k], 126.0f)));
+  for (int k = 0; k < VEC; ++k) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.e[k]) : "f"(fminf(e.e[k], 127.0f)));
   s = vadd(e, gn_splat<VEC>(1.0f));
 #pragma unroll
   for (int k = 0; k < VEC; ++k) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.e[k]) : "f"(s.e[k]));
