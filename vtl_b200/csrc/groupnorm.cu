@@ -199,7 +199,7 @@ __device__ __forceinline__ float2 gn_row_sum(float2 v, float2* sm, int turn) {  
 
 template <int ACT, int VEC, int L, int PER>
 __global__ void __launch_bounds__(kGnRowThreads) gn_rows_fwd_kernel(const float* x, const float* gamma, const float* beta, GnDims d,
-                                                                    float eps, float* y, float* mean_out, float* rstd_out) {
+                                                                    float eps, double part, float* y, float* mean_out, float* rstd_out) {
   __shared__ float2 sm[2 * kGnRowThreads / 32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -218,8 +218,7 @@ __global__ void __launch_bounds__(kGnRowThreads) gn_rows_fwd_kernel(const float*
   float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
   for (int k = 0; k < VEC; ++k) s.x += s1.e[k];
-  const float part = 1.0f / (float)W;
-  const float m0 = gn_row_sum<L>(s, sm, 0).x * part;  // the mean but for its rounding; then the distances from it
+  const float m0 = gn_row_sum<L>(s, sm, 0).x * (float)part;  // the mean but for its rounding; then the distances from it
   const GnVec<VEC> minus0 = gn_splat<VEC>(-m0);
   s1 = gn_splat<VEC>(0.0f);
 #pragma unroll
@@ -233,8 +232,9 @@ __global__ void __launch_bounds__(kGnRowThreads) gn_rows_fwd_kernel(const float*
 #pragma unroll
   for (int k = 0; k < VEC; ++k) s.x += s1.e[k], s.y += s2.e[k];
   s = gn_row_sum<L>(s, sm, 1);
-  const float off = s.x * part, var = fmaf(s.y, part, -off * off);
-  const float mu = m0 + off, rs = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);
+  // (in f64: of values that hardly vary the distances are exact, and all of them may be what m0 was rounded by)
+  const double off = (double)s.x * part, var = fma((double)s.y, part, -off * off);
+  const float mu = (float)((double)m0 + off), rs = 1.0f / sqrtf((float)(var < 0.0 ? 0.0 : var) + eps);
   if (!in) return;
   if (t == 0) mean_out[row] = mu, rstd_out[row] = rs;
   const GnVec<VEC> minus = gn_splat<VEC>(-mu), scale = gn_splat<VEC>(rs);
@@ -346,7 +346,9 @@ __global__ void __launch_bounds__(kGnRowThreads, PER > 4 ? 1 : 2)
 
 // ---------------------------------------------------------------- groups of any size
 // Two passes over x (and g): sums per channel and chunk of positions, then the result.  CTAs take 256 threads as
-// `cols` pieces of VEC channels by 256 / cols rows.  Sums are f64: sum and sum of squares forward, dz and dz * h backward.
+// `cols` pieces of VEC channels by 256 / cols rows.  Sums are f64: forward of the distances from the group's first value,
+// and of their squares (of the values themselves the variance would lose 2^-53 of the mean square, 1e-4 at a mean of 1e6),
+// rows that are asked for together by way of the first of them in f32; backward dz and dz * h.
 // Bound by HBM, 12 bytes per element forward, 20 backward, less what of x and g still lies in L2 for the second pass.
 // Ten samples of 20000 positions by one group of 64 channels: 35 us forward, 64 us backward, 4.4 and 4 TB/s of those bytes.
 // Sixty of 4000 by two groups of 31 (rows on no 16-byte boundary, one channel a load): 48 and 86 us, 3.7 and 3.5 TB/s.
@@ -395,28 +397,46 @@ __global__ void __launch_bounds__(256) gn_sums_kernel(const float* x, const floa
     }
     const GnVec<VEC> minus = vneg(mu);
     const size_t base = (size_t)b * d.S * d.C + c;
-    for (int r = chunk * t.rows + lane; r < r1; r += gn_ahead<VEC> * lanes) {
+    double first[VEC] = {};
+    for (int r = chunk * t.rows + lane, start = r; r < r1; r += gn_ahead<VEC> * lanes) {
       GnVec<VEC> vx[gn_ahead<VEC>], vg[gn_ahead<VEC>];
       gn_rows<VEC>(vx, x + base, r, r1, lanes, d.C);
-      if (BWD) gn_rows<VEC>(vg, g + base, r, r1, lanes, d.C);
+      if (BWD) {
+        gn_rows<VEC>(vg, g + base, r, r1, lanes, d.C);
 #pragma unroll
-      for (int i = 0; i < gn_ahead<VEC>; ++i) {
-        if (r + i * lanes >= r1) break;
-        const GnVec<VEC> v = vx[i];
-        if (BWD) {
-          const GnVec<VEC> h = vmul(vadd(v, minus), rs);
-          const GnVec<VEC> dz = act_bwd<ACT>(vg[i], v, mu, rs, ga, be, h);
+        for (int i = 0; i < gn_ahead<VEC>; ++i) {
+          if (r + i * lanes >= r1) break;
+          const GnVec<VEC> h = vmul(vadd(vx[i], minus), rs);
+          const GnVec<VEC> dz = act_bwd<ACT>(vg[i], vx[i], mu, rs, ga, be, h);
 #pragma unroll
           for (int k = 0; k < VEC; ++k) {
             acc[k].x += (double)dz.e[k];
             acc[k].y = fma((double)dz.e[k], (double)h.e[k], acc[k].y);
           }
-        } else {
+        }
+      } else {
+        if (r == start) {
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) {
-            acc[k].x += (double)v.e[k];
-            acc[k].y = fma((double)v.e[k], (double)v.e[k], acc[k].y);
-          }
+          for (int k = 0; k < VEC; ++k) first[k] = (double)x[(size_t)b * d.S * d.C + (c + k) / d.width * d.width];
+        }
+        // Distances from the first of these rows, `off` from the group's.  (Where that row is far from the others, its
+        // own distance from the mean counts for more than what theirs from it are rounded by.)
+        const GnVec<VEC> from = vneg(vx[0]);
+        GnVec<VEC> s1 = gn_splat<VEC>(0.0f), s2 = s1;
+        float n = 1.0f;
+#pragma unroll
+        for (int i = 1; i < gn_ahead<VEC>; ++i) {
+          if (r + i * lanes >= r1) break;
+          const GnVec<VEC> e = vadd(vx[i], from);
+          s1 = vadd(s1, e);
+          s2 = vfma(e, e, s2);
+          n += 1.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const double off = (double)vx[0].e[k] - first[k], all = (double)n * off, rest = (double)s1.e[k];
+          acc[k].x += all + rest;
+          acc[k].y += fma(all + (rest + rest), off, (double)s2.e[k]);
         }
       }
     }
@@ -436,8 +456,8 @@ __global__ void __launch_bounds__(256) gn_sums_kernel(const float* x, const floa
 // One CTA per (sample, group), T threads: the sums over chunks and channels, in a fixed order.  (With a warp for each, which
 // also divided to find its channels, 79 chunks of 64 channels took 40 us, longer than both passes over x.)
 template <bool BWD>
-__global__ void __launch_bounds__(256) gn_groups_kernel(const double2* partial, int chunks, GnDims d, const float* gamma,
-                                                        double eps, float* mean, float* rstd, float2* coef) {
+__global__ void __launch_bounds__(256) gn_groups_kernel(const double2* partial, int chunks, GnDims d, const float* x,
+                                                        const float* gamma, double eps, float* mean, float* rstd, float2* coef) {
   __shared__ double2 sm[8];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -446,6 +466,7 @@ __global__ void __launch_bounds__(256) gn_groups_kernel(const double2* partial, 
   const int down = T / d.width, along = T % d.width;  // from one entry of a thread to its next
   int row = threadIdx.x / d.width, col = threadIdx.x % d.width;
   double s0 = 0.0, s1 = 0.0;
+  const float first = BWD ? 0.0f : x[(size_t)b * d.S * d.C + grp * d.width];
   while (row < chunks) {
     double2 p[8];
     double w[8];
@@ -469,8 +490,8 @@ __global__ void __launch_bounds__(256) gn_groups_kernel(const double2* partial, 
   if (BWD) {
     coef[k] = make_float2((float)(s0 / n), (float)(s1 / n));
   } else {
-    const double mu = s0 / n, var = s1 / n - mu * mu;
-    mean[k] = (float)mu;
+    const double off = s0 / n, var = s1 / n - off * off;
+    mean[k] = (float)((double)first + off);
     rstd[k] = (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + eps));
   }
 }
@@ -558,6 +579,7 @@ struct GnTile {
   unsigned units;  // B * slabs
   uint32_t zero;   // 0, unknown to the compiler (gn_after)
   int boxes, box_rows;  // of a CTA's piece as the tensor map cuts it
+  bool in_place;        // y lies over x
 };
 
 // How a CTA's piece of a slab lies on its threads.  The same for all slabs but a narrower last one, so the divisions
@@ -763,6 +785,54 @@ __device__ __forceinline__ void gn_take(GnVec<VEC> (&v)[VPT], const float* slots
   }
 }
 
+// The groups of units that are marked by a negative rstd once more, each by one CTA, behind the barrier of the cluster: sums
+// in f64 of the distances from the mean that was found, so that a constant group's variance is zero but for 2^-53 of the
+// square of what that mean is rounded by.  x is still there: where y lies over it, marked units were not written.  Not
+// unrolled, so that the way that units take as a rule keeps its registers; the check for marks at a kernel's end is all that
+// it pays.
+template <int ACT, int T>
+__device__ __forceinline__ void gn_look_again(const float* x, const float* gamma, const float* beta, const GnTile& t, int rank, int ctas,
+                                           double eps, float* y, float* mean_out, float* rstd_out, double2* sm) {
+  __syncthreads();
+  const int tid = threadIdx.x, W = t.d.width;
+  const int n = t.d.S * W;  // (at most what a cluster holds)
+  const GnUnit stride = gn_first(t, gridDim.x / ctas);
+  for (GnUnit u = gn_first(t, blockIdx.x / ctas); u.unit < t.units; u = gn_next(t, u, stride)) {
+    for (int g = rank; g < gn_groups(t, u); g += ctas) {
+      const size_t k = (size_t)u.b * t.d.G + u.slab * t.groups + g;
+      if (!(*(volatile float*)&rstd_out[k] < 0.0f)) continue;  // (the same for all threads: one writes it, behind a barrier)
+      const size_t base = gn_base(t, u) + (size_t)g * W;
+      const double near = (double)*(volatile float*)&mean_out[k];
+      double2 s = make_double2(0.0, 0.0);
+#pragma unroll 1
+      for (int e = tid; e < n; e += T) {
+        const double v = (double)x[base + (size_t)(e / W) * t.d.C + e % W] - near;
+        s.x += v, s.y = fma(v, v, s.y);
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
+      if ((tid & 31) == 0) sm[tid >> 5] = s;
+      __syncthreads();
+      s = sm[0];
+#pragma unroll 1
+      for (int q = 1; q < T / 32; ++q) s.x += sm[q].x, s.y += sm[q].y;
+      const double off = s.x / (double)n, var = s.y / (double)n - off * off;
+      const float mu = (float)(near + off), rs = inv_sqrt((var < 0.0 ? 0.0 : var) + eps);
+      if (tid == 0) mean_out[k] = mu, rstd_out[k] = rs;
+      const int c0 = ((int)u.slab * t.groups + g) * W;
+#pragma unroll 1
+      for (int e = tid; e < n; e += T) {
+        const int c = e % W;
+        const size_t at = base + (size_t)(e / W) * t.d.C + c;
+        GnVec<1> z;
+        z.e[0] = fmaf(x[at] - mu, gamma ? rs * gamma[c0 + c] : rs, beta ? beta[c0 + c] : 0.0f);
+        y[at] = act<ACT>(z).e[0];
+      }
+      __syncthreads();
+    }
+  }
+}
+
 template <int ACT, int VEC, int VPT, bool GROUPED, bool TMA>
 __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads : 1024 / kGnFwdThreads)
     gn_fwd_tile_kernel(const __grid_constant__ CUtensorMap map, const float* x, const float* gamma, const float* beta, GnTile t, double eps, float* y,
@@ -774,6 +844,7 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
   __shared__ double2 sm_pair[T * PAIRS];      // [row lane or warp][entry or group]
   __shared__ GnMail<double2> mail;
   __shared__ float2 sm_stat[kGnMaxGroups];
+  __shared__ unsigned sm_lost;  // the last round in which the sums of a group lost too much
   extern __shared__ __align__(128) float slots[];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
@@ -785,6 +856,7 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
   const bool cq_even = PAIRS == 1 && (cq & (cq - 1)) == 0;
   const double part = 1.0 / ((double)t.d.S * width);
   gn_mail_init(mail);
+  if (tid == 0) sm_lost = ~0u;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the kernel in front is done from here on
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t bar = ptx::smem_u32(&mail.data), box_bytes = (uint32_t)(t.boxes * t.box_rows * t.channels * 4);
@@ -793,10 +865,10 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
       ptx::mbar_arrive_expect_tx(bar, box_bytes);
       gn_fetch_box(slots, &map, t, u, p, bar);
     }
-    if (ctas == 1) __syncthreads();  // (the barrier is ready)
   } else {
     gn_fetch<T, VEC, VPT>(slots, x, t, u, p);
   }
+  if (TMA && ctas == 1) __syncthreads();  // (the barrier is ready)
   if (ctas > 1) cluster.sync();  // everyone's boxes are ready
   for (unsigned round = 0;; ++round) {
     const int turn = round & 1;
@@ -821,43 +893,43 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
           gn_fetch<T, VEC, VPT>(slots, x, t, next, gn_shape<T, VEC>(t, gn_groups(t, next), rank), after);
       }
     }
-    // A thread's own mean K and squared distances from it in f32, then sums of x and x^2 in f64 from them: the variance
-    // loses 2^-53 of the mean square, not 2^-24, and few instructions are f64.
+    // A thread's own mean m, and the sums r and q of the distances from it and of their squares, in f32 (m is rounded, r
+    // says by how much); from these in f64 the sums of x and x^2.  Of these the variance loses some 2^-53 of the mean
+    // square: where that may be more than 2^-27 of variance and eps (a constant group of 30 at an eps of 1e-5), the unit is
+    // left to gn_look_again.  (Sums of the distances from a value that all threads know lose nothing, but it has to
+    // be brought and subtracted for every unit: 26 samples of 129 x 896 by 16 groups 12.0 us, this way 11.6, sums without
+    // care 11.0; 32 of 64 x 64 x 512 98, 96 and 94.)
     double2 acc[PAIRS];
+    {
+      const float n = (float)(p.rows * PER), part_n = p.rows ? __fdividef(1.0f, n) : 0.0f;
+      GnVec<VEC> m = gn_splat<VEC>(0.0f), r = m, q = m;
 #pragma unroll
-    for (int q = 0; q < PAIRS; ++q) {
-      const float n = (float)(p.rows * PER);
-      float sum = 0.0f, dist = 0.0f, mean;
+      for (int i = 0; i < VPT; ++i) m = vadd(m, v[i]);
       if constexpr (PAIRS == 1) {
-        GnVec<VEC> part = gn_splat<VEC>(0.0f);
+        float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) part = vadd(part, v[i]);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) sum += part.e[k];
-        mean = p.rows ? __fdividef(sum, n) : 0.0f;  // any value near the mean serves
-        const GnVec<VEC> minus = gn_splat<VEC>(-mean);
-        part = gn_splat<VEC>(0.0f);
-#pragma unroll
-        for (int i = 0; i < VPT; ++i)
-          if (i < p.rows) {
-            const GnVec<VEC> e = vadd(v[i], minus);
-            part = vfma(e, e, part);
-          }
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) dist += part.e[k];
+        for (int k = 0; k < VEC; ++k) sum += m.e[k];
+        m = gn_splat<VEC>(sum * part_n);  // any value near the mean serves
       } else {
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) sum += v[i].e[q];
-        mean = p.rows ? __fdividef(sum, n) : 0.0f;
-#pragma unroll
-        for (int i = 0; i < VPT; ++i)
-          if (i < p.rows) {
-            const float e = v[i].e[q] - mean;
-            dist = fmaf(e, e, dist);
-          }
+        m = vmul(m, gn_splat<VEC>(part_n));
       }
-      const double nm = (double)n * (double)mean;
-      acc[q] = make_double2(nm, fma(nm, (double)mean, (double)dist));
+      const GnVec<VEC> minus = vneg(m);
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if (i < p.rows) {
+          const GnVec<VEC> e = vadd(v[i], minus);
+          r = vadd(r, e);
+          q = vfma(e, e, q);
+        }
+#pragma unroll
+      for (int k = 0; k < PAIRS; ++k) {
+        if constexpr (PAIRS == 1) {
+#pragma unroll
+          for (int e = 1; e < VEC; ++e) r.e[0] += r.e[e], q.e[0] += q.e[e];
+        }
+        const double rest = (double)r.e[k], s = fma((double)n, (double)m.e[k], rest);
+        acc[k] = make_double2(s, fma(s + rest, (double)m.e[k], (double)q.e[k]));
+      }
     }
     // The pairs of all rows, per entry (a piece, or a channel of it): by shuffles where a warp holds whole rows.
     const int entries = p.cols * PAIRS, parts = p.even ? T / 32 : p.lanes;  // of a row; rows of sums
@@ -915,17 +987,19 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
     if (tid < p.groups) {
       double2 s = make_double2(0.0, 0.0);
       for (int r = 0; r < ctas; ++r) s.x += mail.box[turn][r][tid].x, s.y += mail.box[turn][r][tid].y;
-      const double mu = s.x * part, var = s.y * part - mu * mu;
-      const float2 st = make_float2((float)mu, inv_sqrt((var < 0.0 ? 0.0 : var) + eps));
+      const double off = s.x * part, var = s.y * part - off * off;
+      const float2 st = make_float2((float)off, inv_sqrt((var < 0.0 ? 0.0 : var) + eps));
       sm_stat[tid] = st;
+      const bool lost = __any_sync(~0u >> (32 - p.groups), fabsf(st.x) * st.y > 8192.0f);
+      if (lost) sm_lost = round;
       if (rank == 0) {
         const size_t k = (size_t)u.b * t.d.G + u.slab * t.groups + tid;
         mean_out[k] = st.x;
-        rstd_out[k] = st.y;
+        rstd_out[k] = lost ? -st.y : st.y;  // (a mark for gn_look_again)
       }
     }
     __syncthreads();
-    if (p.rows) {
+    if (p.rows && !(t.in_place && sm_lost == round)) {
       const int c = (int)u.slab * t.groups * width + p.in_slab + p.col * VEC;
       GnVec<VEC> minus, a, be;
 #pragma unroll
@@ -949,6 +1023,7 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
   }
   if (TMA && p.any) gn_last_copies(mail);
   if (ctas > 1) cluster.sync();  // no CTA leaves while another may still send to it
+  if (__builtin_expect(sm_lost != ~0u, 0)) gn_look_again<ACT, T>(x, gamma, beta, t, (int)cluster.block_rank(), (int)cluster.num_blocks(), eps, y, mean_out, rstd_out, sm_pair);
 }
 
 // Backward.  The channel sums of each CTA go to `sums` [B * rsplit][C] (dz, dz * h) for gn_params_kernel.
@@ -1213,8 +1288,8 @@ cudaError_t bwd_tile(vtlb_ctx* ctx, const GnTile& t, int cluster, Args... args) 
   return cluster_launch(ctx, info, gn_bwd_tile_kernel<ACT, VEC, VPT, GROUPED, TMA>, kGnBwdThreads, t.units, cluster, smem, usual, args...);
 }
 
-GnTile tile_of(const GnDims& d, const GnPlan& p) { return GnTile{d, p.groups, p.slabs, p.csplit, p.channels, p.rows, (unsigned)d.B * (unsigned)p.slabs, 0u,
-                p.boxes, p.box_rows}; }
+GnTile tile_of(const GnDims& d, const GnPlan& p, bool in_place) { return GnTile{d, p.groups, p.slabs, p.csplit, p.channels, p.rows, (unsigned)d.B * (unsigned)p.slabs, 0u,
+                p.boxes, p.box_rows, in_place}; }
 
 int check_dims(vtlb_ctx* ctx, const char* fn, int B, int S, int C, int groups, int act_kind, GnDims* d) {
   if (B <= 0 || S <= 0 || C <= 0 || groups <= 0 || C % groups)
@@ -1254,7 +1329,7 @@ int gn_forward_general(vtlb_ctx* ctx, const float* x, GnDims d, const float* gam
                                    none, t, (double2*)partial));
   VTLB_LAUNCHED(ctx);
   VTLB_CUDA(ctx, vtlb_launch_early(gn_groups_kernel<false>, dim3((unsigned)d.B * d.G), dim3(group_threads(d, chunks)), 0,
-                                   ctx->stream, (const double2*)partial, chunks, d, none, eps, mean, rstd, (float2*)nullptr));
+                                   ctx->stream, (const double2*)partial, chunks, d, x, none, eps, mean, rstd, (float2*)nullptr));
   VTLB_LAUNCHED(ctx);
   VTLB_CUDA(ctx, vtlb_launch_early(gn_apply_kernel<ACT, false, VEC>, grid, dim3(256), 0, ctx->stream, x, none, gamma, beta,
                                    (const float*)mean, (const float*)rstd, (const float2*)nullptr, t, y));
@@ -1284,7 +1359,7 @@ int gn_backward_general(vtlb_ctx* ctx, const float* g, const float* x, GnDims d,
   }
   if (!dx) return VTLB_OK;
   VTLB_CUDA(ctx, vtlb_launch_early(gn_groups_kernel<true>, dim3((unsigned)d.B * d.G), dim3(group_threads(d, chunks)), 0,
-                                   ctx->stream, (const double2*)partial, chunks, d, gamma, 0.0, (float*)nullptr,
+                                   ctx->stream, (const double2*)partial, chunks, d, x, gamma, 0.0, (float*)nullptr,
                                    (float*)nullptr, coef));
   VTLB_LAUNCHED(ctx);
   VTLB_CUDA(ctx, vtlb_launch_early(gn_apply_kernel<ACT, true, VEC>, grid, dim3(256), 0, ctx->stream, x, g, gamma, beta, mean,
@@ -1315,7 +1390,7 @@ int gn_forward_rows(vtlb_ctx* ctx, int threads, int per, const float* x, GnDims 
                               : gn_rows_fwd_kernel<ACT, VEC, 256, 8>;
   const int places = kGnRowThreads / threads;
   const size_t ctas = ((size_t)d.B * d.G + places - 1) / places;
-  VTLB_CUDA(ctx, vtlb_launch_early(kern, dim3((unsigned)ctas), dim3(kGnRowThreads), 0, ctx->stream, x, gamma, beta, d, (float)eps, y, mean, rstd));
+  VTLB_CUDA(ctx, vtlb_launch_early(kern, dim3((unsigned)ctas), dim3(kGnRowThreads), 0, ctx->stream, x, gamma, beta, d, (float)eps, 1.0 / (double)d.width, y, mean, rstd));
   VTLB_LAUNCHED(ctx);
   return VTLB_OK;
 }
@@ -1363,7 +1438,7 @@ int gn_forward(vtlb_ctx* ctx, const float* x, GnDims d, const float* gamma, cons
   }
   const GnPlan plan = gn_plan(d.B, d.S, d.C, d.G, vtlb_aligned16(x) && vtlb_aligned16(y), kGnFwdThreads, 4, 16, ctx->sm_count);
   if (plan.on_chip) {
-    const GnTile t = tile_of(d, plan);
+    const GnTile t = tile_of(d, plan, x == y);
     const int cluster = plan.csplit * plan.rsplit;
     const bool grouped = d.width % 4 == 0;
     CUtensorMap map = {};
@@ -1407,7 +1482,7 @@ int gn_backward(vtlb_ctx* ctx, const float* g, const float* x, GnDims d, const f
   vtlb_workspace ws(ctx);
   void* scratch = nullptr;
   if (plan.on_chip) {
-    const GnTile t = tile_of(d, plan);
+    const GnTile t = tile_of(d, plan, false);
     const int cluster = plan.csplit * plan.rsplit;
     const int rows = d.B * plan.rsplit;
     if (dgamma || dbeta)
