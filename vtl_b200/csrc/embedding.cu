@@ -341,7 +341,7 @@ __device__ __forceinline__ void zero_absent(const EmbGrad& p, size_t row0, size_
 #pragma unroll 4
         for (int c = lane; c < body; c += 32) out[c] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (lane < head) row[lane] = 0.0f;
-        if (end + lane < p.D) row[end + lane] = 0.0f;
+        if (lane < p.D - end) row[end + lane] = 0.0f;
       }
     } else {  // element by element, a warp's 32 next to one another
       float* out = p.dW + r0 * p.D;
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(256, 4) embedding_few_kernel(EmbGrad p, vtlb_m
           const size_t row = (size_t)rows[k + u] * p.D;
           if (VEC) {
             if (own) v[u] = __ldg(reinterpret_cast<const float4*>(p.g + row) + c);
-          } else if (4 * c - (int)(row & 3) < p.D) {
+          } else if (4u * (uint32_t)c < (uint32_t)p.D + (uint32_t)(row & 3)) {
             v[u] = block_load(p.g, (row & ~(size_t)3) + 4 * (size_t)c, total, aligned);
           }
         }
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(256, DROP ? 3 : 4) embedding_sums_kernel(EmbGr
         const size_t row = (size_t)window[k + u - w0].y * p.D;
         if (VEC)
           v[u] = __ldg(reinterpret_cast<const float4*>(p.g + row) + c);
-        else if (4 * c - (int)(row & 3) < p.D)
+        else if (4u * (uint32_t)c < (uint32_t)p.D + (uint32_t)(row & 3))
           v[u] = block_load(p.g, (row & ~(size_t)3) + 4 * (size_t)c, total, aligned);
       }
     }
@@ -671,7 +671,7 @@ int embedding_bwd_batch(vtlb_ctx* ctx, vtlb_workspace& ws, const float* g, const
                         int D, float scale, const vtlb_mask& m, float* dW, int accumulate) {
   EmbGrad p = {};
   p.g = g, p.ids = ids, p.dW = dW, p.first_pos = first_pos, p.n = n, p.V = V, p.D = D, p.scale = scale, p.accumulate = accumulate;
-  p.cols = (D + 3) / 4;
+  p.cols = D / 4 + (D % 4 != 0);
   const bool vec = D % 4 == 0 && vtlb_aligned16(g) && vtlb_aligned16(dW);
   // Each zeroing CTA reads all ids, so they are no more than write four times what all of them read, but two per SM
   // where there are 32 KB to write for each.
