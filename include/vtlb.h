@@ -438,9 +438,9 @@ int vtlb_ids_from_f32(vtlb_ctx* ctx, const void* d_src, size_t n, void* d_ids_i3
  * the statistics; the backward pass reads them, and x, and recomputes z.  d_y may be d_x where x is not needed again.
  * Backward, dz = g * act'(z): dgamma[c] = sum dz * h, dbeta[c] = sum dz over samples and positions,
  * dx = rstd * (gamma dz - mean(gamma dz) - h * mean(gamma dz h)), the means over the group; any output may be NULL,
- * d_dx may be d_g or d_x.  Other buffers may not overlap.  B * S and B * groups go to 2^31 - 1, S to 65535 * 256.  The
- * backward pass takes up to 8 C B min(S, 8) bytes of workspace for the sums of dgamma and dbeta (16 C B per 32 to 256
- * positions for groups too large for the chip). */
+ * d_dx may be d_g or d_x.  Other buffers may not overlap.  B * S and B * groups go to 2^31 - 1, S to 65535 * 256, C to
+ * 2^31 - 1024.  The backward pass takes up to 8 C B min(S, 8) bytes of workspace for the sums of dgamma and dbeta (16 C B
+ * per 32 to 256 positions for groups too large for the chip). */
 #define VTLB_ACT_NONE 0
 #define VTLB_ACT_RELU 1
 #define VTLB_ACT_SILU 2

@@ -4,8 +4,6 @@
 // Backward, with dz = g * act'(z) and n = S * C/groups:
 //   dgamma_c = sum over samples and positions of dz * h,   dbeta_c = sum of dz,
 //   dx = rstd * (gamma_c * dz - (sum gamma dz) / n - h * (sum gamma dz h) / n), the sums over the group.
-#include <climits>
-
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -1296,6 +1294,7 @@ int check_dims(vtlb_ctx* ctx, const char* fn, int B, int S, int C, int groups, i
     return vtlb_fail(ctx, VTLB_EINVAL, "%s: bad shape B=%d S=%d C=%d groups=%d", fn, B, S, C, groups);
   if (act_kind != VTLB_ACT_NONE && act_kind != VTLB_ACT_RELU && act_kind != VTLB_ACT_SILU)
     return vtlb_fail(ctx, VTLB_EINVAL, "%s: unknown activation %d", fn, act_kind);
+  if (C > kGnMaxChannels) return vtlb_fail(ctx, VTLB_EINVAL, "%s: C=%d: channels go to %d", fn, C, kGnMaxChannels);
   // (CTAs, units and rows of sums are counted in 31 bits; a sample's chunks are a grid's second dimension)
   if ((long long)B * groups > INT_MAX || (long long)B * S > INT_MAX || S > 65535 * kRows)
     return vtlb_fail(ctx, VTLB_EINVAL, "%s: B=%d S=%d groups=%d: B * S and B * groups go to 2^31 - 1, S to %d", fn, B, S, groups, 65535 * kRows);

@@ -1,5 +1,6 @@
 // How group norm cuts its work (groupnorm.cu); plain C++, so that it can be checked for every size without a GPU.
 #pragma once
+#include <climits>
 
 // Channels are taken in slabs of whole groups.  A thread-block cluster owns one slab of one sample; its CTAs cut the
 // positions into `rsplit` equal stretches (and a slab too wide for the threads of one CTA into `csplit` pieces), and
@@ -18,6 +19,7 @@ struct GnPlan {
 };
 
 constexpr int kGnFwdThreads = 512, kGnBwdThreads = 256, kGnMaxGroups = 32, kGnMaxCluster = 8;
+constexpr int kGnMaxChannels = INT_MAX - 1023;  // a CTA's channels, up to 1024, are rounded up and counted in ints
 constexpr int kGnMaxSmem = 150 << 10;  // for the pieces; with the kernels' static arrays within 227 KB
 
 // The kernels have `middle` and `most` rows per thread to choose from, and one; a row's pieces take a power of two of the
