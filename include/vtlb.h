@@ -54,8 +54,9 @@ const char* vtlb_last_error(vtlb_ctx* ctx); /* ctx may be NULL: process-wide las
 int vtlb_check_status(vtlb_ctx* ctx, uint32_t* status);
 /* Self-test of the bounded device-side waits (no counterpart in the reference, whose GPU calls
  * block on the default stream): launches a one-CTA kernel that waits on an mbarrier for at most
- * limit_ns (1 ns .. 100 ms) with the same wait routine as the tcgen05 kernels.  arrive != 0: a
- * second thread arrives and the wait is satisfied.  arrive == 0: nobody arrives, the wait gives
+ * limit_ns (1 ns .. 100 ms) with the same wait routine as the tcgen05 kernels.  arrive == 2: a wait
+ * as group norm's kernels have it, for which nobody arrives.  Else arrive != 0: a second thread
+ * arrives and the wait is satisfied.  arrive == 0: nobody arrives, the wait gives
  * up, the kernel returns normally and sets the status word, so the next vtlb_check_status
  * returns VTLB_ETIMEOUT -- the failure path of a stuck pipeline, without anything being stuck. */
 int vtlb_wait_probe(vtlb_ctx* ctx, uint64_t limit_ns, int arrive);

@@ -683,23 +683,21 @@ __device__ __forceinline__ void gn_send(GnMail<T>& m, int turn, int rank, int ct
   const uint32_t to = ptx::smem_u32(&m.box[turn][rank][g]), bar = ptx::smem_u32(&m.full[turn]);
   for (int r = 0; r < ctas; ++r) gn_post(gn_remote(to, r), gn_remote(bar, r), v);
 }
-// The first warp waits for the sums of all CTAs (at most two seconds: then the status word says so, and the results
-// are not valid).  `round` counts the units of this CTA.
+// The first warp waits for the sums of all CTAs (at most two seconds: then the status word says so at the kernel's
+// end, and the results are not valid).  `round` counts the units of this CTA.
 template <typename T>
-__device__ __forceinline__ void gn_receive(GnMail<T>& m, int turn, unsigned round, int ctas, int groups, uint32_t* status) {
+__device__ __forceinline__ void gn_receive(GnMail<T>& m, int turn, unsigned round, int ctas, int groups) {
   const uint32_t bar = ptx::smem_u32(&m.full[turn]);
   if (threadIdx.x == 0) ptx::mbar_arrive_expect_tx(bar, (uint32_t)(ctas * groups * sizeof(T)));
   __syncwarp();
-  if (!ptx::mbar_wait_bounded(bar, (round >> 1) & 1, &m.abort, 2000000000ull) && (threadIdx.x & 31) == 0)
-    atomicOr(status, VTLB_ST_NORM_TIMEOUT);
+  ptx::mbar_wait_bounded(bar, (round >> 1) & 1, &m.abort, 2000000000ull);
   __syncwarp();  // lanes leave the wait one by one
 }
 
 // Waits, for at most two seconds, until the slots are filled for unit number `round` of this CTA.
 template <typename T>
-__device__ __forceinline__ void gn_wait_data(GnMail<T>& m, unsigned round, uint32_t* status) {
-  if (!ptx::mbar_wait_bounded(ptx::smem_u32(&m.data), round & 1, &m.abort, 2000000000ull) && threadIdx.x == 0)
-    atomicOr(status, VTLB_ST_NORM_TIMEOUT);
+__device__ __forceinline__ void gn_wait_data(GnMail<T>& m, unsigned round) {
+  ptx::mbar_wait_bounded(ptx::smem_u32(&m.data), round & 1, &m.abort, 2000000000ull);
   __syncwarp();  // lanes leave the wait one by one, and a warp that is not whole counts as a whole one at a barrier
 }
 
@@ -873,7 +871,7 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
     GnVec<VEC> v[VPT];
     const GnUnit next = gn_next(t, u, stride);
     if constexpr (TMA) {
-      if (p.any) gn_wait_data(mail, round, status);
+      if (p.any) gn_wait_data(mail, round);
       gn_take_box(v, slots, t, p);
       gn_slots_read();
       if (tid == 0 && p.any && next.unit < t.units && !mail.abort) {
@@ -981,7 +979,7 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
       }
       if (ctas == 1) __syncthreads();
     }
-    if (warp == 0 && ctas > 1) gn_receive(mail, turn, round, ctas, p.groups, status);
+    if (warp == 0 && ctas > 1) gn_receive(mail, turn, round, ctas, p.groups);
     if (tid < p.groups) {
       double2 s = make_double2(0.0, 0.0);
       for (int r = 0; r < ctas; ++r) s.x += mail.box[turn][r][tid].x, s.y += mail.box[turn][r][tid].y;
@@ -1019,6 +1017,7 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
     u = next;
     if (gn_groups(t, u) != p.groups) p = gn_shape<T, VEC>(t, gn_groups(t, u), rank);
   }
+  if (TMA || ctas > 1) ptx::report_abort(&mail.abort, status, VTLB_ST_NORM_TIMEOUT);  // whichever thread's wait it was
   if (TMA && p.any) gn_last_copies(mail);
   if (ctas > 1) cluster.sync();  // no CTA leaves while another may still send to it
   if (__builtin_expect(sm_lost != ~0u, 0)) gn_look_again<ACT, T>(x, gamma, beta, t, (int)cluster.block_rank(), (int)cluster.num_blocks(), eps, y, mean_out, rstd_out, sm_pair);
@@ -1096,7 +1095,7 @@ __global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads :
       }
       uint32_t after = 0;
       if constexpr (TMA) {
-        if (p.any) gn_wait_data(mail, round, status);
+        if (p.any) gn_wait_data(mail, round);
         gn_take_box(vx, slots, t, p);
         gn_take_box(vg, slots_g, t, p);
         gn_slots_read();
@@ -1181,7 +1180,7 @@ __global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads :
         }
       }
       if (ctas == 1) __syncthreads();
-      if (warp == 0 && ctas > 1) gn_receive(mail, turn, round, ctas, p.groups, status);
+      if (warp == 0 && ctas > 1) gn_receive(mail, turn, round, ctas, p.groups);
       if (tid < p.groups) {
         float2 s = make_float2(0.f, 0.f);
         for (int r = 0; r < ctas; ++r) s.x += mail.box[turn][r][tid].x, s.y += mail.box[turn][r][tid].y;
@@ -1211,6 +1210,7 @@ __global__ void __launch_bounds__(kGnBwdThreads, VPT > 4 ? 512 / kGnBwdThreads :
     u = next;
     if (gn_groups(t, u) != p.groups) p = gn_shape<T, VEC>(t, gn_groups(t, u), rank);
   }
+  if (TMA || ctas > 1) ptx::report_abort(&mail.abort, status, VTLB_ST_NORM_TIMEOUT);  // whichever thread's wait it was
   if (TMA && p.any) gn_last_copies(mail);
   if (ctas > 1) cluster.sync();
 }

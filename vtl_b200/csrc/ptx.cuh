@@ -75,6 +75,12 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
   }
 }
 
+// Behind the last wait of a CTA (all of its threads): whether a wait of any thread ran out goes to the status word.
+__device__ __forceinline__ void report_abort(const volatile uint32_t* abort_flag, uint32_t* status, uint32_t bit) {
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(status, bit);
+}
+
 // ---------------------------------------------------------------- TMA
 // 2-D tiled load global -> shared of this CTA; completion is signalled on `bar`
 // as transaction bytes.  x is the innermost (contiguous) coordinate in elements

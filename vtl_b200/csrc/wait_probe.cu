@@ -5,6 +5,8 @@
 // ORs VTLB_ST_GEMM_TIMEOUT into the status word exactly as the GEMM kernels' teardown does --
 // so the path from a wait that ran out to VTLB_ETIMEOUT on the host can be exercised without a
 // kernel that is actually stuck.  The kernel always returns; the context stays usable.
+// `arrive` = 2 is the same for group norm, whose threads wait each for itself: one that is not the first waits for nobody, the
+// first does not wait, and what the CTA reports is VTLB_ST_NORM_TIMEOUT.
 #include "common.cuh"
 #include "ptx.cuh"
 
@@ -21,6 +23,11 @@ __global__ void __launch_bounds__(64) wait_probe_kernel(uint64_t limit_ns, int a
     ptx::fence_barrier_init();
   }
   __syncthreads();
+  if (arrive == 2) {
+    if (threadIdx.x == 32) ptx::mbar_wait_bounded(bar, 0, abort_flag, limit_ns);
+    ptx::report_abort(&abort_word, status, VTLB_ST_NORM_TIMEOUT);
+    return;
+  }
   if (threadIdx.x == 32 && arrive) ptx::mbar_arrive(bar);
   if (threadIdx.x == 0) ptx::mbar_wait_bounded(bar, 0, abort_flag, limit_ns);  // raises abort_word on expiry
   __syncthreads();
