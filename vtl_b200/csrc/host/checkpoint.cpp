@@ -3,7 +3,9 @@
 // encode_tensor / decode_tensor (:421-473).  The tensor payloads (f64 big-endian, base64) are
 // produced and consumed on the device (vtlb_ckpt_encode_f32 / vtlb_ckpt_decode_f32); the host
 // only frames them in JSON.  Optimizer moments, which the reference leaves out (its loader is
-// commented out, :376-417), are written under that loader's key names.
+// commented out, :376-417), are written under that loader's key names.  A dropout layer's entry of
+// layer_data has, beside its empty weights, "state": {"seed", "step"} (decimal text), so that a run
+// that is resumed draws the masks that the run it continues would have drawn.
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -276,6 +278,26 @@ const char* weight_key(const std::string& layer_type, size_t j, std::string& scr
   return scratch.c_str();
 }
 
+// A layer's state out of its entry; a checkpoint written without it leaves the layer's.
+void load_state(Layer& l, const JValue& entry, size_t i) {
+  const JValue* saved = entry.get("state");
+  if (!saved) return;
+  std::vector<std::pair<uint64_t*, uint64_t>> values;
+  for (const auto& field : l.state()) {
+    const JValue* v = saved->get(field.first);
+    uint64_t n = 0;
+    bool good = v && v->kind == JValue::Str && !v->str.empty();
+    for (size_t k = 0; good && k < v->str.size(); ++k) {
+      const unsigned digit = (unsigned char)v->str[k] - '0';
+      good = digit <= 9 && n <= (UINT64_MAX - digit) / 10;
+      n = n * 10 + digit;
+    }
+    if (!good) throw Error(VTLB_EINVAL, "checkpoint: bad state '" + field.first + "' of layer " + std::to_string(i));
+    values.emplace_back(field.second, n);
+  }
+  for (const auto& v : values) *v.first = v.second;
+}
+
 JValue parse_model(const std::string& path) {
   const std::string text = read_file(path);
   JValue model = JParser(text).parse();
@@ -319,7 +341,14 @@ void Sequential::save_checkpoint(const std::string& path, int epoch, double loss
       layer_data += ':';
       json_string(layer_data, encode_tensor(vars[j]->value));
     }
-    layer_data += "}}";
+    layer_data += '}';
+    const auto state = l->state();
+    for (size_t j = 0; j < state.size(); ++j) {
+      layer_data += j ? "," : ",\"state\":{";
+      json_string(layer_data, state[j].first);
+      layer_data += ":\"" + std::to_string(*state[j].second) + '"';
+    }
+    layer_data += state.empty() ? "}" : "}}";
   }
   layer_defs += ']';
   layer_data += ']';
@@ -392,6 +421,7 @@ void Sequential::load_weights(const std::string& path, AdamOptimizer* opt) {
       if (!enc) throw Error(VTLB_EINVAL, "Missing weight " + key + " for layer " + std::to_string(i));
       decode_tensor_into(enc->str, vars[j]->value);
     }
+    load_state(*layers[i], data.arr[i], i);
   }
   if (opt) {
     const JValue& o = model.at("optimizer");

@@ -183,6 +183,8 @@ struct Layer {
   // map its builder registers (nn/models/sequential_info.v:40-215), in insertion order
   virtual const char* type_name() const = 0;
   virtual std::vector<std::pair<std::string, int>> config() const { return {}; }
+  // what a resumed run needs beside the weights; a checkpoint keeps it as decimal text (a JSON number holds 53 bits)
+  virtual std::vector<std::pair<std::string, uint64_t*>> state() { return {}; }
 };
 
 // nn/layers/input.v
@@ -343,6 +345,7 @@ struct DropoutLayer : Layer {
   std::vector<int> output_shape() const override { return shape; }
   const char* kind() const override { return "dropout"; }
   const char* type_name() const override { return "DropoutLayer"; }
+  std::vector<std::pair<std::string, uint64_t*>> state() override { return {{"seed", &seed}, {"step", &step}}; }
   std::vector<std::pair<std::string, int>> config() const override { return {{"prob_millionths", (int)(p * 1e6 + 0.5)}}; }
 };
 

@@ -222,7 +222,8 @@ class Model:
         _ck(self.lib.vtlh_model_groupnorm(self.h, int(groups), float(eps), {"none": 0, "relu": 1, "silu": 2}[activation]))
 
     def dropout_state(self, dropout_index):
-        """(key, next step) of a dropout layer: with set_dropout_state, what it takes to repeat or resume its masks."""
+        """(key, next step) of a dropout layer: with set_dropout_state, what it takes to repeat its masks.  A checkpoint
+        holds both."""
         seed, step = C.c_ulonglong(0), C.c_ulonglong(0)
         _ck(self.lib.vtlh_model_get_dropout_state(self.h, int(dropout_index), C.byref(seed), C.byref(step)))
         return seed.value, step.value
