@@ -100,3 +100,16 @@ def test_keys_and_steps_of_64_bits(tmp_path):
     assert m.dropout_state(0) == (2**64 - 1, 2**63 + 1)
     m.close()
     s.close()
+
+
+def test_a_checkpoint_tells_scale_eps_and_probability(tmp_path):
+    path = str(tmp_path / "c.json")
+    s = session(5)
+    m = model(s)
+    m.save_checkpoint(path, 0, 0.0)
+    config = [layer["config"] for layer in json.load(open(path))["layers"]]
+    assert config[1]["scale"] == 1.5 and config[1]["vocabulary"] == V and config[1]["dim"] == D
+    assert config[2]["prob"] == 0.3 and config[5]["prob"] == 0.123456789
+    assert config[3]["eps"] == 1e-3 and config[3]["num_groups"] == 2 and config[3]["activation"] == 2
+    m.close()
+    s.close()

@@ -331,6 +331,12 @@ void Sequential::save_checkpoint(const std::string& path, int epoch, double loss
       json_string(layer_defs, kv.first);
       layer_defs += ':' + std::to_string(kv.second);
     }
+    for (const auto& kv : l->config_reals()) {
+      if (!first) layer_defs += ',';
+      first = false;
+      json_string(layer_defs, kv.first);
+      layer_defs += ':' + json_number(kv.second);
+    }
     layer_defs += "}}";
     layer_data += "{\"weights\":{";
     const auto vars = l->variables();

@@ -183,6 +183,8 @@ struct Layer {
   // map its builder registers (nn/models/sequential_info.v:40-215), in insertion order
   virtual const char* type_name() const = 0;
   virtual std::vector<std::pair<std::string, int>> config() const { return {}; }
+  // and what of it is no whole number
+  virtual std::vector<std::pair<std::string, double>> config_reals() const { return {}; }
   // what a resumed run needs beside the weights; a checkpoint keeps it as decimal text (a JSON number holds 53 bits)
   virtual std::vector<std::pair<std::string, uint64_t*>> state() { return {}; }
 };
@@ -347,6 +349,7 @@ struct DropoutLayer : Layer {
   const char* type_name() const override { return "DropoutLayer"; }
   std::vector<std::pair<std::string, uint64_t*>> state() override { return {{"seed", &seed}, {"step", &step}}; }
   std::vector<std::pair<std::string, int>> config() const override { return {{"prob_millionths", (int)(p * 1e6 + 0.5)}}; }
+  std::vector<std::pair<std::string, double>> config_reals() const override { return {{"prob", p}}; }
 };
 
 // Table lookup: tokens [batch, ...] (whole numbers in an f32 tensor; anything else, as padding, gives a row of zeros)
@@ -365,6 +368,7 @@ struct EmbeddingLayer : Layer {
   const char* kind() const override { return "embedding"; }
   const char* type_name() const override { return "EmbeddingLayer"; }
   std::vector<std::pair<std::string, int>> config() const override { return {{"vocabulary", vocabulary}, {"dim", dim}}; }
+  std::vector<std::pair<std::string, double>> config_reals() const override { return {{"scale", scale}}; }
 
  private:
   VarPtr run(const VarPtr& input, const DropoutLayer::Mask& mask);
@@ -391,6 +395,7 @@ struct GroupNormLayer : Layer {
   std::vector<std::pair<std::string, int>> config() const override {
     return {{"num_groups", groups}, {"num_channels", channels}, {"activation", activation}};
   }
+  std::vector<std::pair<std::string, double>> config_reals() const override { return {{"eps", eps}}; }
 };
 
 // nn/types/loss.v:7-27, nn/loss/mse.v:30-41, nn/loss/softmax_cross_entropy.v
