@@ -1,0 +1,51 @@
+"""The V hooks (vtl_b200/vglue) read as text, since no V toolchain is at hand: what a compiler, or a leak, would show."""
+import glob
+import os
+import re
+
+import pytest
+
+VGLUE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "vtl_b200", "vglue")
+HOOKS = [f for f in sorted(glob.glob(os.path.join(VGLUE, "*_d_b200.v"))) if os.path.basename(f) != "c_d_b200.v"]
+FALLIBLE = r"\bs\.(?:as_tensor|upload|alloc|alloc_f32|resident|to_host)\("
+
+
+def code(path):
+    return re.sub(r"//[^\n]*", "", open(path).read())
+
+
+def functions(path):
+    """(name, signature, body) of each function of a file."""
+    src = code(path)
+    for m in re.finditer(r"^(?:pub )?fn (?:\([^)]*\) )?(\w+)\([^\n]*\{$", src, re.M):
+        end = src.index("\n}", m.end())
+        yield m.group(1), m.group(0), src[m.end():end]
+
+
+def call_end(text, start):
+    """The index behind the parenthesis that closes the one in front of `start`."""
+    depth = 1
+    for i in range(start, len(text)):
+        depth += {"(": 1, ")": -1}.get(text[i], 0)
+        if depth == 0:
+            return i + 1
+    raise AssertionError("unbalanced parentheses")
+
+
+def test_there_are_hooks():
+    names = {n for f in HOOKS for n, _, _ in functions(f)}
+    assert {"linear_forward_f32", "embedding_backward_f32", "groupnorm_forward_f32", "dropout_forward_f32"} <= names
+
+
+@pytest.mark.parametrize("path", HOOKS, ids=os.path.basename)
+def test_results_are_unwrapped(path):
+    """A call that may fail gives its value by `!`; only `return s.as_tensor(...)` of a function that returns one result
+    hands the result on as it is."""
+    for name, signature, body in functions(path):
+        for m in re.finditer(FALLIBLE, body):
+            end = call_end(body, m.end())
+            if body[end:end + 1] == "!":
+                continue
+            line = body[body.rfind("\n", 0, m.start()) + 1:body.find("\n", end) if "\n" in body[end:] else len(body)]
+            assert re.fullmatch(r"\s*return s\.as_tensor\(.*\)", line, re.S), (name, line)
+            assert re.search(r"\) !&vtl\.Tensor\[f32\] \{$", signature), name
