@@ -49,3 +49,25 @@ def test_results_are_unwrapped(path):
             line = body[body.rfind("\n", 0, m.start()) + 1:body.find("\n", end) if "\n" in body[end:] else len(body)]
             assert re.fullmatch(r"\s*return s\.as_tensor\(.*\)", line, re.S), (name, line)
             assert re.search(r"\) !&vtl\.Tensor\[f32\] \{$", signature), name
+
+
+# what a hook hands on to its caller instead of freeing it: the indices that the pooling's backward call frees, the codes of
+# a quantised layer
+HANDED_ON = {("maxpool2d_forward_f32", "didx"), ("new_quant_linear", "d_wq"), ("new_quant_linear", "d_sw")}
+
+
+@pytest.mark.parametrize("path", [f for f in HOOKS if "session" not in f], ids=os.path.basename)
+def test_buffers_are_freed(path):
+    """as_tensor copies to the host and takes nothing over: whatever a hook allocates or uploads it frees in a defer."""
+    for name, _, body in functions(path):
+        freed = set()
+        for m in re.finditer(r"\bdefer \{(.*?)\n\t\}", body, re.S):
+            block = m.group(1)
+            freed |= set(re.findall(r"s\.free\((\w+)\)", block))
+            for names in re.findall(r"for \w+ in \[([^\]]*)\]", block):
+                freed |= {n.strip() for n in names.split(",")}
+        for line in body.splitlines():
+            m = re.match(r"\s*([\w, ]+?) := (.*\bs\.(?:alloc|alloc_f32|upload)\(.*)", line)
+            if m:
+                for var in m.group(1).split(","):
+                    assert var.strip() in freed or (name, var.strip()) in HANDED_ON, (name, var.strip())
