@@ -71,3 +71,21 @@ def test_buffers_are_freed(path):
             if m:
                 for var in m.group(1).split(","):
                     assert var.strip() in freed or (name, var.strip()) in HANDED_ON, (name, var.strip())
+
+
+@pytest.mark.parametrize("path", HOOKS, ids=os.path.basename)
+def test_sizes_in_bytes_are_no_products_of_ints(path):
+    """An int holds less than 2 GiB: 2^30 elements of four bytes would come to no bytes at all.  Sizes are counted by alloc_f32,
+    from dimensions, or in usize."""
+    src = code(path)
+    for m in re.finditer(r"\bs\.alloc\(", src):
+        args = src[m.end():call_end(src, m.end()) - 1]
+        assert "*" not in args or all(f.strip().startswith("usize(") for f in args.split("*")) or args == "bytes", args
+    for m in re.finditer(r"usize\(", src):
+        args = src[m.end():call_end(src, m.end()) - 1]
+        assert not re.search(r"\*\s*4\b|\b4\s*\*", args), args
+    if path.endswith("session_d_b200.v"):
+        assert "pub fn (s &DeviceSession) alloc(bytes usize) !voidptr {" in src
+        assert "pub fn (s &DeviceSession) alloc_f32(dims ...int) !voidptr {" in src
+        total = src[src.index(") alloc_f32("):]
+        assert "usize(4)" in total and "*= usize(dim)" in total
