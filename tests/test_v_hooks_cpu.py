@@ -89,3 +89,14 @@ def test_sizes_in_bytes_are_no_products_of_ints(path):
         assert "pub fn (s &DeviceSession) alloc_f32(dims ...int) !voidptr {" in src
         total = src[src.index(") alloc_f32("):]
         assert "usize(4)" in total and "*= usize(dim)" in total
+
+
+def test_group_norm_takes_any_rank():
+    """[batch, channels] and [batch, ..., channels]: no hook of group norm indexes a fixed third dimension."""
+    path = os.path.join(VGLUE, "token_layers_d_b200.v")
+    bodies = {n: b for n, _, b in functions(path)}
+    for name in ("groupnorm_forward_f32", "groupnorm_backward_f32"):
+        assert "shape[2]" not in bodies[name] and "shape[1]" not in bodies[name], name
+        assert "norm_sizes(x.shape)!" in bodies[name], name
+    body = bodies["norm_sizes"]
+    assert "shape.len < 2" in body and "return error(" in body and "shape.last()" in body and "shape[1..shape.len - 1]" in body
