@@ -100,3 +100,12 @@ def test_group_norm_takes_any_rank():
         assert "norm_sizes(x.shape)!" in bodies[name], name
     body = bodies["norm_sizes"]
     assert "shape.len < 2" in body and "return error(" in body and "shape.last()" in body and "shape[1..shape.len - 1]" in body
+
+
+@pytest.mark.parametrize("path", HOOKS, ids=os.path.basename)
+def test_no_field_has_the_name_of_a_method(path):
+    src = code(path)
+    for m in re.finditer(r"struct (\w+) \{(.*?)\n\}", src, re.S):
+        fields = set(re.findall(r"^\t(\w+)\s+\S", m.group(2), re.M))
+        methods = set(re.findall(r"fn \((?:mut )?\w+ &?%s\) (\w+)\(" % m.group(1), src))
+        assert not fields & methods, (m.group(1), fields & methods)
