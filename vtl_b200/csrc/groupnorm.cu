@@ -348,8 +348,8 @@ __global__ void __launch_bounds__(kGnRowThreads, PER > 4 ? 1 : 2)
 // and of their squares (of the values themselves the variance would lose 2^-53 of the mean square, 1e-4 at a mean of 1e6),
 // rows that are asked for together by way of the first of them in f32; backward dz and dz * h.
 // Bound by HBM, 12 bytes per element forward, 20 backward, less what of x and g still lies in L2 for the second pass.
-// Ten samples of 20000 positions by one group of 64 channels: 35 us forward, 64 us backward, 4.4 and 4 TB/s of those bytes.
-// Sixty of 4000 by two groups of 31 (rows on no 16-byte boundary, one channel a load): 48 and 86 us, 3.7 and 3.5 TB/s.
+// Ten samples of 20000 positions by one group of 64 channels: 35 us forward, 55 us backward, 4.4 and 4.7 TB/s of those bytes.
+// Sixty of 4000 by two groups of 31 (rows on no 16-byte boundary, one channel a load): 42 and 71 us, 4.2 TB/s.
 constexpr int kRows = 256;  // positions per chunk, fewer where there would be too few CTAs
 
 struct GnGrid {
@@ -415,7 +415,15 @@ __global__ void __launch_bounds__(256) gn_sums_kernel(const float* x, const floa
       } else {
         if (r == start) {
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) first[k] = (double)x[(size_t)b * d.S * d.C + (c + k) / d.width * d.width];
+          for (int k = 0; k < VEC; ++k) first[k] = (double)x[(size_t)b * d.S * d.C + (d.G == 1 ? 0 : (c + k) / d.width * d.width)];
+        }
+        if (r + lanes >= r1) {  // one row
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            const double off = (double)vx[0].e[k] - first[k];
+            acc[k].x += off, acc[k].y = fma(off, off, acc[k].y);
+          }
+          break;
         }
         // Distances from the first of these rows, `off` from the group's.  (Where that row is far from the others, its
         // own distance from the mean counts for more than what theirs from it are rounded by.)
@@ -564,13 +572,13 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const float* x, const flo
 // x is read once: it stays in registers between the sums and the result (groupnorm_plan.h).  A cluster goes through
 // several units (a slab of groups of one sample), the next one's values on their way into shared memory while this
 // one's are worked on.  Bound by HBM, 8 bytes per element forward, 12 backward: with SiLU, 32 samples of 64 x 64 positions by
-// 512 channels forward in 91 to 94 us, 5.8 TB/s, 88 % of a plain copy's rate (the same loads and stores without the sums: 6.2
+// 512 channels forward in 95 to 96 us, 5.6 TB/s, 86 % of a plain copy's rate (the same loads and stores without the sums: 6.2
 // TB/s); 64 of 32 x 32 backward in 74 to 77 us, 5.3 TB/s (the barriers around the sums of a unit are not hidden with two
 // CTAs of 256 threads, all that their registers leave room for).  Forward 512 threads with sixteen pieces each: the
 // registers of a cluster of four hold 64 x 64 positions of 32 channels, 128 bytes of a row at a time.  Small maps are bound by
-// the host: two samples of 8 x 8 by 128 channels 6.4 us forward.  Channels that are no multiple of four come by 4-byte
-// cp.async: three samples of 17 x 19 by 330 channels backward in 8.6 us with both launches, latency throughout.
-// Groups whose width is no multiple of four keep sums per channel: 2.7 to 3.9 TB/s.
+// the host: two samples of 8 x 8 by 128 channels 6.5 us forward.  Channels that are no multiple of four come by 4-byte
+// cp.async: three samples of 17 x 19 by 330 channels backward in 8.4 to 9 us with both launches, latency throughout.
+// Groups whose width is no multiple of four keep sums per channel: 2.9 to 3.9 TB/s.
 struct GnTile {
   GnDims d;
   int groups, slabs, csplit, channels, rows;
