@@ -437,6 +437,8 @@ int vtlb_ids_from_f32(vtlb_ctx* ctx, const void* d_src, size_t n, void* d_ids_i3
  * rstd = 1 / sqrt(variance + eps) (biased), z = gamma[c] * h + beta[c] (NULL: 1 and 0), y = act(z): nothing, ReLU as
  * above, or SiLU z / (1 + exp(-z)).  groups = 1 and S = 1 is a layer norm over C.  d_mean and d_rstd [B, groups] receive
  * the statistics; the backward pass reads them, and x, and recomputes z.  d_y may be d_x where x is not needed again.
+ * However far from zero a group lies, its variance is that of the values; their distances from the mean are squared in
+ * f32, so they are to be below 1e17, and with eps = 0 those below 1e-18 may count as zero.
  * Backward, dz = g * act'(z): dgamma[c] = sum dz * h, dbeta[c] = sum dz over samples and positions,
  * dx = rstd * (gamma dz - mean(gamma dz) - h * mean(gamma dz h)), the means over the group; any output may be NULL,
  * d_dx may be d_g or d_x.  Other buffers may not overlap.  B * S and B * groups go to 2^31 - 1, S to 65535 * 256, C to

@@ -115,3 +115,21 @@ def test_groups_that_hardly_vary_beside_others(dev, B, S, C, G, kind):
     assert np.array_equal(mean.numpy(), stats[0]) and np.array_equal(rstd.numpy(), stats[1])
     for b in (d, dga, dbe, y, mean, rstd):
         b.free()
+
+
+@pytest.mark.parametrize("B,S,C,G", SHAPES)
+@pytest.mark.parametrize("size", [1e-18, 1.0, 1e17])
+def test_the_range_of_distances(dev, B, S, C, G, size):
+    """x = +-size in turn, eps = 0: y is the sign of x, or close to it where there is one more of either."""
+    sign = np.where(np.add.outer(np.arange(S), np.arange(C)) % 2, 1, -1)
+    x = np.ascontiguousarray(np.broadcast_to(sign, (B, S, C)), np.float32) * np.float32(size)
+    d = dev.to_device(x)
+    y, mean, rstd = dev.zeros(x.shape), dev.zeros((B, G)), dev.zeros((B, G))
+    dev.groupnorm_fwd_f32(d, B, S, C, G, None, None, 0.0, ref.NONE, y, mean, rstd)
+    want, wm, wr = ref.groupnorm(x, G, None, None, 0.0, ref.NONE)
+    # chains of at most 128 additions, each term rounded twice, its square three times; h three more
+    assert (np.abs(mean.numpy() - wm) <= 130 * U * size).all()
+    assert (np.abs(rstd.numpy() - wr) <= 70 * U * wr).all()
+    assert np.abs(y.numpy() - want).max() <= 210 * U
+    for b in (d, y, mean, rstd):
+        b.free()

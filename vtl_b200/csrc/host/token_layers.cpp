@@ -1,5 +1,7 @@
 // Host mirror of the layers of token models: EmbeddingLayer, DropoutLayer and GroupNormLayer (the reference's embedding
-// and dropout layers are host loops; group norm takes the place of its layer norm, which is one group).
+// and dropout layers are host loops).  Group norm takes its statistics over all positions of a sample, so one group of [batch,
+// channels] is a layer norm; of [batch, tokens, channels] it is not one per token, which
+// vtlb_groupnorm_fwd_f32 gives for batch * tokens samples of one position.
 #include <cmath>
 #include <cstring>
 

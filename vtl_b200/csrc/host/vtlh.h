@@ -55,7 +55,8 @@ int vtlh_model_avgpool2d(vtlh_model* m, int kh, int kw, int ph, int pw, int sh, 
 int vtlh_model_global_avgpool2d(vtlh_model* m);
 int vtlh_model_batchnorm1d(vtlh_model* m, int num_features, double eps, double momentum);
 /* embedding: tokens as whole numbers in an f32 tensor [batch, ...] (anything else is padding) -> [batch, ..., dim];
- * dropout: active in train_step, not in forward; groupnorm: channels last, activation 0 none, 1 ReLU, 2 SiLU */
+ * dropout: active in train_step, not in forward; groupnorm: channels last, statistics over all positions of a sample
+ * and the channels of a group, activation 0 none, 1 ReLU, 2 SiLU */
 int vtlh_model_embedding(vtlh_model* m, int vocabulary, int dim, double scale);
 int vtlh_model_dropout(vtlh_model* m, double p);
 int vtlh_model_groupnorm(vtlh_model* m, int groups, double eps, int activation);

@@ -218,7 +218,8 @@ class Model:
         _ck(self.lib.vtlh_model_dropout(self.h, float(p)))
 
     def groupnorm(self, groups, eps=1e-5, activation="none"):
-        """Channels last; activation "none", "relu" or "silu"."""
+        """Channels last, statistics over all positions of a sample (tokens, padding among them) and the channels of a
+        group; activation "none", "relu" or "silu"."""
         _ck(self.lib.vtlh_model_groupnorm(self.h, int(groups), float(eps), {"none": 0, "relu": 1, "silu": 2}[activation]))
 
     def dropout_state(self, dropout_index):
