@@ -791,15 +791,16 @@ __device__ __forceinline__ void gn_take(GnVec<VEC> (&v)[VPT], const float* slots
 
 // The groups of units that are marked by a negative rstd once more, each by one CTA, behind the barrier of the cluster: sums
 // in f64 of the distances from the mean that was found, so that a constant group's variance is zero but for 2^-53 of the
-// square of what that mean is rounded by.  x is still there: where y lies over it, marked units were not written.  Not
-// unrolled, so that the way that units take as a rule keeps its registers; the check for marks at a kernel's end is all that
-// it pays.
-template <int ACT, int T>
+// square of what that mean is rounded by.  x is still there: where y lies over it, marked units were not written.  It takes
+// no registers from the way that units take as a rule, which pays for the check at the kernel's end.  x is read twice more, four
+// pieces a thread at a time: 32 samples of 64 x 64 x 512 that are all marked 520 us (95 where none is; one piece at a time 1850).
+template <int ACT, int T, int V>
 __device__ __forceinline__ void gn_look_again(const float* x, const float* gamma, const float* beta, const GnTile& t, int rank, int ctas,
                                            double eps, float* y, float* mean_out, float* rstd_out, double2* sm) {
   __syncthreads();
   const int tid = threadIdx.x, W = t.d.width;
-  const int n = t.d.S * W;  // (at most what a cluster holds)
+  constexpr int U = 4;
+  const int cols = W / V, n = t.d.S * cols;  // pieces (at most what a cluster holds)
   const GnUnit stride = gn_first(t, gridDim.x / ctas);
   for (GnUnit u = gn_first(t, blockIdx.x / ctas); u.unit < t.units; u = gn_next(t, u, stride)) {
     for (int g = rank; g < gn_groups(t, u); g += ctas) {
@@ -808,10 +809,26 @@ __device__ __forceinline__ void gn_look_again(const float* x, const float* gamma
       const size_t base = gn_base(t, u) + (size_t)g * W;
       const double near = (double)*(volatile float*)&mean_out[k];
       double2 s = make_double2(0.0, 0.0);
+      const auto fetch = [&](GnVec<V>(&v)[U], int e0) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int e = e0 + i * T;
+          if (e < n) v[i] = gn_load<V>(x + base + (size_t)(e / cols) * t.d.C + e % cols * V);
+        }
+      };
 #pragma unroll 1
-      for (int e = tid; e < n; e += T) {
-        const double v = (double)x[base + (size_t)(e / W) * t.d.C + e % W] - near;
-        s.x += v, s.y = fma(v, v, s.y);
+      for (int e = tid; e < n; e += U * T) {
+        GnVec<V> v[U];
+        fetch(v, e);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          if (e + i * T >= n) break;
+#pragma unroll
+          for (int q = 0; q < V; ++q) {
+            const double far = (double)v[i].e[q] - near;
+            s.x += far, s.y = fma(far, far, s.y);
+          }
+        }
       }
 #pragma unroll
       for (int o = 16; o; o >>= 1) s.x += __shfl_xor_sync(~0u, s.x, o), s.y += __shfl_xor_sync(~0u, s.y, o);
@@ -820,17 +837,23 @@ __device__ __forceinline__ void gn_look_again(const float* x, const float* gamma
       s = sm[0];
 #pragma unroll 1
       for (int q = 1; q < T / 32; ++q) s.x += sm[q].x, s.y += sm[q].y;
-      const double off = s.x / (double)n, var = s.y / (double)n - off * off;
+      const double all = (double)n * V, off = s.x / all, var = s.y / all - off * off;
       const float mu = (float)(near + off), rs = inv_sqrt((var < 0.0 ? 0.0 : var) + eps);
       if (tid == 0) mean_out[k] = mu, rstd_out[k] = rs;
       const int c0 = ((int)u.slab * t.groups + g) * W;
 #pragma unroll 1
-      for (int e = tid; e < n; e += T) {
-        const int c = e % W;
-        const size_t at = base + (size_t)(e / W) * t.d.C + c;
-        GnVec<1> z;
-        z.e[0] = fmaf(x[at] - mu, gamma ? rs * gamma[c0 + c] : rs, beta ? beta[c0 + c] : 0.0f);
-        y[at] = act<ACT>(z).e[0];
+      for (int e0 = tid; e0 < n; e0 += U * T) {
+        GnVec<V> v[U];
+        fetch(v, e0);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int e = e0 + i * T, c = e % cols * V;
+          if (e >= n) break;
+#pragma unroll
+          for (int q = 0; q < V; ++q)
+            v[i].e[q] = fmaf(v[i].e[q] - mu, gamma ? rs * __ldg(gamma + c0 + c + q) : rs, beta ? __ldg(beta + c0 + c + q) : 0.0f);
+          gn_store<V>(y + base + (size_t)(e / cols) * t.d.C + c, act<ACT>(v[i]));
+        }
       }
       __syncthreads();
     }
@@ -901,8 +924,8 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
     // says by how much); from these in f64 the sums of x and x^2.  Of these the variance loses some 2^-53 of the mean
     // square: where that may be more than 2^-27 of variance and eps (a constant group of 30 at an eps of 1e-5), the unit is
     // left to gn_look_again.  (Sums of the distances from a value that all threads know lose nothing, but it has to
-    // be brought and subtracted for every unit: 26 samples of 129 x 896 by 16 groups 12.0 us, this way 11.6, sums without
-    // care 11.0; 32 of 64 x 64 x 512 98, 96 and 94.)
+    // be brought and subtracted for every unit: 26 samples of 129 x 896 by 16 groups 12.0 us, this way 11.6 to 11.9, sums
+    // without care 11.0; 32 of 64 x 64 x 512 96, 95 and 93.)
     double2 acc[PAIRS];
     {
       const float n = (float)(p.rows * PER), part_n = p.rows ? __fdividef(1.0f, n) : 0.0f;
@@ -1028,7 +1051,7 @@ __global__ void __launch_bounds__(kGnFwdThreads, VPT > 8 ? 512 / kGnFwdThreads :
   if (TMA || ctas > 1) ptx::report_abort(&mail.abort, status, VTLB_ST_NORM_TIMEOUT);  // whichever thread's wait it was
   if (TMA && p.any) gn_last_copies(mail);
   if (ctas > 1) cluster.sync();  // no CTA leaves while another may still send to it
-  if (__builtin_expect(sm_lost != ~0u, 0)) gn_look_again<ACT, T>(x, gamma, beta, t, (int)cluster.block_rank(), (int)cluster.num_blocks(), eps, y, mean_out, rstd_out, sm_pair);
+  if (__builtin_expect(sm_lost != ~0u, 0)) gn_look_again<ACT, T, GROUPED ? VEC : 1>(x, gamma, beta, t, (int)cluster.block_rank(), (int)cluster.num_blocks(), eps, y, mean_out, rstd_out, sm_pair);
 }
 
 // Backward.  The channel sums of each CTA go to `sums` [B * rsplit][C] (dz, dz * h) for gn_params_kernel.
