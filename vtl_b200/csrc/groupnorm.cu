@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const float* x, const flo
 // x is read once: it stays in registers between the sums and the result (groupnorm_plan.h).  A cluster goes through
 // several units (a slab of groups of one sample), the next one's values on their way into shared memory while this
 // one's are worked on.  Bound by HBM, 8 bytes per element forward, 12 backward: with SiLU, 32 samples of 64 x 64 positions by
-// 512 channels forward in 95 to 96 us, 5.6 TB/s, 86 % of a plain copy's rate (the same loads and stores without the sums: 6.2
+// 512 channels forward in 95 to 97 us, 5.6 TB/s, 86 % of a plain copy's rate (the same loads and stores without the sums: 6.2
 // TB/s); 64 of 32 x 32 backward in 74 to 77 us, 5.3 TB/s (the barriers around the sums of a unit are not hidden with two
 // CTAs of 256 threads, all that their registers leave room for).  Forward 512 threads with sixteen pieces each: the
 // registers of a cluster of four hold 64 x 64 positions of 32 channels, 128 bytes of a row at a time.  Small maps are bound by
